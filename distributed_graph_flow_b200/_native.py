@@ -30,6 +30,8 @@ ERR_UNSUPPORTED = 102
 F32 = 0
 BF16 = 1
 
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "sigmoid": 4}  # DGFX_ACT_*
+
 CALL_INDEX_DEVICE = (1 << 64) - 1  # DGFX_CALL_INDEX_DEVICE
 
 MODE_RANDOM = 0
@@ -102,6 +104,16 @@ SIGNATURES = {
     "dgfx_segment_softmax": (_int, [_vp, _i32, _vp, _int, _i64, _vp, _i64, _i64, _i32, _vp, _int, _vp, _sz, _vp]),
     "dgfx_dense_concat_bf16": (_int, [_vp, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i32, _vp, _vp]),
     "dgfx_dense_check": (_int, [_vp]),
+    "dgfx_segment_group_norm_workspace_size": (_int, [_i64, _i64, _i64, _i64, _int, _i32, ctypes.POINTER(_sz)]),
+    "dgfx_segment_group_norm": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _i64, _vp, _vp, ctypes.c_float, _i32, _vp, _vp,
+                                       _vp, _vp, _sz, _vp]),
+    "dgfx_segment_group_norm_backward": (_int, [_vp, _vp, _int, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i32,
+                                                _vp, _vp, _vp, _vp, _sz, _vp]),
+    "dgfx_gated_scan_workspace_size": (_int, [_i64, _i64, ctypes.POINTER(_sz), ctypes.POINTER(_sz)]),
+    "dgfx_gated_scan": (_int, [_vp, _vp, _int, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "dgfx_gated_scan_backward": (_int, [_vp, _vp, _int, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                                        _sz, _vp]),
+    "dgfx_gated_scan_step": (_int, [_vp, _vp, _int, _i64, _i64, _vp, _vp, _vp, _vp]),
     "dgfx_halo_partition_workspace_size": (_int, [_i64, _i32, ctypes.POINTER(_sz)]),
     "dgfx_halo_partition": (_int, [_vp, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _sz, _vp]),
     "dgfx_gather_rows_local": (_int, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp]),

@@ -320,3 +320,266 @@ def batch_mean_aggregate(batch, features, out=None, stream=None):
         _native.ptr(batch.edge_dst), int(batch.B), cap, _native.ptr(features), _dtype_code(features.dtype), F,
         _native.ptr(out), _native.stream_handle(stream)))
     return out
+
+
+# ---------------------------------------------------------------------------
+# Layer operators around the aggregation: group norm over the segments of a
+# merged batch, gated recurrence over ragged windows.
+# ---------------------------------------------------------------------------
+def _activation_code(who: str, activation: str) -> int:
+    if activation not in _native.ACTIVATIONS:
+        raise ValueError(f"{who}: unknown activation {activation!r}; expected one of {sorted(_native.ACTIVATIONS)}")
+    return _native.ACTIVATIONS[activation]
+
+
+def _layer_input(who: str, name: str, t, shape, dtypes) -> int:
+    """Checks one operand (type, shape with None for any extent, contiguity)
+    and returns its dtype code."""
+    import torch
+
+    codes = {torch.float32: _native.F32, torch.bfloat16: _native.BF16}
+    allowed = [d for d in codes if d in dtypes]
+    if t.dtype not in allowed:
+        raise ValueError(f"{who}: {name} must be " + " or ".join(str(a).replace("torch.", "") for a in allowed))
+    if t.dim() != len(shape) or any(w is not None and int(n) != int(w) for n, w in zip(t.shape, shape)):
+        want = ", ".join("any" if w is None else str(int(w)) for w in shape)
+        raise ValueError(f"{who}: {name} is {list(t.shape)}, expected [{want}]")
+    if not t.is_contiguous():
+        raise ValueError(f"{who}: {name} must be contiguous")
+    return codes[t.dtype]
+
+
+def _layer_offsets(who: str, offsets) -> int:
+    """Checks segment offsets (int64 [segments + 1]) and returns the number of segments."""
+    import torch
+
+    if offsets.dtype != torch.int64 or offsets.dim() != 1 or int(offsets.numel()) < 1 or not offsets.is_contiguous():
+        raise ValueError(f"{who}: offsets must be a contiguous int64 vector of segments + 1 values")
+    return int(offsets.numel()) - 1
+
+
+class _LayerLaunch:
+    """Device and stream of one call: every operand on one CUDA device, which
+    becomes the current one; allocations inside belong to the call's stream,
+    and operands used on a stream other than the current one are recorded on
+    it, so that their memory is not handed out while the call still runs."""
+
+    def __init__(self, who: str, stream, *operands):
+        torch = _native.require_cuda()
+        operands = [t for t in operands if t is not None]
+        self.device = operands[0].device
+        if self.device.type != "cuda" or any(t.device != self.device for t in operands):
+            raise ValueError(f"{who}: all tensors must be on one CUDA device, got "
+                             + ", ".join(sorted({str(t.device) for t in operands})))
+        self._guards = []
+        if self.device.index != torch.cuda.current_device():
+            self._guards.append(torch.cuda.device(self.device))
+        self._stream = stream
+        self._operands = operands
+
+    def __enter__(self) -> int:
+        import torch
+
+        for g in self._guards:
+            g.__enter__()
+        current = torch.cuda.current_stream()
+        if self._stream is None or self._stream == current:
+            return int(current.cuda_stream)
+        if self._stream.device != self.device:
+            for g in reversed(self._guards):
+                g.__exit__(None, None, None)
+            raise ValueError(f"the stream belongs to {self._stream.device}, the tensors to {self.device}")
+        for t in self._operands:
+            t.record_stream(self._stream)
+        inner = torch.cuda.stream(self._stream)
+        inner.__enter__()
+        self._guards.append(inner)
+        return int(self._stream.cuda_stream)
+
+    def __exit__(self, *exc):
+        for g in reversed(self._guards):
+            g.__exit__(*exc)
+        return False
+
+
+def _layer_workspace(device, nbytes: int):
+    import torch
+
+    return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
+
+
+def segment_group_norm(x, offsets, groups: int, weight=None, bias=None, eps: float = 1e-5, activation: str = "none",
+                       stream=None):
+    """Group norm with an activation over ragged segments, channels last:
+    every segment (rows offsets[s] .. offsets[s+1] of x, e.g. the graphs of a
+    merged batch with offsets = its node_offsets) and every group of C /
+    ``groups`` adjacent channels is normalised by its own mean and biased
+    variance, y = act((x - mean) * rstd * weight + bias). With one segment per
+    graph this is the per-graph norm of a GNN layer; with groups = C an
+    instance norm, with groups = 1 and one row per segment a layer norm.
+
+    x [rows, C] float32 / bfloat16 (rows a multiple of 16 bytes, at most
+    4096), offsets int64 [segments + 1] ascending, on the device (no host
+    synchronisation), weight and bias float32 [C] or None, activation one of
+    none, relu, silu, gelu (erf form), sigmoid. Rows outside of every segment
+    (a merged batch's spare capacity) give zeros and are never used, whatever they
+    hold. Returns (y, mean, rstd); mean and rstd, float32 [segments, groups],
+    are what ``segment_group_norm_backward`` takes."""
+    import torch
+
+    who = "segment_group_norm"
+    code = _layer_input(who, "x", x, (None, None), (torch.float32, torch.bfloat16))
+    rows, channels = int(x.shape[0]), int(x.shape[1])
+    nseg = _layer_offsets(who, offsets)
+    act = _activation_code(who, activation)
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None:
+            _layer_input(who, name, t, (channels,), (torch.float32,))
+    lib = _native.lib()
+    need = ctypes.c_size_t()
+    _native.check(lib.dgfx_segment_group_norm_workspace_size(rows, channels, int(groups), nseg, code, 0,
+                                                             ctypes.byref(need)))
+    if not eps > 0:
+        raise ValueError(f"{who}: eps must be positive")
+    with _LayerLaunch(who, stream, x, offsets, weight, bias) as sh:
+        y = torch.empty_like(x)
+        mean = torch.empty((nseg, int(groups)), dtype=torch.float32, device=x.device)
+        rstd = torch.empty_like(mean)
+        ws = _layer_workspace(x.device, need.value)
+        _native.check(lib.dgfx_segment_group_norm(
+            _native.ptr(x), code, rows, channels, int(groups), _native.ptr(offsets), nseg, _native.ptr(weight),
+            _native.ptr(bias), float(eps), act, _native.ptr(y), _native.ptr(mean), _native.ptr(rstd), _native.ptr(ws),
+            need.value, sh))
+    return y, mean, rstd
+
+
+def segment_group_norm_backward(grad, x, offsets, mean, rstd, weight=None, bias=None, activation: str = "none",
+                                stream=None):
+    """Gradients of ``segment_group_norm``: (dx, dweight, dbias) from the
+    gradient of y, the forward inputs and the returned mean and rstd. dx has
+    x's type, dweight and dbias are float32 sums over all segments (None for
+    a weight or bias that is None), in a fixed order. Rows outside of every
+    segment get zeros, and what grad holds there is not used."""
+    import torch
+
+    who = "segment_group_norm_backward"
+    code = _layer_input(who, "x", x, (None, None), (torch.float32, torch.bfloat16))
+    rows, channels = int(x.shape[0]), int(x.shape[1])
+    _layer_input(who, "grad", grad, x.shape, (x.dtype,))
+    nseg = _layer_offsets(who, offsets)
+    act = _activation_code(who, activation)
+    _layer_input(who, "mean", mean, (nseg, None), (torch.float32,))
+    groups = int(mean.shape[1])
+    _layer_input(who, "rstd", rstd, (nseg, groups), (torch.float32,))
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None:
+            _layer_input(who, name, t, (channels,), (torch.float32,))
+    lib = _native.lib()
+    need = ctypes.c_size_t()
+    _native.check(lib.dgfx_segment_group_norm_workspace_size(rows, channels, groups, nseg, code, 1,
+                                                             ctypes.byref(need)))
+    with _LayerLaunch(who, stream, grad, x, offsets, mean, rstd, weight, bias) as sh:
+        dx = torch.empty_like(x)
+        dw = None if weight is None else torch.empty_like(weight)
+        db = None if bias is None else torch.empty_like(bias)
+        ws = _layer_workspace(x.device, need.value)
+        _native.check(lib.dgfx_segment_group_norm_backward(
+            _native.ptr(grad), _native.ptr(x), code, rows, channels, groups, _native.ptr(offsets), nseg,
+            _native.ptr(mean), _native.ptr(rstd), _native.ptr(weight), _native.ptr(bias), act, _native.ptr(dx),
+            _native.ptr(dw), _native.ptr(db), _native.ptr(ws), need.value, sh))
+    return dx, dw, db
+
+
+def _scan_sizes(rows: int, channels: int):
+    need, saved = ctypes.c_size_t(), ctypes.c_size_t()
+    _native.check(_native.lib().dgfx_gated_scan_workspace_size(rows, channels, ctypes.byref(need),
+                                                               ctypes.byref(saved)))
+    return need.value, saved.value // 4
+
+
+def gated_scan(x, gate, offsets, initial=None, return_sequence: bool = True, return_saved: bool = False, stream=None):
+    """Gated linear recurrence over ragged windows (e.g. the causal windows
+    of sampled nodes' time series): per channel and segment,
+
+        a_t = sigmoid(gate_t),  h_t = a_t h_{t-1} + (1 - a_t) x_t.
+
+    x and gate [rows, C] float32 / bfloat16 (C a multiple of 4), offsets int64
+    [segments + 1] ascending, on the device; initial float32 [segments, C] is
+    the state before each segment's first row (None: zeros). Returns (h,
+    final): h [rows, C] in x's type, zeros in rows outside of every segment
+    (whose inputs are never used), and final float32 [segments, C], the state
+    after each segment's last row (its initial state if it has no rows).
+    States are float32 throughout. return_sequence=False skips h (returned as
+    None); return_saved=True appends what ``gated_scan_backward`` takes."""
+    import torch
+
+    who = "gated_scan"
+    code = _layer_input(who, "x", x, (None, None), (torch.float32, torch.bfloat16))
+    rows, channels = int(x.shape[0]), int(x.shape[1])
+    _layer_input(who, "gate", gate, x.shape, (x.dtype,))
+    nseg = _layer_offsets(who, offsets)
+    if initial is not None:
+        _layer_input(who, "initial", initial, (nseg, channels), (torch.float32,))
+    need, saved_n = _scan_sizes(rows, channels)
+    with _LayerLaunch(who, stream, x, gate, offsets, initial) as sh:
+        h = torch.empty_like(x) if return_sequence else None
+        final = torch.empty((nseg, channels), dtype=torch.float32, device=x.device)
+        saved = torch.empty(saved_n, dtype=torch.float32, device=x.device) if return_saved else None
+        ws = _layer_workspace(x.device, need)
+        _native.check(_native.lib().dgfx_gated_scan(
+            _native.ptr(x), _native.ptr(gate), code, rows, channels, _native.ptr(offsets), nseg, _native.ptr(initial),
+            _native.ptr(h), _native.ptr(final), _native.ptr(saved), _native.ptr(ws), need, sh))
+    return (h, final, saved) if return_saved else (h, final)
+
+
+def gated_scan_backward(grad, x, gate, offsets, saved, initial=None, grad_final=None, stream=None):
+    """Gradients of ``gated_scan``: (dx, dgate, dinitial) from the gradients
+    of h (None: zeros) and of final (None: zeros), the forward inputs and
+    ``saved``. dinitial is None where initial is. Rows outside of every
+    segment get zeros."""
+    import torch
+
+    who = "gated_scan_backward"
+    code = _layer_input(who, "x", x, (None, None), (torch.float32, torch.bfloat16))
+    rows, channels = int(x.shape[0]), int(x.shape[1])
+    _layer_input(who, "gate", gate, x.shape, (x.dtype,))
+    if grad is not None:
+        _layer_input(who, "grad", grad, x.shape, (x.dtype,))
+    nseg = _layer_offsets(who, offsets)
+    for name, t in (("initial", initial), ("grad_final", grad_final)):
+        if t is not None:
+            _layer_input(who, name, t, (nseg, channels), (torch.float32,))
+    need, saved_n = _scan_sizes(rows, channels)
+    _layer_input(who, "saved", saved, (saved_n,), (torch.float32,))
+    with _LayerLaunch(who, stream, x, grad, gate, offsets, saved, initial, grad_final) as sh:
+        dx, dgate = torch.empty_like(x), torch.empty_like(gate)
+        dinitial = None if initial is None else torch.empty_like(initial)
+        ws = _layer_workspace(x.device, need)
+        _native.check(_native.lib().dgfx_gated_scan_backward(
+            _native.ptr(x), _native.ptr(gate), code, rows, channels, _native.ptr(offsets), nseg, _native.ptr(initial),
+            _native.ptr(saved), _native.ptr(grad), _native.ptr(grad_final), _native.ptr(dx), _native.ptr(dgate),
+            _native.ptr(dinitial), _native.ptr(ws), need, sh))
+    return dx, dgate, dinitial
+
+
+def gated_scan_step(x, gate, state, out_state=None, stream=None):
+    """One step of ``gated_scan`` for n independent sequences (online use):
+    state' = a state + (1 - a) x with a = sigmoid(gate). x and gate [n, C],
+    state float32 [n, C]; returns (h, state'), h in x's type. out_state may be
+    ``state`` itself, which is then updated in place."""
+    import torch
+
+    who = "gated_scan_step"
+    code = _layer_input(who, "x", x, (None, None), (torch.float32, torch.bfloat16))
+    n, channels = int(x.shape[0]), int(x.shape[1])
+    _layer_input(who, "gate", gate, x.shape, (x.dtype,))
+    _layer_input(who, "state", state, (n, channels), (torch.float32,))
+    if out_state is not None:
+        _layer_input(who, "out_state", out_state, (n, channels), (torch.float32,))
+    with _LayerLaunch(who, stream, x, gate, state, out_state) as sh:
+        h = torch.empty_like(x)
+        new_state = torch.empty_like(state) if out_state is None else out_state
+        _native.check(_native.lib().dgfx_gated_scan_step(
+            _native.ptr(x), _native.ptr(gate), code, n, channels, _native.ptr(state), _native.ptr(h),
+            _native.ptr(new_state), sh))
+    return h, new_state

@@ -32,7 +32,8 @@ NVCC_FLAGS = ARCH + [
     f"-I{INCLUDE}",
 ]
 SOURCES = ["capi.cu", "primitives.cu", "csr_build.cu", "sampler.cu", "aggregate.cu", "halo.cu", "peer.cu", "synth.cu",
-           "transform.cu", "dense.cu", "subgraph.cu", "negatives.cu", "idmap.cu", "timeseries.cu", "sparse_ops.cu"]
+           "transform.cu", "dense.cu", "subgraph.cu", "negatives.cu", "idmap.cu", "timeseries.cu", "sparse_ops.cu",
+           "segment_norm.cu", "gated_scan.cu"]
 
 
 def nvcc() -> str:

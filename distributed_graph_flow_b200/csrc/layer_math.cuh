@@ -1,0 +1,115 @@
+// Device helpers shared by the layer operators (gated dense, segment group
+// norm, gated scan): activations with their derivatives, 16-byte vectors of
+// fp32 / bf16 as fp32 values, and the ragged-segment lookup.
+#pragma once
+
+#include <cuda_bf16.h>
+
+#include "common.cuh"
+
+namespace dgfx {
+
+// 1 / (1 + e^-z) without overflow at either end: e^-z = inf gives 0.
+__device__ __forceinline__ float sigmoid_f(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
+
+// Activations (DGFX_ACT_*) and their derivatives in fp32. gelu is the exact
+// form z Phi(z) = z (1 + erf(z / sqrt 2)) / 2. relu'(0) = 0. relu compares
+// instead of taking a maximum, so that NaN passes through.
+template <int ACT>
+__device__ __forceinline__ float act_f(float z) {
+  if (ACT == DGFX_ACT_RELU) return z < 0.0f ? 0.0f : z;
+  if (ACT == DGFX_ACT_SILU) return z * sigmoid_f(z);
+  if (ACT == DGFX_ACT_GELU) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+  if (ACT == DGFX_ACT_SIGMOID) return sigmoid_f(z);
+  return z;
+}
+
+// act(z) and act'(z) together (they share the exponential).
+template <int ACT>
+__device__ __forceinline__ void act_both_f(float z, float* value, float* slope) {
+  if (ACT == DGFX_ACT_RELU) {
+    *value = z < 0.0f ? 0.0f : z;
+    *slope = z > 0.0f ? 1.0f : 0.0f;
+  } else if (ACT == DGFX_ACT_SILU) {
+    const float s = sigmoid_f(z);
+    *value = z * s;
+    *slope = s * (1.0f + z * (1.0f - s));
+  } else if (ACT == DGFX_ACT_GELU) {
+    const float cdf = 0.5f + 0.5f * erff(z * 0.70710678118654752f);
+    *value = z * cdf;
+    *slope = cdf + z * 0.39894228040143268f * __expf(-0.5f * z * z);
+  } else if (ACT == DGFX_ACT_SIGMOID) {
+    const float s = sigmoid_f(z);
+    *value = s;
+    *slope = s * (1.0f - s);
+  } else {
+    *value = z;
+    *slope = 1.0f;
+  }
+}
+
+// 16 bytes of T as fp32 values.
+template <class T>
+struct Vec16;
+template <>
+struct Vec16<float> {
+  static constexpr int N = 4;
+  __device__ static __forceinline__ void unpack(const uint4& r, float (&f)[4]) {
+    f[0] = __uint_as_float(r.x);
+    f[1] = __uint_as_float(r.y);
+    f[2] = __uint_as_float(r.z);
+    f[3] = __uint_as_float(r.w);
+  }
+  __device__ static __forceinline__ uint4 pack(const float (&f)[4]) {
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  }
+};
+template <>
+struct Vec16<__nv_bfloat16> {
+  static constexpr int N = 8;
+  __device__ static __forceinline__ void unpack(const uint4& r, float (&f)[8]) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      f[2 * q] = __uint_as_float(w[q] << 16);
+      f[2 * q + 1] = __uint_as_float(w[q] & 0xFFFF0000u);
+    }
+  }
+  __device__ static __forceinline__ uint4 pack(const float (&f)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * q], f[2 * q + 1]);
+      w[q] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+
+// First segment whose end lies past `row` (nseg if none): every lane of the
+// warp probes one of 32 evenly spaced ends per round, so the search takes
+// ceil(log32) dependent loads. Call from a full warp; all lanes get it.
+__device__ __forceinline__ int64_t warp_first_segment(const int64_t* __restrict__ off, int64_t nseg, int64_t row) {
+  const int lane = threadIdx.x & 31;
+  int64_t lo = 0, hi = nseg;  // the answer lies in [lo, hi]
+  while (hi > lo) {
+    const int64_t step = (hi - lo + 31) >> 5;
+    const int64_t p = lo + step * (lane + 1) - 1;  // last index of this lane's part
+    const bool past = p >= hi || off[p + 1] > row;
+    const unsigned m = __ballot_sync(0xffffffffu, past);
+    const int k = m == 0u ? 32 : __ffs(static_cast<int>(m)) - 1;
+    const int64_t nlo = lo + step * k;
+    const int64_t nhi = lo + step * (k + 1) - 1;
+    lo = nlo < hi ? nlo : hi;
+    hi = nhi < hi ? nhi : hi;
+  }
+  return lo;
+}
+
+__host__ __device__ __forceinline__ int64_t clamp64(int64_t v, int64_t lo, int64_t hi) {
+  return v < lo ? lo : (v > hi ? hi : v);
+}
+
+inline bool ptr_aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+}  // namespace dgfx

@@ -45,6 +45,15 @@ enum {
 
 enum { DGFX_F32 = 0, DGFX_BF16 = 1 };
 
+/* Activations of the layer operators. GELU is the exact (erf) form. */
+enum {
+  DGFX_ACT_NONE = 0,
+  DGFX_ACT_RELU = 1,
+  DGFX_ACT_SILU = 2,
+  DGFX_ACT_GELU = 3,
+  DGFX_ACT_SIGMOID = 4
+};
+
 /* Sampling modes. RANDOM and FIRST are the reference's two modes
  * (create_sampler(debug_sampling=False/True), in_memory_sampler.py:349-363,
  * applied in SampleBuilder::RecursiveGrow, in_memory_sampler_ext.cc:250-279).
@@ -335,6 +344,75 @@ int dgfx_dense_concat_bf16(const void* d_x1, int64_t k1, const void* d_x2,
                            const float* d_bias, int64_t n, int32_t relu,
                            void* d_y, dgfx_stream stream);
 int dgfx_dense_check(dgfx_stream stream);
+
+/* ------------------------------------------------------------------------
+ * Group norm with an activation over ragged segments, channels last (for
+ * instance the graphs of a merged batch: d_offsets = its node_offsets).
+ * Segment s is rows d_offsets[s] .. d_offsets[s+1] of d_x [rows, channels]
+ * (dtype; ascending offsets, int64 [nseg + 1], read on the device and clamped
+ * to [0, rows]); group g is channels / groups adjacent channels. Over the
+ * values of (s, g): mean, rstd = 1 / sqrt(biased variance + eps);
+ *   d_y = act((x - mean) * rstd * d_weight[c] + d_bias[c])
+ * with act a DGFX_ACT_*; d_weight, d_bias fp32 [channels] or NULL (1 and 0).
+ * d_mean, d_rstd fp32 [nseg, groups] are outputs that the backward call
+ * reads (0 and 1 / sqrt(eps) for a segment without rows). Rows outside of every
+ * segment are written as zeros, and what they hold is not used. Sums are fp32 around
+ * the mean, in a fixed order. Rows are a multiple of 16 bytes and at most
+ * 4096 bytes; d_x, d_y, d_dy, d_dx 16-byte aligned and contiguous.
+ * The backward call gives d_dx (dtype) and, where not NULL, d_dweight and
+ * d_dbias (fp32 [channels], sums over all segments).
+ * ------------------------------------------------------------------------ */
+int dgfx_segment_group_norm_workspace_size(int64_t rows, int64_t channels, int64_t groups,
+                                           int64_t nseg, int dtype, int32_t backward,
+                                           size_t* bytes);
+int dgfx_segment_group_norm(const void* d_x, int dtype, int64_t rows, int64_t channels,
+                            int64_t groups, const int64_t* d_offsets, int64_t nseg,
+                            const float* d_weight, const float* d_bias, float eps,
+                            int32_t activation, void* d_y, float* d_mean, float* d_rstd,
+                            void* d_workspace, size_t workspace_bytes, dgfx_stream stream);
+int dgfx_segment_group_norm_backward(const void* d_dy, const void* d_x, int dtype, int64_t rows,
+                                     int64_t channels, int64_t groups, const int64_t* d_offsets,
+                                     int64_t nseg, const float* d_mean, const float* d_rstd,
+                                     const float* d_weight, const float* d_bias,
+                                     int32_t activation, void* d_dx, float* d_dweight,
+                                     float* d_dbias, void* d_workspace, size_t workspace_bytes,
+                                     dgfx_stream stream);
+
+/* ------------------------------------------------------------------------
+ * Gated linear recurrence over ragged windows (for instance the packed
+ * windows of dgfx_gather_segments), per channel:
+ *   a_t = sigmoid(gate_t),  h_t = a_t h_{t-1} + (1 - a_t) x_t
+ * down the rows of every segment (offsets as for the group norm). The state
+ * before a segment's first row is d_initial[s] (fp32 [nseg, channels], NULL:
+ * zeros); d_final[s] (fp32, may be NULL) is the state after its last row
+ * (the initial state of a segment without rows). d_h [rows, channels] (dtype; may be
+ * NULL when only the final states are wanted) gets every h_t, zeros in the
+ * rows outside of every segment. States are fp32. d_saved (may be NULL) is
+ * what the backward call needs: saved_bytes of
+ * dgfx_gated_scan_workspace_size. channels a multiple of 4; d_x, d_gate, d_h
+ * aligned to 4 elements.
+ * Backward: d_grad_h (dtype, NULL: zeros) and d_grad_final (fp32, NULL:
+ * zeros) to d_dx, d_dgate (dtype; zeros outside of the segments) and
+ * d_dinitial (fp32, may be NULL).
+ * dgfx_gated_scan_step is one step of n independent sequences:
+ * d_new_state [n, channels] (fp32; may be d_state itself) and the same values
+ * in dtype in d_h.
+ * ------------------------------------------------------------------------ */
+int dgfx_gated_scan_workspace_size(int64_t rows, int64_t channels, size_t* workspace_bytes,
+                                   size_t* saved_bytes);
+int dgfx_gated_scan(const void* d_x, const void* d_gate, int dtype, int64_t rows,
+                    int64_t channels, const int64_t* d_offsets, int64_t nseg,
+                    const float* d_initial, void* d_h, float* d_final, float* d_saved,
+                    void* d_workspace, size_t workspace_bytes, dgfx_stream stream);
+int dgfx_gated_scan_backward(const void* d_x, const void* d_gate, int dtype, int64_t rows,
+                             int64_t channels, const int64_t* d_offsets, int64_t nseg,
+                             const float* d_initial, const float* d_saved, const void* d_grad_h,
+                             const float* d_grad_final, void* d_dx, void* d_dgate,
+                             float* d_dinitial, void* d_workspace, size_t workspace_bytes,
+                             dgfx_stream stream);
+int dgfx_gated_scan_step(const void* d_x, const void* d_gate, int dtype, int64_t n,
+                         int64_t channels, const float* d_state, void* d_h,
+                         float* d_new_state, dgfx_stream stream);
 
 /* ------------------------------------------------------------------------
  * Halo feature exchange (node-range-partitioned features across ranks).
