@@ -104,6 +104,10 @@ SIGNATURES = {
     "dgfx_segment_softmax": (_int, [_vp, _i32, _vp, _int, _i64, _vp, _i64, _i64, _i32, _vp, _int, _vp, _sz, _vp]),
     "dgfx_dense_concat_bf16": (_int, [_vp, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i32, _vp, _vp]),
     "dgfx_dense_check": (_int, [_vp]),
+    "dgfx_gated_dense_concat_bf16": (_int, [_vp, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i32, _vp, _vp]),
+    "dgfx_gated_dense_concat_backward_workspace_size": (_int, [_i64, _i64, _i64, _i64, ctypes.POINTER(_sz)]),
+    "dgfx_gated_dense_concat_backward_bf16": (_int, [_vp, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i32, _vp,
+                                                     _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "dgfx_segment_group_norm_workspace_size": (_int, [_i64, _i64, _i64, _i64, _int, _i32, ctypes.POINTER(_sz)]),
     "dgfx_segment_group_norm": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _i64, _vp, _vp, ctypes.c_float, _i32, _vp, _vp,
                                        _vp, _vp, _sz, _vp]),

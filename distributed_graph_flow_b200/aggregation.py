@@ -323,8 +323,8 @@ def batch_mean_aggregate(batch, features, out=None, stream=None):
 
 
 # ---------------------------------------------------------------------------
-# Layer operators around the aggregation: group norm over the segments of a
-# merged batch, gated recurrence over ragged windows.
+# Layer operators around the aggregation: gated dense layer, group norm over
+# the segments of a merged batch, gated recurrence over ragged windows.
 # ---------------------------------------------------------------------------
 def _activation_code(who: str, activation: str) -> int:
     if activation not in _native.ACTIVATIONS:
@@ -406,6 +406,92 @@ def _layer_workspace(device, nbytes: int):
     import torch
 
     return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
+
+
+def _gated_operands(who: str, x1, x2, w_gate, w_up, b_gate, b_up):
+    """Checks the operands of the gated dense layer; (m, k1, k2, n)."""
+    import torch
+
+    bf16 = (torch.bfloat16,)
+    _layer_input(who, "x1", x1, (None, None), bf16)
+    m, k1 = int(x1.shape[0]), int(x1.shape[1])
+    k2 = 0
+    if x2 is not None:
+        _layer_input(who, "x2", x2, (m, None), bf16)
+        k2 = int(x2.shape[1])
+    _layer_input(who, "w_gate", w_gate, (None, k1 + k2), bf16)
+    n = int(w_gate.shape[0])
+    _layer_input(who, "w_up", w_up, (n, k1 + k2), bf16)
+    for name, t in (("b_gate", b_gate), ("b_up", b_up)):
+        if t is not None:
+            _layer_input(who, name, t, (n,), (torch.float32,))
+    return m, k1, k2, n
+
+
+def gated_dense_concat(x1, x2, w_gate, w_up, b_gate=None, b_up=None, activation: str = "silu", out=None, stream=None):
+    """act(X @ w_gate.T + b_gate) * (X @ w_up.T + b_up) with X = concat[x1,
+    x2] on the tensor cores: the gated form of the dense update after the
+    aggregation (``dense_concat``). Both projections, the activation and the product run in one
+    kernel; neither the concat nor the projections are written to memory.
+
+    x1 [M, K1], x2 [M, K2] or None, w_gate and w_up [N, K1 + K2] (torch Linear
+    layout) bfloat16, biases float32 [N] or None; K1, K2 and N multiples of 8;
+    contiguous. activation: silu, gelu (erf form), relu, sigmoid or none. fp32
+    accumulation, one rounding to bfloat16. ``dense_check`` reports pipeline
+    timeouts of this call too."""
+    import torch
+
+    who = "gated_dense_concat"
+    m, k1, k2, n = _gated_operands(who, x1, x2, w_gate, w_up, b_gate, b_up)
+    act = _activation_code(who, activation)
+    if out is not None:
+        _layer_input(who, "out", out, (m, n), (torch.bfloat16,))
+    _gated_sizes(k1, k2, m, n)
+    with _LayerLaunch(who, stream, x1, x2, w_gate, w_up, b_gate, b_up, out) as sh:
+        if out is None:
+            out = torch.empty((m, n), dtype=torch.bfloat16, device=x1.device)
+        _native.check(_native.lib().dgfx_gated_dense_concat_bf16(
+            _native.ptr(x1), k1, _native.ptr(x2), k2, m, _native.ptr(w_gate), _native.ptr(w_up), _native.ptr(b_gate),
+            _native.ptr(b_up), n, act, _native.ptr(out), sh))
+    return out
+
+
+def _gated_sizes(k1: int, k2: int, m: int, n: int) -> int:
+    need = ctypes.c_size_t()
+    _native.check(_native.lib().dgfx_gated_dense_concat_backward_workspace_size(k1, k2, m, n, ctypes.byref(need)))
+    return need.value
+
+
+def gated_dense_concat_backward(grad, x1, x2, w_gate, w_up, b_gate=None, b_up=None, activation: str = "silu",
+                                need_input: bool = True, need_weight: bool = True, stream=None):
+    """Gradients of ``gated_dense_concat``: (dx1, dx2, dw_gate, dw_up, db_gate,
+    db_up) from the gradient of its output (bfloat16 [M, N]) and its inputs;
+    None where the input is None. The projections are computed again instead
+    of being kept, and the gradients of the two projections (2 M N values of
+    workspace) are rounded to bfloat16 once, as operands of the products that
+    follow; the bias gradients (float32) are summed before that rounding.
+    need_input=False skips dx1 and dx2, need_weight=False dw_gate and dw_up
+    (returned as None). Sums run in a fixed order."""
+    import torch
+
+    who = "gated_dense_concat_backward"
+    m, k1, k2, n = _gated_operands(who, x1, x2, w_gate, w_up, b_gate, b_up)
+    _layer_input(who, "grad", grad, (m, n), (torch.bfloat16,))
+    act = _activation_code(who, activation)
+    need = _gated_sizes(k1, k2, m, n)
+    with _LayerLaunch(who, stream, x1, x2, w_gate, w_up, b_gate, b_up, grad) as sh:
+        dx1 = torch.empty_like(x1) if need_input else None
+        dx2 = torch.empty_like(x2) if need_input and x2 is not None else None
+        dwg = torch.empty_like(w_gate) if need_weight else None
+        dwu = torch.empty_like(w_up) if need_weight else None
+        dbg = None if b_gate is None else torch.empty_like(b_gate)
+        dbu = None if b_up is None else torch.empty_like(b_up)
+        ws = _layer_workspace(x1.device, need)
+        _native.check(_native.lib().dgfx_gated_dense_concat_backward_bf16(
+            _native.ptr(grad), _native.ptr(x1), k1, _native.ptr(x2), k2, m, _native.ptr(w_gate), _native.ptr(w_up),
+            _native.ptr(b_gate), _native.ptr(b_up), n, act, _native.ptr(dx1), _native.ptr(dx2), _native.ptr(dwg),
+            _native.ptr(dwu), _native.ptr(dbg), _native.ptr(dbu), _native.ptr(ws), need, sh))
+    return dx1, dx2, dwg, dwu, dbg, dbu
 
 
 def segment_group_norm(x, offsets, groups: int, weight=None, bias=None, eps: float = 1e-5, activation: str = "none",

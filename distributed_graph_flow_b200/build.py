@@ -33,7 +33,7 @@ NVCC_FLAGS = ARCH + [
 ]
 SOURCES = ["capi.cu", "primitives.cu", "csr_build.cu", "sampler.cu", "aggregate.cu", "halo.cu", "peer.cu", "synth.cu",
            "transform.cu", "dense.cu", "subgraph.cu", "negatives.cu", "idmap.cu", "timeseries.cu", "sparse_ops.cu",
-           "segment_norm.cu", "gated_scan.cu"]
+           "gated.cu", "segment_norm.cu", "gated_scan.cu"]
 
 
 def nvcc() -> str:

@@ -23,16 +23,10 @@
 // error flag (dgfx_dense_check), the roles leave their loops, outstanding
 // copies and MMAs are drained with bounded waits and TMEM is freed.
 // No TMA multicast, no clusters.
-#include <cuda.h>
-#include <cuda_bf16.h>
-#include <cudaTypedefs.h>
-
 #include <algorithm>
 #include <map>
-#include <mutex>
-#include <string>
 
-#include "common.cuh"
+#include "tensor_core.cuh"
 
 namespace dgfx {
 namespace {
@@ -41,117 +35,8 @@ constexpr int kBM = 128;
 constexpr int kBK = 64;
 constexpr int kStages = 4;
 constexpr int kThreads = 192;
-constexpr uint64_t kWaitNs = 2000000000ull;  // 2 s per wait
 
 __device__ unsigned int g_dense_err;
-
-__device__ __forceinline__ uint32_t smem_u32(const void* p) {
-  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-
-__device__ __forceinline__ uint64_t now_ns() {
-  uint64_t t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  return t;
-}
-
-__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
-}
-
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
-  asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.shared::cta.b64 st, [%0];\n\t}" ::"r"(bar) : "memory");
-}
-
-__device__ __forceinline__ void mbar_arrive_expect_tx(uint32_t bar, uint32_t bytes) {
-  asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n\t}" ::"r"(bar),
-               "r"(bytes)
-               : "memory");
-}
-
-__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-
-// Waits for the phase of `parity` to complete; false on timeout or when
-// another role already aborted (the abort word is then set).
-__device__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
-  if (mbar_test(bar, parity)) return true;
-  const uint64_t t0 = now_ns();
-  for (uint32_t i = 1;; ++i) {
-    if (mbar_test(bar, parity)) return true;
-    if ((i & 255u) == 0) {
-      if (*abort_flag) return false;
-      if (now_ns() - t0 > kWaitNs) {
-        *abort_flag = 1;
-        atomicOr(&g_dense_err, 1u);
-        return false;
-      }
-    }
-    if (i > 32) __nanosleep(20);
-  }
-}
-
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int32_t x,
-                                            int32_t y) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
-          dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
-      : "memory");
-}
-
-// Shared-memory matrix descriptor: K-major operand, 128-byte swizzle, rows of
-// 128 bytes, 8-row atoms 1024 bytes apart (stride byte offset).
-__device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t saddr) {
-  uint64_t d = 0;
-  d |= static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4);
-  d |= static_cast<uint64_t>(1) << 16;            // leading byte offset (unused for swizzled K-major)
-  d |= static_cast<uint64_t>(1024 >> 4) << 32;    // stride byte offset
-  d |= static_cast<uint64_t>(1) << 46;            // descriptor version (tcgen05)
-  d |= static_cast<uint64_t>(2) << 61;            // SWIZZLE_128B
-  return d;
-}
-
-// Instruction descriptor, kind::f16: D fp32, A and B bf16, both K-major.
-__host__ __device__ constexpr uint32_t idesc_bf16(int m, int n) {
-  return (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) |
-         (static_cast<uint32_t>(m >> 4) << 24);
-}
-
-__device__ __forceinline__ void mma_bf16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-                                         uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-
-__device__ __forceinline__ void mma_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
-
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
-        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
-        "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
-        "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
-      : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
 
 template <int BN>
 struct DenseSmem {
@@ -232,7 +117,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
         const int32_t mb = static_cast<int32_t>(t / n_tiles), nb = static_cast<int32_t>(t % n_tiles);
         for (int32_t kb = 0; kb < kb_total; ++kb) {
-          if (!mbar_wait(empty0 + 8 * s, ph ^ 1u, abort_flag)) {
+          if (!mbar_wait(empty0 + 8 * s, ph ^ 1u, abort_flag, &g_dense_err)) {
             ok = false;
             break;
           }
@@ -273,11 +158,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       bool any = false;
       for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-        if (!mbar_wait(acce0 + 8 * b, aph ^ 1u, abort_flag)) break;
+        if (!mbar_wait(acce0 + 8 * b, aph ^ 1u, abort_flag, &g_dense_err)) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(b * BN);
         for (int32_t kb = 0; kb < kb_total; ++kb) {
-          if (!mbar_wait(full0 + 8 * s, ph, abort_flag)) {
+          if (!mbar_wait(full0 + 8 * s, ph, abort_flag, &g_dense_err)) {
             ok = false;
             break;
           }
@@ -327,7 +212,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t aph = 0;
     for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
       bool ready = true;
-      if (lane == 0) ready = mbar_wait(accf0 + 8 * b, aph, abort_flag);
+      if (lane == 0) ready = mbar_wait(accf0 + 8 * b, aph, abort_flag, &g_dense_err);
       ready = __shfl_sync(0xffffffffu, ready ? 1 : 0, 0) != 0;
       if (!ready) break;
       tc_fence_after();
@@ -412,35 +297,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, []() {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess) {
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-    }
-  });
-  return fn;
-}
-
-// Row-major bf16 [rows, cols] matrix, box = box_rows x 64 columns, 128-byte swizzle.
-int make_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, uint32_t box_rows) {
-  auto fn = encode_fn();
-  if (fn == nullptr) return fail(DGFX_ERR_CUDA, "dgfx_dense: cuTensorMapEncodeTiled unavailable");
-  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
-  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(cols) * 2};
-  const cuuint32_t box[2] = {static_cast<cuuint32_t>(kBK), box_rows};
-  const cuuint32_t estr[2] = {1, 1};
-  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return fail(DGFX_ERR_CUDA, "dgfx_dense: cuTensorMapEncodeTiled failed (" + std::to_string(r) + ")");
-  return DGFX_OK;
-}
-
 template <int BN>
 int launch_dense(const CUtensorMap& x1, const CUtensorMap& x2, const CUtensorMap& w, const CUtensorMap& ym, int64_t m,
                  int32_t n, int32_t kb1, int32_t kbt, const float* bias, int32_t relu, cudaStream_t stream) {
@@ -463,6 +319,8 @@ int launch_dense(const CUtensorMap& x1, const CUtensorMap& x2, const CUtensorMap
   return DGFX_OK;
 }
 
+}  // namespace
+
 unsigned int* dense_err_word() {
   static std::mutex mu;
   static std::map<int, unsigned int*> cache;
@@ -476,6 +334,8 @@ unsigned int* dense_err_word() {
   cache[dev] = static_cast<unsigned int*>(p);
   return static_cast<unsigned int*>(p);
 }
+
+namespace {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 

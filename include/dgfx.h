@@ -346,6 +346,36 @@ int dgfx_dense_concat_bf16(const void* d_x1, int64_t k1, const void* d_x2,
 int dgfx_dense_check(dgfx_stream stream);
 
 /* ------------------------------------------------------------------------
+ * Gated dense layer over a concat on the tensor cores, with its backward
+ * pass: with X = concat[d_x1, d_x2] (bf16 [m, k1 + k2], never materialised),
+ *   d_h[m, n] = act(X @ d_w_gate^T + d_b_gate) * (X @ d_w_up^T + d_b_up)
+ * d_w_gate, d_w_up bf16 [n, k1 + k2] (torch Linear layout), biases fp32 [n] or
+ * NULL, act a DGFX_ACT_*; fp32 accumulation, both projections and the gate
+ * in one kernel, one rounding to bf16. k1 >= 8; k1, k2 and n multiples of 8;
+ * operands contiguous and 16-byte aligned.
+ * Backward from d_dh (bf16 [m, n]): d_dx1, d_dx2 (bf16, each may be NULL),
+ * d_dw_gate and d_dw_up (bf16, both or neither), d_db_gate, d_db_up (fp32,
+ * each may be NULL). The projections are computed again; the gradients of
+ * the two projections are rounded to bf16 once, as matrix operands (the bias
+ * gradients are summed in fp32 before that). Sums run in a fixed order.
+ * Pipeline waits that run out are reported by dgfx_dense_check.
+ * ------------------------------------------------------------------------ */
+int dgfx_gated_dense_concat_bf16(const void* d_x1, int64_t k1, const void* d_x2, int64_t k2,
+                                 int64_t m, const void* d_w_gate, const void* d_w_up,
+                                 const float* d_b_gate, const float* d_b_up, int64_t n,
+                                 int32_t activation, void* d_h, dgfx_stream stream);
+int dgfx_gated_dense_concat_backward_workspace_size(int64_t k1, int64_t k2, int64_t m, int64_t n,
+                                                    size_t* bytes);
+int dgfx_gated_dense_concat_backward_bf16(const void* d_dh, const void* d_x1, int64_t k1,
+                                          const void* d_x2, int64_t k2, int64_t m,
+                                          const void* d_w_gate, const void* d_w_up,
+                                          const float* d_b_gate, const float* d_b_up, int64_t n,
+                                          int32_t activation, void* d_dx1, void* d_dx2,
+                                          void* d_dw_gate, void* d_dw_up, float* d_db_gate,
+                                          float* d_db_up, void* d_workspace,
+                                          size_t workspace_bytes, dgfx_stream stream);
+
+/* ------------------------------------------------------------------------
  * Group norm with an activation over ragged segments, channels last (for
  * instance the graphs of a merged batch: d_offsets = its node_offsets).
  * Segment s is rows d_offsets[s] .. d_offsets[s+1] of d_x [rows, channels]

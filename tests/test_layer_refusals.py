@@ -13,6 +13,18 @@ def _x(rows=8, c=16, dtype=torch.float32):
     return torch.zeros((rows, c), dtype=dtype)
 
 
+BF = torch.bfloat16
+
+
+def _gated(x1=None, x2=None, w_gate=None, w_up=None, **kw):
+    x1 = _x(8, 16, BF) if x1 is None else x1
+    x2 = _x(8, 16, BF) if x2 is None else x2
+    k = x1.shape[1] + x2.shape[1]
+    w_gate = _x(16, k, BF) if w_gate is None else w_gate
+    w_up = _x(16, k, BF) if w_up is None else w_up
+    return aggregation.gated_dense_concat(x1, x2, w_gate, w_up, **kw)
+
+
 @pytest.mark.parametrize("call,match", [
     (lambda: aggregation.segment_group_norm(_x(dtype=torch.float16), OFF, 4), "x must be float32 or bfloat16"),
     (lambda: aggregation.segment_group_norm(_x()[:, ::2], OFF, 4), "contiguous"),
@@ -36,6 +48,19 @@ def _x(rows=8, c=16, dtype=torch.float32):
     (lambda: aggregation.gated_scan(_x(), _x(), OFF, initial=torch.zeros(3, 16)), "initial is"),
     (lambda: aggregation.gated_scan(_x(), _x(), OFF.float()), "offsets"),
     (lambda: aggregation.gated_scan_backward(_x(), _x(), _x(), OFF, torch.zeros(3)), "saved is"),
+    (lambda: _gated(x1=_x(8, 12, BF)), "multiples of 8"),
+    (lambda: _gated(x1=_x(8, 16)), "x1 must be bfloat16"),
+    (lambda: _gated(x2=_x(7, 16, BF)), "x2 is"),
+    (lambda: _gated(w_gate=_x(24, 32, BF)), "w_up is"),
+    (lambda: _gated(w_up=_x(16, 24, BF)), "w_up is"),
+    (lambda: _gated(w_gate=_x(12, 32, BF), w_up=_x(12, 32, BF)), "multiples of 8"),
+    (lambda: _gated(w_gate=_x(32, 16, BF).t()), "w_gate must be contiguous"),
+    (lambda: _gated(b_gate=torch.zeros(16, dtype=BF)), "b_gate must be float32"),
+    (lambda: _gated(b_up=torch.zeros(8)), "b_up is"),
+    (lambda: _gated(activation="swish"), "unknown activation"),
+    (lambda: _gated(out=_x(8, 16)), "out must be bfloat16"),
+    (lambda: aggregation.gated_dense_concat_backward(_x(8, 24, BF), _x(8, 16, BF), None, _x(16, 16, BF),
+                                                     _x(16, 16, BF)), "grad is"),
     (lambda: aggregation.gated_scan_step(_x(), _x(), torch.zeros(8, 8)), "state is"),
     (lambda: aggregation.gated_scan_step(_x(), _x(), torch.zeros(16, 8).t()), "state must be contiguous"),
 ])
