@@ -34,31 +34,6 @@ constexpr int kRows = 8;  // rows per thread
 constexpr int kCh = 4;    // channels per thread: 16 bytes of fp32, 8 of bf16
 constexpr int kMaxTile = kThreads * kRows;
 
-template <class T>
-struct Quad;
-template <>
-struct Quad<float> {
-  using raw = uint4;
-  __device__ static __forceinline__ void unpack(const raw& r, float (&f)[kCh]) { Vec16<float>::unpack(r, f); }
-  __device__ static __forceinline__ raw pack(const float (&f)[kCh]) { return Vec16<float>::pack(f); }
-  __device__ static __forceinline__ raw zero() { return make_uint4(0, 0, 0, 0); }
-};
-template <>
-struct Quad<__nv_bfloat16> {
-  using raw = uint2;
-  __device__ static __forceinline__ void unpack(const raw& r, float (&f)[kCh]) {
-    f[0] = __uint_as_float(r.x << 16);
-    f[1] = __uint_as_float(r.x & 0xFFFF0000u);
-    f[2] = __uint_as_float(r.y << 16);
-    f[3] = __uint_as_float(r.y & 0xFFFF0000u);
-  }
-  __device__ static __forceinline__ raw pack(const float (&f)[kCh]) {
-    const __nv_bfloat162 a = __floats2bfloat162_rn(f[0], f[1]), b = __floats2bfloat162_rn(f[2], f[3]);
-    return make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
-  }
-  __device__ static __forceinline__ raw zero() { return make_uint2(0, 0); }
-};
-
 // a = sigmoid(g) and 1 - a, both to full relative precision: e^-|g| never
 // overflows, and neither comes from a subtraction.
 __device__ __forceinline__ void gate_pair(float g, float* a, float* keep) {

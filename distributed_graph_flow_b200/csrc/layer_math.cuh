@@ -86,6 +86,32 @@ struct Vec16<__nv_bfloat16> {
   }
 };
 
+// Four adjacent values of T (a quad) as fp32.
+template <class T>
+struct Quad;
+template <>
+struct Quad<float> {
+  using raw = uint4;
+  __device__ static __forceinline__ void unpack(const raw& r, float (&f)[4]) { Vec16<float>::unpack(r, f); }
+  __device__ static __forceinline__ raw pack(const float (&f)[4]) { return Vec16<float>::pack(f); }
+  __device__ static __forceinline__ raw zero() { return make_uint4(0, 0, 0, 0); }
+};
+template <>
+struct Quad<__nv_bfloat16> {
+  using raw = uint2;
+  __device__ static __forceinline__ void unpack(const raw& r, float (&f)[4]) {
+    f[0] = __uint_as_float(r.x << 16);
+    f[1] = __uint_as_float(r.x & 0xFFFF0000u);
+    f[2] = __uint_as_float(r.y << 16);
+    f[3] = __uint_as_float(r.y & 0xFFFF0000u);
+  }
+  __device__ static __forceinline__ raw pack(const float (&f)[4]) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(f[0], f[1]), b = __floats2bfloat162_rn(f[2], f[3]);
+    return make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+  }
+  __device__ static __forceinline__ raw zero() { return make_uint2(0, 0); }
+};
+
 // First segment whose end lies past `row` (nseg if none): every lane of the
 // warp probes one of 32 evenly spaced ends per round, so the search takes
 // ceil(log32) dependent loads. Call from a full warp; all lanes get it.
