@@ -11,30 +11,32 @@
 //   dgate_t = delta_t (h_{t-1} - x_t) a_t (1 - a_t),  dinitial[s] = e_first.
 //
 // All rows form one flat scan that restarts at the first row of a segment,
-// so windows of any lengths balance. The rows are cut into tiles of equal
-// height; a tile's effect on the state that enters it is (A, H): state ->
-// A state + H, and A < 0 marks a tile (or a part of one) that holds a
-// restart, whose outgoing state is H alone (selected, not multiplied: a NaN
-// of one window never reaches the next).
+// cut into chunks of equal height whatever the windows' lengths, so the work
+// balances. A thread owns two adjacent channels of one chunk and walks its rows one by
+// one, the next rows' loads in flight; neighbouring threads are neighbouring channels,
+// so loads and stores are whole rows, and nothing is shared between threads.
 //
-// One pass over the data, bound by HBM: persistent CTAs take tiles in order
-// from a counter, each thread's inputs (kCh channels of a few consecutive
-// rows) come by cp.async into its own slots of shared memory and move to registers,
-// and the slots are refilled with the next tile's rows while this one's scan
-// runs. A tile publishes its (A, H) as soon as it has them. The state that
-// enters it is then composed from its predecessors' back to the tile where
-// its first row's segment began, no further: from the (A, H) of the tiles of its
-// group (32 tiles), of the groups of its supergroup (32 groups, each composed
-// by its last tile) and the state that left the supergroup before; so a
-// long segment costs a chain of one hop per 1024 tiles, and short windows
-// look one tile back. The shape of that composition is fixed by the tile's
-// number, so results do not change from run to run. A tile only waits for
-// tiles taken before it; waits are bounded, and one that runs out is latched
-// in the status word of dgfx_dense_check and ends all others.
+//   chunk kernel   what a chunk does to a state that passes through its last
+//                  row: (A, H), state -> A state + H. Only the segment that crosses
+//                  that edge matters, so only its rows in the chunk are read:
+//                  a few rows where windows are short, all of them inside of
+//                  a long one. A < 0 marks a segment that began in the chunk:
+//                  the outgoing state is H alone (selected, not multiplied: a
+//                  NaN of one window never reaches the next).
+//   level kernel   (A, H) of groups of 32 chunks, and of 32 groups.
+//   apply kernel   composes the state that enters its chunk, back to the
+//                  chunk where that segment began and no further (at most 31 chunks, 31
+//                  groups and the supergroups before them), then walks
+//                  the rows and writes. No thread waits for another.
 //
-// The backward pass runs the tiles from the last to the first. It computes
-// the forward states again, from the state that entered the tile (saved by
-// the forward pass: 4 bytes per tile and channel), instead of reading h.
+// Bound by HBM: one read of each input and one write of each output where
+// windows are short, and up to a second read of gate and x (gate and grad,
+// going backward) inside of windows longer than a chunk. The composition's
+// shape depends on the sizes alone, so results do not change from run to run.
+//
+// Going backward, h is not read but computed again, from states that the
+// forward pass saves before every kBlock-th row (4 bytes per kBlock rows and
+// channel), in registers.
 //
 // States, products and gradients of states are fp32; h, dx and dgate are
 // rounded once when written. Rows outside [off[0], off[nseg]) are written as
@@ -43,20 +45,38 @@
 #include <string>
 
 #include "layer_math.cuh"
-#include "tensor_core.cuh"
 
 namespace dgfx {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kCh = 4;  // channels per thread: 16 bytes of fp32, 8 of bf16
-constexpr int kGroup = 32;
-constexpr int kSuper = kGroup * kGroup;
+constexpr int kCh = 4;     // channels per thread of the single step
+constexpr int kBlock = 8;  // rows loaded at a time; rows between saved states
+constexpr int kLevel = 32;
 constexpr int kSms = 148;
 
-// Rows per thread: 64 bytes of each input.
+// Two adjacent values of T as fp32.
 template <class T>
-constexpr int kRows = sizeof(T) == 2 ? 8 : 4;
+struct Pair;
+template <>
+struct Pair<float> {
+  using raw = float2;
+  __device__ static __forceinline__ float2 unpack(raw r) { return r; }
+  __device__ static __forceinline__ raw pack(float2 f) { return f; }
+  __device__ static __forceinline__ raw zero() { return make_float2(0.0f, 0.0f); }
+};
+template <>
+struct Pair<__nv_bfloat16> {
+  using raw = uint32_t;
+  __device__ static __forceinline__ float2 unpack(raw r) {
+    return make_float2(__uint_as_float(r << 16), __uint_as_float(r & 0xFFFF0000u));
+  }
+  __device__ static __forceinline__ raw pack(float2 f) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  __device__ static __forceinline__ raw zero() { return 0u; }
+};
 
 // a = sigmoid(g) and 1 - a, both to full relative precision: e^-|g| never
 // overflows, and neither comes from a subtraction.
@@ -65,24 +85,6 @@ __device__ __forceinline__ void gate_pair(float g, float* a, float* keep) {
   const float big = __fdividef(1.0f, 1.0f + e), small = e * big;
   *a = g >= 0.0f ? big : small;
   *keep = g >= 0.0f ? small : big;
-}
-
-// Shape of the tiling. Columns are groups of kCh channels; a tile is `width`
-// columns wide (at most 16: 128 bytes of a bf16 row) and `subs` threads high.
-struct Geometry {
-  int32_t cols, width, across, subs, tile_rows;
-  int64_t tiles;
-};
-
-Geometry geometry(int64_t rows, int64_t channels, int dtype) {
-  Geometry g;
-  g.cols = static_cast<int32_t>(channels / kCh);
-  g.across = (g.cols + 15) / 16;
-  g.width = (g.cols + g.across - 1) / g.across;
-  g.subs = kThreads / g.width;
-  g.tile_rows = g.subs * (dtype == DGFX_F32 ? kRows<float> : kRows<__nv_bfloat16>);
-  g.tiles = ceil_div(std::max<int64_t>(rows, 1), g.tile_rows);
-  return g;
 }
 
 struct Params {
@@ -97,619 +99,422 @@ struct Params {
   void* dx;
   void* dgate;
   float* dinitial;
-  float* save;         // forward: state entering each tile [tiles, channels], or null
+  float* save;         // forward: states before every kBlock-th row [ceil(rows / kBlock), channels], or null
   const float* saved;  // backward: the same
-  float2* tile_ah;     // [tiles, channels], by the order of processing
-  float2* group_ah;    // [groups, channels]
-  float* super_state;  // [supergroups, channels]
-  uint32_t* tile_flag;  // [tiles, across]; then groups, supergroups, the counter and the abort word
-  uint32_t* group_flag;
-  uint32_t* super_flag;
-  uint32_t* counter;
-  uint32_t* aborted;
-  int32_t* first_seg;  // per tile: the segment of its first row (or the next one)
-  int32_t* origin;     // per tile: the tile (by number) where the segment that enters it began
-  unsigned int* err;
-  int64_t rows, channels, nseg;
-  int64_t clear_words;
-  Geometry geo;
-  int32_t up;  // backward: tiles are processed from the last to the first
+  float4* chunk_ah;    // (A, H, A, H) of two channels: [chunks, pairs]
+  float4* group_ah;    // [groups, pairs]
+  float4* super_ah;    // [supergroups, pairs]
+  int32_t* edge_seg;   // per chunk: where its first (backward: last) row stands among the segments
+  int64_t rows, nseg, chunks, groups, supers;
+  int32_t channels, pairs, chunk_rows;
 };
 
-// ---------------------------------------------------------------------------
-// Before the scan: where every tile stands among the segments, outputs of the
-// segments without rows, and cleared flags. A warp per segment.
-// ---------------------------------------------------------------------------
-__global__ void scan_plan_kernel(Params p, const float* __restrict__ empty_in, float* __restrict__ empty_out) {
-  const int64_t threads = static_cast<int64_t>(gridDim.x) * blockDim.x;
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  const int lane = threadIdx.x & 31;
-  for (int64_t i = t; i < p.clear_words; i += threads) p.tile_flag[i] = 0;
-  const int64_t lo = clamp64(p.off[0], 0, p.rows), hi = clamp64(p.off[p.nseg], lo, p.rows);
-  const int64_t tr = p.geo.tile_rows;
-  // Tiles whose first row (last row, going up) lies outside of every segment
-  // have nothing to wait for.
-  for (int64_t i = t; i < p.geo.tiles; i += threads) {
-    const int64_t row0 = i * tr, row1 = (row0 + tr < p.rows ? row0 + tr : p.rows) - 1;
-    if (row0 < lo || row0 >= hi) p.first_seg[i] = row0 < lo ? 0 : static_cast<int32_t>(p.nseg);
-    const int64_t edge = p.up ? row1 : row0;
-    if (edge < lo || edge >= hi) p.origin[i] = static_cast<int32_t>(i);
+// The largest i in [0, n] with off[i] <= row, -1 if there is none: eight-way,
+// the probes of a round independent of one another.
+__device__ __forceinline__ int64_t last_at_most(const int64_t* __restrict__ off, int64_t n, int64_t row) {
+  int64_t lo = -1, hi = n + 1;
+  while (hi - lo > 1) {
+    const int64_t step = (hi - lo + 7) >> 3;
+    int below = 0;
+#pragma unroll
+    for (int k = 1; k < 8; ++k) {
+      const int64_t q = lo + step * k;
+      below += q < hi && __ldg(off + q) <= row;
+    }
+    lo += step * below;
+    hi = lo + step < hi ? lo + step : hi;
   }
-  for (int64_t s = t >> 5; s < p.nseg; s += threads >> 5) {
-    const int64_t b = clamp64(p.off[s], lo, hi), e = clamp64(p.off[s + 1], b, hi);
-    if (b == e) {
-      if (empty_out != nullptr) {
-        for (int64_t c = lane; c < p.channels; c += 32) {
-          empty_out[s * p.channels + c] = empty_in != nullptr ? empty_in[s * p.channels + c] : 0.0f;
-        }
-      }
-      continue;
-    }
-    // Tiles whose first row lies in [b, e).
-    for (int64_t i = (b + tr - 1) / tr + lane; i * tr < e; i += 32) {
-      p.first_seg[i] = static_cast<int32_t>(s);
-      if (!p.up) p.origin[i] = static_cast<int32_t>(b / tr);
-    }
-    if (p.up) {  // tiles whose last row does
-      for (int64_t i = b / tr + lane; i < p.geo.tiles; i += 32) {
-        const int64_t row1 = (i * tr + tr < p.rows ? i * tr + tr : p.rows) - 1;
-        if (row1 >= e) break;
-        p.origin[i] = static_cast<int32_t>((e - 1) / tr);
-      }
-    }
-  }
+  return lo;
 }
 
-// The segment structure of one tile: for each row the segment that starts
-// (ends) there, -1 if none. [lo, hi) are the rows inside any segment.
-struct TileSegments {
-  int32_t* starts;
-  int32_t* ends;
-  int64_t lo, hi;
-};
-
-__device__ __forceinline__ void find_segments(const Params& p, int64_t tile, TileSegments& ts) {
-  const int64_t row0 = tile * p.geo.tile_rows;
-  const int64_t row_end = row0 + p.geo.tile_rows < p.rows ? row0 + p.geo.tile_rows : p.rows;
-  // Clamped: offsets that do not ascend may leave it unset.
-  const int64_t first = clamp64(__ldcg(p.first_seg + tile), 0, p.nseg);
-  for (int i = threadIdx.x; i < p.geo.tile_rows; i += kThreads) {
-    ts.starts[i] = -1;
-    ts.ends[i] = -1;
+// (A, H) of two channels.
+struct Effect {
+  float4 v;
+  __device__ Effect() : v(make_float4(1.0f, 0.0f, 1.0f, 0.0f)) {}
+  __device__ void then(const float4& n) {
+    v.y = n.x < 0.0f ? n.y : fmaf(n.x, v.y, n.y);
+    v.w = n.z < 0.0f ? n.w : fmaf(n.z, v.w, n.w);
+    v.x = (n.x < 0.0f || v.x < 0.0f) ? -1.0f : v.x * n.x;
+    v.z = (n.z < 0.0f || v.z < 0.0f) ? -1.0f : v.z * n.z;
   }
-  __syncthreads();
-  for (int64_t s = first + threadIdx.x;; s += kThreads) {
-    bool more = false;
-    if (s < p.nseg) {
-      const int64_t b = __ldg(p.off + s), e = __ldg(p.off + s + 1);
-      if (b < e) {
-        if (b >= row0 && b < row_end) ts.starts[b - row0] = static_cast<int32_t>(s);
-        if (e > row0 && e <= row_end) ts.ends[e - 1 - row0] = static_cast<int32_t>(s);
+  // Items `from`, from + dir, .. (n of them) of a table, in that order.
+  __device__ void then_items(const float4* __restrict__ table, int64_t from, int dir, int64_t n, int64_t pitch) {
+    for (int64_t i = 0; i < n; i += 8) {
+      float4 t[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (i + k < n) t[k] = __ldg(table + (from + dir * (i + k)) * pitch);
       }
-      more = threadIdx.x == kThreads - 1 && b < row_end;
-    }
-    if (!__syncthreads_or(more)) break;
-  }
-}
-
-__device__ __forceinline__ float enter(float a, float h, float state) { return a < 0.0f ? h : fmaf(a, state, h); }
-
-// (a, h) followed by (na, nh).
-__device__ __forceinline__ void then(float* a, float* h, float na, float nh) {
-  *h = enter(na, nh, *h);
-  *a = (na < 0.0f || *a < 0.0f) ? -1.0f : *a * na;
-}
-
-// Exclusive composition of the subs' (A, H) in place, `up` from the last row
-// to the first; the tile's own (A, H) in *ta, *th. One thread per channel.
-__device__ __forceinline__ void compose(float* sa, float* sh, int chans, int subs, bool up, int ch, float* ta,
-                                        float* th) {
-  float a = 1.0f, h = 0.0f;
-  for (int k = 0; k < subs; ++k) {
-    const int i = (up ? subs - 1 - k : k) * chans + ch;
-    const float ca = sa[i], chv = sh[i];
-    sa[i] = a;
-    sh[i] = h;
-    then(&a, &h, ca, chv);
-  }
-  *ta = a;
-  *th = h;
-}
-
-__device__ __forceinline__ uint32_t load_flag(const uint32_t* f) {
-  uint32_t v;
-  asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(f) : "memory");
-  return v;
-}
-
-__device__ __forceinline__ void raise_flag(uint32_t* f) {
-  asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(f), "r"(1u) : "memory");
-}
-
-// Waits (one warp) until every lane's flag is up; lanes without one pass
-// null. Gives up after 2 s, or when another wait of this launch did.
-__device__ __forceinline__ void wait_flags(const Params& p, const uint32_t* flag) {
-  const uint64_t t0 = now_ns();
-  for (uint32_t i = 1;; ++i) {
-    const bool up = flag == nullptr || load_flag(flag) != 0;
-    if (__all_sync(0xffffffffu, up)) return;
-    if ((i & 63u) == 0) {
-      bool stop = false;
-      if ((threadIdx.x & 31) == 0) {
-        stop = load_flag(p.aborted) != 0;
-        if (!stop && now_ns() - t0 > kWaitNs) {
-          raise_flag(p.aborted);
-          atomicOr(p.err, 2u);
-          stop = true;
-        }
-      }
-      if (__any_sync(0xffffffffu, stop)) return;
-    }
-  }
-}
-
-// Work of one CTA on one tile in the order of processing: publishing and the
-// state that enters. fold: (A, H) of consecutive tiles or groups, composed by
-// all threads (each a contiguous part per channel, then the parts in order).
-struct Chain {
-  const Params& p;
-  float2* parts;  // [kThreads]
-  float* state;   // [chans]: the state that enters the tile
-  int chans, part, lanes, my_ch, my_part;
-  int64_t gch;  // this thread's channel of the fold
-
-  __device__ Chain(const Params& params, float2* parts_, float* state_, int part_)
-      : p(params), parts(parts_), state(state_), chans(params.geo.width * kCh), part(part_) {
-    lanes = kThreads / chans;
-    my_part = threadIdx.x / chans;
-    my_ch = threadIdx.x - my_part * chans;
-    gch = static_cast<int64_t>(part) * chans + my_ch;
-  }
-
-  // Composes groups [g0, g1) and then tiles [t0, t1) for this thread's
-  // channel; valid in the threads of part 0. Contains barriers.
-  __device__ float2 fold(int64_t g0, int64_t g1, int64_t t0, int64_t t1) {
-    const int ng = static_cast<int>(g1 - g0), n = ng + static_cast<int>(t1 - t0);
-    const int each = (n + lanes - 1) / lanes;
-    float a = 1.0f, h = 0.0f;
-    if (my_part < lanes && gch < p.channels) {
-      const int from = my_part * each, to = min(n, from + each);
-#pragma unroll 4
-      for (int i = from; i < to; ++i) {
-        const float2* src = i < ng ? p.group_ah + (g0 + i) * p.channels : p.tile_ah + (t0 + i - ng) * p.channels;
-        const float2 v = __ldcg(src + gch);
-        then(&a, &h, v.x, v.y);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (i + k < n) then(t[k]);
       }
     }
-    parts[threadIdx.x] = make_float2(a, h);
-    __syncthreads();
-    a = 1.0f;
-    h = 0.0f;
-    if (my_part == 0) {
-      for (int k = 0; k < lanes; ++k) {
-        const float2 v = parts[k * chans + my_ch];
-        then(&a, &h, v.x, v.y);
-      }
-    }
-    __syncthreads();
-    return make_float2(a, h);
-  }
-
-  // Publishes tile j's (A, H) (threads of part 0 hold it) and its group's, if
-  // j is the last of it.
-  __device__ void publish(int64_t j, float2 ah) {
-    if (my_part == 0 && gch < p.channels) __stcg(p.tile_ah + j * p.channels + gch, ah);
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) raise_flag(p.tile_flag + j * p.geo.across + part);
-    if (j % kGroup != kGroup - 1) return;
-    const int64_t t0 = j - (kGroup - 1);
-    if (threadIdx.x < 32) wait_flags(p, p.tile_flag + (t0 + threadIdx.x) * p.geo.across + part);
-    __syncthreads();
-    const float2 g = fold(0, 0, t0, j + 1);
-    if (my_part == 0 && gch < p.channels) __stcg(p.group_ah + j / kGroup * p.channels + gch, g);
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) raise_flag(p.group_flag + j / kGroup * p.geo.across + part);
-  }
-
-  // The state that enters tile j, whose segment began in tile k0 <= j (all in the
-  // order of processing), into state[]; `ah` is the tile's own (part 0).
-  // Publishes the state that leaves j if it ends a supergroup.
-  __device__ void enter_tile(int64_t j, int64_t k0, float2 ah) {
-    float st = 0.0f;
-    if (k0 < j) {
-      const int64_t gs = j / kGroup * kGroup, ss = j / kSuper * kSuper;
-      const int64_t t0 = k0 > gs ? k0 : gs;
-      const int64_t g1 = gs / kGroup;
-      int64_t g0 = g1;
-      if (k0 < gs) g0 = k0 > ss ? k0 / kGroup : ss / kGroup;
-      const bool super = k0 < ss;
-      if (threadIdx.x < 32) {
-        const int lane = threadIdx.x;
-        wait_flags(p, t0 + lane < j ? p.tile_flag + (t0 + lane) * p.geo.across + part : nullptr);
-        if (g0 < g1) wait_flags(p, g0 + lane < g1 ? p.group_flag + (g0 + lane) * p.geo.across + part : nullptr);
-        if (super) wait_flags(p, lane == 0 ? p.super_flag + (ss / kSuper - 1) * p.geo.across + part : nullptr);
-      }
-      __syncthreads();
-      const float2 f = fold(g0, g1, t0, j);
-      if (my_part == 0 && gch < p.channels) {
-        if (super) st = __ldcg(p.super_state + (ss / kSuper - 1) * p.channels + gch);
-        st = enter(f.x, f.y, st);
-      }
-    }
-    if (my_part == 0) state[my_ch] = st;
-    if (j % kSuper == kSuper - 1) {
-      if (my_part == 0 && gch < p.channels) {
-        __stcg(p.super_state + j / kSuper * p.channels + gch, enter(ah.x, ah.y, st));
-      }
-      __threadfence();
-      __syncthreads();
-      if (threadIdx.x == 0) raise_flag(p.super_flag + j / kSuper * p.geo.across + part);
-    }
-    __syncthreads();
   }
 };
 
-// One quad to this thread's slot; zeros instead if it is not there.
+__device__ __forceinline__ float2 load2(const float* base, int64_t row, int channels, int ch) {
+  return __ldg(reinterpret_cast<const float2*>(base + row * channels + ch));
+}
+__device__ __forceinline__ void store2(float* base, int64_t row, int channels, int ch, float2 v) {
+  *reinterpret_cast<float2*>(base + row * channels + ch) = v;
+}
+
 template <class T>
-__device__ __forceinline__ void fetch(void* slot, const void* src, bool there) {
-  constexpr int kBytes = sizeof(typename Quad<T>::raw);
-  const int n = there ? kBytes : 0;
-  if (kBytes == 16) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(slot)), "l"(src), "r"(n) : "memory");
+__device__ __forceinline__ typename Pair<T>::raw load_pair(const void* base, int64_t row, int pairs, int pair) {
+  return __ldg(static_cast<const typename Pair<T>::raw*>(base) + row * pairs + pair);
+}
+
+// ---------------------------------------------------------------------------
+// Chunk kernels
+// ---------------------------------------------------------------------------
+// Forward: thread (j, pair) looks at the edge below chunk j - 1, the first
+// row of chunk j: it notes where that row stands and writes the effect of
+// chunk j - 1 on the segment that crosses the edge.
+template <class T>
+__global__ void __launch_bounds__(kThreads) scan_chunk_kernel(Params p) {
+  using P = Pair<T>;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  const int64_t j = t / p.pairs;
+  const int pair = static_cast<int>(t - j * p.pairs);
+  if (j >= p.chunks) return;
+  const int64_t edge = j * p.chunk_rows;
+  const int64_t seg = last_at_most(p.off, p.nseg, edge);
+  if (pair == 0) p.edge_seg[j] = static_cast<int32_t>(seg);
+  if (j == 0) return;
+  Effect f;
+  f.v = make_float4(-1.0f, 0.0f, -1.0f, 0.0f);
+  if (seg >= 0 && seg < p.nseg) {
+    const int64_t first = edge - p.chunk_rows, begin = __ldg(p.off + seg);
+    const int64_t from = begin > first ? begin : first;
+    if (from < edge) {
+      float2 a = make_float2(1.0f, 1.0f), h = make_float2(0.0f, 0.0f);
+      if (begin >= first && p.initial != nullptr) h = load2(p.initial, seg, p.channels, 2 * pair);
+      for (int64_t r = from; r < edge; r += kBlock) {
+        typename P::raw g[kBlock], x[kBlock];
+#pragma unroll
+        for (int i = 0; i < kBlock; ++i) {
+          if (r + i < edge) {
+            g[i] = load_pair<T>(p.gate, r + i, p.pairs, pair);
+            x[i] = load_pair<T>(p.x, r + i, p.pairs, pair);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < kBlock; ++i) {
+          if (r + i < edge) {
+            const float2 gv = P::unpack(g[i]), xv = P::unpack(x[i]);
+            float2 av, kv;
+            gate_pair(gv.x, &av.x, &kv.x);
+            gate_pair(gv.y, &av.y, &kv.y);
+            h.x = fmaf(av.x, h.x, kv.x * xv.x);
+            h.y = fmaf(av.y, h.y, kv.y * xv.y);
+            a.x *= av.x;
+            a.y *= av.y;
+          }
+        }
+      }
+      const bool began = begin >= first;
+      f.v = make_float4(began ? -1.0f : a.x, h.x, began ? -1.0f : a.y, h.y);
+    }
+  }
+  p.chunk_ah[(j - 1) * p.pairs + pair] = f.v;
+}
+
+// Backward: thread (j, pair) looks at the edge above chunk j: the effect of
+// chunk j, upwards, on the segment that crosses it; and notes the last
+// segment with rows that begins at or before chunk j's last row.
+template <class T>
+__global__ void __launch_bounds__(kThreads) scan_chunk_up_kernel(Params p) {
+  using P = Pair<T>;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  const int64_t j = t / p.pairs;
+  const int pair = static_cast<int>(t - j * p.pairs);
+  if (j >= p.chunks) return;
+  const int64_t edge = j * p.chunk_rows;
+  const int64_t stop = edge + p.chunk_rows < p.rows ? edge + p.chunk_rows : p.rows;
+  if (pair == 0) {
+    int64_t last = last_at_most(p.off, p.nseg, stop - 1);
+    if (last == p.nseg) --last;
+    while (last >= 0 && __ldg(p.off + last) >= __ldg(p.off + last + 1)) --last;
+    p.edge_seg[j] = static_cast<int32_t>(last);
+  }
+  if (j == 0) return;
+  const int64_t seg = last_at_most(p.off, p.nseg, edge);
+  Effect f;
+  f.v = make_float4(-1.0f, 0.0f, -1.0f, 0.0f);
+  if (seg >= 0 && seg < p.nseg && __ldg(p.off + seg) < edge) {
+    const int64_t end = __ldg(p.off + seg + 1);
+    const int64_t to = end < stop ? end : stop;
+    float2 a = make_float2(1.0f, 1.0f), e = make_float2(0.0f, 0.0f);
+    if (end <= stop && p.grad_final != nullptr) e = load2(p.grad_final, seg, p.channels, 2 * pair);
+    for (int64_t r = to; r > edge; r -= kBlock) {  // rows r - 1, r - 2, ..
+      typename P::raw g[kBlock], d[kBlock];
+#pragma unroll
+      for (int i = 0; i < kBlock; ++i) {
+        if (r - 1 - i >= edge) {
+          g[i] = load_pair<T>(p.gate, r - 1 - i, p.pairs, pair);
+          d[i] = p.grad != nullptr ? load_pair<T>(p.grad, r - 1 - i, p.pairs, pair) : P::zero();
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kBlock; ++i) {
+        if (r - 1 - i >= edge) {
+          const float2 gv = P::unpack(g[i]), dv = P::unpack(d[i]);
+          float2 av, kv;
+          gate_pair(gv.x, &av.x, &kv.x);
+          gate_pair(gv.y, &av.y, &kv.y);
+          e.x = av.x * (dv.x + e.x);
+          e.y = av.y * (dv.y + e.y);
+          a.x *= av.x;
+          a.y *= av.y;
+        }
+      }
+    }
+    const bool ended = end <= stop;
+    f.v = make_float4(ended ? -1.0f : a.x, e.x, ended ? -1.0f : a.y, e.y);
+  }
+  p.chunk_ah[j * p.pairs + pair] = f.v;
+}
+
+// Effects of groups of kLevel items of the level below, in the order of the
+// pass (`up`: from the last to the first).
+__global__ void __launch_bounds__(kThreads) scan_level_kernel(const float4* __restrict__ items, int64_t count, int pairs,
+                                                              int up, float4* __restrict__ out, int64_t outs) {
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  const int64_t g = t / pairs;
+  const int pair = static_cast<int>(t - g * pairs);
+  if (g >= outs) return;
+  const int64_t first = g * kLevel, last = first + kLevel < count ? first + kLevel : count;
+  Effect f;
+  f.then_items(items + pair, up ? last - 1 : first, up ? -1 : 1, last - first, pairs);
+  out[g * pairs + pair] = f.v;
+}
+
+// The state that enters chunk j when the segment at its edge began in chunk
+// o < j (going up: ends in chunk o > j).
+__device__ __forceinline__ float2 entering(const Params& p, int64_t j, int64_t o, int pair, bool up) {
+  Effect f;
+  const int64_t g = j / kLevel, s = g / kLevel, go = o / kLevel, so = go / kLevel;
+  if (up) {
+    if (so > s) f.then_items(p.super_ah + pair, so, -1, so - s, p.pairs);
+    const int64_t g_hi = so > s ? (s + 1) * kLevel - 1 : go;
+    if (go > g) f.then_items(p.group_ah + pair, g_hi, -1, g_hi - g, p.pairs);
+    const int64_t c_hi = go > g ? (g + 1) * kLevel - 1 : o;
+    f.then_items(p.chunk_ah + pair, c_hi, -1, c_hi - j, p.pairs);
   } else {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(smem_u32(slot)), "l"(src), "r"(n) : "memory");
+    if (so < s) f.then_items(p.super_ah + pair, so, 1, s - so, p.pairs);
+    const int64_t g_lo = so < s ? s * kLevel : go;
+    if (go < g) f.then_items(p.group_ah + pair, g_lo, 1, g - g_lo, p.pairs);
+    const int64_t c_lo = go < g ? g * kLevel : o;
+    f.then_items(p.chunk_ah + pair, c_lo, 1, j - c_lo, p.pairs);
+  }
+  return make_float2(f.v.y, f.v.w);
+}
+
+// out[s] = in[s] (0 without `in`) for the segments without rows, one thread
+// per segment.
+__device__ __forceinline__ void fill_empty(const Params& p, const float* in, float* out) {
+  const int64_t threads = static_cast<int64_t>(gridDim.x) * kThreads;
+  for (int64_t s = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; s < p.nseg; s += threads) {
+    if (__ldg(p.off + s) < __ldg(p.off + s + 1)) continue;
+    for (int c = 0; c < p.channels; c += 2) {
+      store2(out, s, p.channels, c, in != nullptr ? load2(in, s, p.channels, c) : make_float2(0.0f, 0.0f));
+    }
   }
 }
 
-__device__ __forceinline__ void fetch_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void fetch_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// ---------------------------------------------------------------------------
+// Apply kernels
+// ---------------------------------------------------------------------------
+template <class T>
+__global__ void __launch_bounds__(kThreads, 3) scan_apply_kernel(Params p) {
+  using P = Pair<T>;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  const int64_t j = t / p.pairs;
+  const int pair = static_cast<int>(t - j * p.pairs), ch = 2 * pair;
+  if (j < p.chunks) {
+    const int64_t r0 = j * p.chunk_rows;
+    const int n = static_cast<int>(p.rows - r0 < p.chunk_rows ? p.rows - r0 : p.chunk_rows);
+    typename P::raw g[kBlock], x[kBlock];
+#pragma unroll
+    for (int i = 0; i < kBlock; ++i) {
+      if (i < n) {
+        g[i] = load_pair<T>(p.gate, r0 + i, p.pairs, pair);
+        x[i] = load_pair<T>(p.x, r0 + i, p.pairs, pair);
+      }
+    }
+    // The current segment, the row (from r0) where it ends, and whether there
+    // is one: rows before the first and behind the last have none.
+    int64_t seg = p.edge_seg[j];
+    const int64_t hi = clamp64(__ldg(p.off + p.nseg), 0, p.rows);
+    auto until = [&](int64_t row) { return static_cast<int>(clamp64(row - r0, 0, p.chunk_rows + 1)); };
+    bool inside = seg >= 0 && seg < p.nseg;
+    int limit;
+    float2 st = make_float2(0.0f, 0.0f);
+    if (inside) {
+      const int64_t begin = clamp64(__ldg(p.off + seg), 0, r0);
+      limit = until(__ldg(p.off + seg + 1));
+      if (begin < r0) st = entering(p, j, begin / p.chunk_rows, pair, false);
+      else if (p.initial != nullptr) st = load2(p.initial, seg, p.channels, ch);
+    } else {
+      limit = seg < 0 ? until(__ldg(p.off)) : p.chunk_rows + 1;
+    }
+    if (limit == 0) limit = p.chunk_rows + 1;  // only where offsets do not ascend
+    for (int b0 = 0; b0 < n; b0 += kBlock) {
+      typename P::raw gn[kBlock], xn[kBlock];
+#pragma unroll
+      for (int i = 0; i < kBlock; ++i) {
+        if (b0 + kBlock + i < n) {
+          gn[i] = load_pair<T>(p.gate, r0 + b0 + kBlock + i, p.pairs, pair);
+          xn[i] = load_pair<T>(p.x, r0 + b0 + kBlock + i, p.pairs, pair);
+        }
+      }
+      if (p.save != nullptr) store2(p.save, (r0 + b0) / kBlock, p.channels, ch, st);
+#pragma unroll
+      for (int i = 0; i < kBlock; ++i) {
+        const int r = b0 + i;
+        if (r < n) {
+          const float2 gv = P::unpack(g[i]), xv = P::unpack(x[i]);
+          float2 av, kv;
+          gate_pair(gv.x, &av.x, &kv.x);
+          gate_pair(gv.y, &av.y, &kv.y);
+          st.x = inside ? fmaf(av.x, st.x, kv.x * xv.x) : 0.0f;
+          st.y = inside ? fmaf(av.y, st.y, kv.y * xv.y) : 0.0f;
+          if (p.h != nullptr) static_cast<typename P::raw*>(p.h)[(r0 + r) * p.pairs + pair] = P::pack(st);
+          if (r + 1 == limit) {  // this row is the segment's last: on to the next one with rows
+            if (inside && p.final != nullptr) store2(p.final, seg, p.channels, ch, st);
+            int64_t end = r0 + r + 1;
+            do {
+              ++seg;
+              if (seg < p.nseg) end = __ldg(p.off + seg + 1);
+            } while (seg < p.nseg && end <= r0 + r + 1);
+            inside = seg < p.nseg;
+            limit = inside ? until(end < hi ? end : hi) : p.chunk_rows + 1;
+            st = inside && p.initial != nullptr ? load2(p.initial, seg, p.channels, ch) : make_float2(0.0f, 0.0f);
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kBlock; ++i) {
+        g[i] = gn[i];
+        x[i] = xn[i];
+      }
+    }
+  }
+  if (p.final != nullptr) fill_empty(p, p.initial, p.final);
 }
 
-// Shared memory of a CTA: INPUTS x rows x threads slots of quads, the subs'
-// (A, H), the fold's parts, the entering state, the tile's segments.
-template <class T, int INPUTS, bool KEEP>
-struct Smem {
-  using raw = typename Quad<T>::raw;
-  raw* slots;
-  float4* keep;  // backward: 1 - a of this thread's rows
-  float *sa, *sh, *state;
-  float2* parts;
-  int32_t *starts, *ends;
-  static size_t bytes(const Geometry& g) {
-    return static_cast<size_t>(INPUTS) * kRows<T> * kThreads * sizeof(raw) +
-           (KEEP ? static_cast<size_t>(kRows<T>) * kThreads * sizeof(float4) : 0) +
-           2 * kThreads * kCh * sizeof(float) + kThreads * sizeof(float2) + 64 * sizeof(float) +
-           2 * static_cast<size_t>(g.tile_rows) * sizeof(int32_t);
-  }
-  __device__ Smem(void* base, const Geometry& g) {
-    char* b = static_cast<char*>(base);
-    auto take = [&](size_t n) {
-      char* r = b;
-      b += n;
-      return r;
+template <class T>
+__global__ void __launch_bounds__(kThreads, 2) scan_apply_up_kernel(Params p) {
+  using P = Pair<T>;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  const int64_t j = t / p.pairs;
+  const int pair = static_cast<int>(t - j * p.pairs), ch = 2 * pair;
+  if (j < p.chunks) {
+    const int64_t r0 = j * p.chunk_rows;
+    const int n = static_cast<int>(p.rows - r0 < p.chunk_rows ? p.rows - r0 : p.chunk_rows);
+    const int64_t lo64 = clamp64(__ldg(p.off), 0, p.rows), hi64 = clamp64(__ldg(p.off + p.nseg), lo64, p.rows);
+    auto rel = [&](int64_t row) { return static_cast<int>(clamp64(row - r0, -1, p.chunk_rows + 1)); };
+    const int lo = rel(lo64), hi = rel(hi64);
+    auto fetch = [&](int b0, typename P::raw(&g)[kBlock], typename P::raw(&x)[kBlock], typename P::raw(&d)[kBlock]) {
+#pragma unroll
+      for (int i = 0; i < kBlock; ++i) {
+        if (b0 + i < n) {
+          g[i] = load_pair<T>(p.gate, r0 + b0 + i, p.pairs, pair);
+          x[i] = load_pair<T>(p.x, r0 + b0 + i, p.pairs, pair);
+          d[i] = p.grad != nullptr ? load_pair<T>(p.grad, r0 + b0 + i, p.pairs, pair) : P::zero();
+        }
+      }
     };
-    slots = reinterpret_cast<raw*>(take(static_cast<size_t>(INPUTS) * kRows<T> * kThreads * sizeof(raw)));
-    keep = reinterpret_cast<float4*>(take(KEEP ? kRows<T> * kThreads * sizeof(float4) : 0));
-    sa = reinterpret_cast<float*>(take(kThreads * kCh * sizeof(float)));
-    sh = reinterpret_cast<float*>(take(kThreads * kCh * sizeof(float)));
-    parts = reinterpret_cast<float2*>(take(kThreads * sizeof(float2)));
-    state = reinterpret_cast<float*>(take(64 * sizeof(float)));
-    starts = reinterpret_cast<int32_t*>(take(g.tile_rows * sizeof(int32_t)));
-    ends = reinterpret_cast<int32_t*>(take(g.tile_rows * sizeof(int32_t)));
-  }
-  __device__ raw* slot(int input, int i) { return slots + (input * kRows<T> + i) * kThreads + threadIdx.x; }
-};
-
-// Where a ticket's tile lies and this thread in it.
-struct Spot {
-  int64_t j, tile, r0;  // order of processing, number, this thread's first row
-  int part, col;
-  bool on;
-};
-
-__device__ __forceinline__ Spot spot_of(const Params& p, uint32_t ticket, int sub, int lc, int rows_each) {
-  Spot s;
-  s.j = ticket / p.geo.across;
-  s.part = static_cast<int>(ticket - s.j * p.geo.across);
-  s.tile = p.up ? p.geo.tiles - 1 - s.j : s.j;
-  s.col = s.part * p.geo.width + lc;
-  s.on = sub < p.geo.subs && s.col < p.geo.cols;
-  s.r0 = s.tile * p.geo.tile_rows + static_cast<int64_t>(sub) * rows_each;
-  return s;
-}
-
-template <class T, int N>
-__device__ __forceinline__ void fetch_rows(const Params& p, const Spot& s, const void* base, Smem<T, N, N == 3>& sm,
-                                           int input) {
-  using raw = typename Quad<T>::raw;
-  const raw* src = static_cast<const raw*>(base);
-#pragma unroll
-  for (int i = 0; i < kRows<T>; ++i) {
-    const bool there = s.on && s.r0 + i < p.rows && src != nullptr;
-    fetch<T>(sm.slot(input, i), there ? src + (s.r0 + i) * p.geo.cols + s.col : static_cast<const raw*>(p.x), there);
-  }
-}
-
-template <class T>
-__global__ void __launch_bounds__(kThreads, 2) scan_forward_kernel(Params p) {
-  using Q = Quad<T>;
-  constexpr int R = kRows<T>;
-  extern __shared__ __align__(16) char smem_raw[];
-  __shared__ uint32_t next_ticket;
-  Smem<T, 2, false> sm(smem_raw, p.geo);
-  const int sub = threadIdx.x / p.geo.width, lc = threadIdx.x - sub * p.geo.width;
-  const int chans = p.geo.width * kCh, slot = sub * chans + lc * kCh;
-  const uint32_t tickets = static_cast<uint32_t>(p.geo.tiles * p.geo.across);
-  TileSegments ts;
-  ts.starts = sm.starts;
-  ts.ends = sm.ends;
-  ts.lo = clamp64(p.off[0], 0, p.rows);
-  ts.hi = clamp64(p.off[p.nseg], ts.lo, p.rows);
-
-  if (threadIdx.x == 0) next_ticket = atomicAdd(p.counter, 1u);
-  __syncthreads();
-  uint32_t ticket = next_ticket;
-  Spot s = spot_of(p, ticket, sub, lc, R);
-  if (ticket < tickets) {
-    fetch_rows<T, 2>(p, s, p.gate, sm, 0);
-    fetch_rows<T, 2>(p, s, p.x, sm, 1);
-  }
-  fetch_commit();
-  while (ticket < tickets) {
-    __syncthreads();  // everyone has read next_ticket
-    if (threadIdx.x == 0) next_ticket = atomicAdd(p.counter, 1u);
-    find_segments(p, s.tile, ts);
-    const uint32_t ahead = next_ticket;
-    const int64_t origin = clamp64(__ldcg(p.origin + s.tile), 0, s.tile);
-    fetch_wait<0>();
-
-    float a[R][kCh], u[R][kCh];
-    float pa[kCh], ph[kCh];
-#pragma unroll
-    for (int c = 0; c < kCh; ++c) {
-      pa[c] = 1.0f;
-      ph[c] = 0.0f;
+    typename P::raw g[kBlock], x[kBlock], d[kBlock];
+    int b0 = (n - 1) / kBlock * kBlock;
+    fetch(b0, g, x, d);
+    float2 before = load2(p.saved, (r0 + b0) / kBlock, p.channels, ch);
+    // The segment of the current row (with rows; -1 when none is left), its
+    // first row and the row behind its last, from r0.
+    int64_t seg = p.edge_seg[j];
+    int begin = seg >= 0 ? rel(__ldg(p.off + seg)) : -1;
+    int end = seg >= 0 ? rel(__ldg(p.off + seg + 1)) : -1;
+    float2 e = make_float2(0.0f, 0.0f);
+    if (seg >= 0) {
+      const int64_t end64 = clamp64(__ldg(p.off + seg + 1), 0, p.rows);
+      if (end64 > r0 + n) e = entering(p, j, (end64 - 1) / p.chunk_rows, pair, true);
     }
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-      float xv[kCh], gv[kCh];
-      Q::unpack(*sm.slot(0, i), gv);
-      Q::unpack(*sm.slot(1, i), xv);
-      const bool inside = s.r0 + i >= ts.lo && s.r0 + i < ts.hi;
-      const int32_t seg = s.on ? ts.starts[sub * R + i] : -1;
-      const bool restart = seg >= 0 || !inside;
-#pragma unroll
-      for (int c = 0; c < kCh; ++c) {
-        float av, keep;
-        gate_pair(gv[c], &av, &keep);
-        float uv = keep * xv[c];
-        if (seg >= 0 && p.initial != nullptr) uv = fmaf(av, __ldg(p.initial + seg * p.channels + s.col * kCh + c), uv);
-        a[i][c] = restart ? -1.0f : av;
-        u[i][c] = inside ? uv : 0.0f;
-        ph[c] = restart ? u[i][c] : fmaf(av, ph[c], uv);
-        pa[c] = (restart || pa[c] < 0.0f) ? -1.0f : pa[c] * av;
+    for (; b0 >= 0; b0 -= kBlock) {
+      typename P::raw gn[kBlock], xn[kBlock], dn[kBlock];
+      float2 before_next = make_float2(0.0f, 0.0f);
+      if (b0 > 0) {
+        fetch(b0 - kBlock, gn, xn, dn);
+        before_next = load2(p.saved, (r0 + b0) / kBlock - 1, p.channels, ch);
       }
-    }
-    // The next tile's rows into the slots just read.
-    const Spot ns = spot_of(p, ahead, sub, lc, R);
-    if (ahead < tickets) {
-      fetch_rows<T, 2>(p, ns, p.gate, sm, 0);
-      fetch_rows<T, 2>(p, ns, p.x, sm, 1);
-    }
-    fetch_commit();
-    if (sub < p.geo.subs) {
-#pragma unroll
-      for (int c = 0; c < kCh; ++c) {
-        sm.sa[slot + c] = pa[c];
-        sm.sh[slot + c] = ph[c];
+      // Which rows of the block start a segment, and the segment of the first.
+      uint32_t starts = 0;
+      int64_t low = seg;
+      int b = begin;
+      while (low >= 0 && b >= b0) {
+        if (b < b0 + kBlock) starts |= 1u << (b - b0);
+        do {
+          --low;
+        } while (low >= 0 && __ldg(p.off + low) >= __ldg(p.off + low + 1));
+        b = low >= 0 ? rel(__ldg(p.off + low)) : -1;
       }
-    }
-    __syncthreads();
-    Chain chain(p, sm.parts, sm.state, s.part);
-    float2 ah = make_float2(1.0f, 0.0f);
-    if (threadIdx.x < chans) compose(sm.sa, sm.sh, chans, p.geo.subs, false, threadIdx.x, &ah.x, &ah.y);
-    chain.publish(s.j, ah);
-    chain.enter_tile(s.j, origin, ah);
-    if (p.save != nullptr && threadIdx.x < chans && chain.gch < p.channels) {
-      p.save[s.tile * p.channels + chain.gch] = sm.state[threadIdx.x];
-    }
-    if (s.on) {
-      float st[kCh];
+      // The forward states again: q = (h_{t-1} - x_t) a_t (1 - a_t).
+      float2 a[kBlock], keep[kBlock], q[kBlock];
+      float2 st = before;
 #pragma unroll
-      for (int c = 0; c < kCh; ++c) st[c] = enter(sm.sa[slot + c], sm.sh[slot + c], sm.state[lc * kCh + c]);
+      for (int i = 0; i < kBlock; ++i) {
+        if (b0 + i < n) {
+          if ((starts >> i) & 1u) {
+            do {
+              ++low;
+            } while (__ldg(p.off + low) >= __ldg(p.off + low + 1));
+            st = p.initial != nullptr ? load2(p.initial, low, p.channels, ch) : make_float2(0.0f, 0.0f);
+          }
+          const float2 gv = P::unpack(g[i]), xv = P::unpack(x[i]);
+          gate_pair(gv.x, &a[i].x, &keep[i].x);
+          gate_pair(gv.y, &a[i].y, &keep[i].y);
+          q[i].x = (st.x - xv.x) * (a[i].x * keep[i].x);
+          q[i].y = (st.y - xv.y) * (a[i].y * keep[i].y);
+          st.x = fmaf(a[i].x, st.x, keep[i].x * xv.x);
+          st.y = fmaf(a[i].y, st.y, keep[i].y * xv.y);
+        }
+      }
 #pragma unroll
-      for (int i = 0; i < R; ++i) {
-        if (s.r0 + i < p.rows) {
-#pragma unroll
-          for (int c = 0; c < kCh; ++c) st[c] = enter(a[i][c], u[i][c], st[c]);
-          if (p.h != nullptr) static_cast<typename Q::raw*>(p.h)[(s.r0 + i) * p.geo.cols + s.col] = Q::pack(st);
-          const int32_t seg = ts.ends[sub * R + i];
-          if (seg >= 0 && p.final != nullptr) {
-            *reinterpret_cast<float4*>(p.final + seg * p.channels + s.col * kCh) = make_float4(st[0], st[1], st[2], st[3]);
+      for (int i = kBlock - 1; i >= 0; --i) {
+        const int r = b0 + i;
+        if (r < n) {
+          const bool inside = r >= lo && r < hi;
+          if (r + 1 == end) {
+            e = p.grad_final != nullptr ? load2(p.grad_final, seg, p.channels, ch) : make_float2(0.0f, 0.0f);
+          }
+          const float2 dv = P::unpack(d[i]);
+          const float2 delta = make_float2(dv.x + e.x, dv.y + e.y);
+          e.x = inside ? a[i].x * delta.x : 0.0f;
+          e.y = inside ? a[i].y * delta.y : 0.0f;
+          const float2 dx = make_float2(inside ? keep[i].x * delta.x : 0.0f, inside ? keep[i].y * delta.y : 0.0f);
+          const float2 dg = make_float2(inside ? q[i].x * delta.x : 0.0f, inside ? q[i].y * delta.y : 0.0f);
+          static_cast<typename P::raw*>(p.dx)[(r0 + r) * p.pairs + pair] = P::pack(dx);
+          static_cast<typename P::raw*>(p.dgate)[(r0 + r) * p.pairs + pair] = P::pack(dg);
+          if ((starts >> i) & 1u) {  // this row is the segment's first: on to the one before
+            if (p.dinitial != nullptr) store2(p.dinitial, seg, p.channels, ch, e);
+            do {
+              --seg;
+            } while (seg >= 0 && __ldg(p.off + seg) >= __ldg(p.off + seg + 1));
+            end = seg >= 0 ? r : -1;
+            begin = seg >= 0 ? rel(__ldg(p.off + seg)) : -1;
           }
         }
       }
+#pragma unroll
+      for (int i = 0; i < kBlock; ++i) {
+        g[i] = gn[i];
+        x[i] = xn[i];
+        d[i] = dn[i];
+      }
+      before = before_next;
     }
-    ticket = ahead;
-    s = ns;
   }
-}
-
-template <class T>
-__global__ void __launch_bounds__(kThreads, 2) scan_backward_kernel(Params p) {
-  using Q = Quad<T>;
-  constexpr int R = kRows<T>;
-  extern __shared__ __align__(16) char smem_raw[];
-  __shared__ uint32_t next_ticket;
-  Smem<T, 3, true> sm(smem_raw, p.geo);
-  const int sub = threadIdx.x / p.geo.width, lc = threadIdx.x - sub * p.geo.width;
-  const int chans = p.geo.width * kCh, slot = sub * chans + lc * kCh;
-  const uint32_t tickets = static_cast<uint32_t>(p.geo.tiles * p.geo.across);
-  TileSegments ts;
-  ts.starts = sm.starts;
-  ts.ends = sm.ends;
-  ts.lo = clamp64(p.off[0], 0, p.rows);
-  ts.hi = clamp64(p.off[p.nseg], ts.lo, p.rows);
-
-  if (threadIdx.x == 0) next_ticket = atomicAdd(p.counter, 1u);
-  __syncthreads();
-  uint32_t ticket = next_ticket;
-  Spot s = spot_of(p, ticket, sub, lc, R);
-  if (ticket < tickets) {
-    fetch_rows<T, 3>(p, s, p.gate, sm, 0);
-    fetch_rows<T, 3>(p, s, p.x, sm, 1);
-  }
-  fetch_commit();
-  if (ticket < tickets) fetch_rows<T, 3>(p, s, p.grad, sm, 2);
-  fetch_commit();
-  while (ticket < tickets) {
-    __syncthreads();
-    if (threadIdx.x == 0) next_ticket = atomicAdd(p.counter, 1u);
-    find_segments(p, s.tile, ts);
-    const uint32_t ahead = next_ticket;
-    const Spot ns = spot_of(p, ahead, sub, lc, R);
-    const int64_t origin = clamp64(__ldcg(p.origin + s.tile), s.tile, p.geo.tiles - 1);
-    fetch_wait<1>();  // gate and x are here, grad may still be on its way
-
-    // The forward states of this tile again.
-    float a[R][kCh], q[R][kCh];
-    float pa[kCh], ph[kCh];
-#pragma unroll
-    for (int c = 0; c < kCh; ++c) {
-      pa[c] = 1.0f;
-      ph[c] = 0.0f;
-    }
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-      float xv[kCh], gv[kCh], kv[kCh];
-      Q::unpack(*sm.slot(0, i), gv);
-      Q::unpack(*sm.slot(1, i), xv);
-      const bool inside = s.r0 + i >= ts.lo && s.r0 + i < ts.hi;
-      const int32_t seg = s.on ? ts.starts[sub * R + i] : -1;
-      const bool restart = seg >= 0 || !inside;
-#pragma unroll
-      for (int c = 0; c < kCh; ++c) {
-        gate_pair(gv[c], &a[i][c], &kv[c]);
-        float uv = kv[c] * xv[c];
-        if (seg >= 0 && p.initial != nullptr) {
-          uv = fmaf(a[i][c], __ldg(p.initial + seg * p.channels + s.col * kCh + c), uv);
-        }
-        ph[c] = restart ? (inside ? uv : 0.0f) : fmaf(a[i][c], ph[c], uv);
-        pa[c] = (restart || pa[c] < 0.0f) ? -1.0f : pa[c] * a[i][c];
-      }
-      sm.keep[i * kThreads + threadIdx.x] = make_float4(kv[0], kv[1], kv[2], kv[3]);
-    }
-    if (sub < p.geo.subs) {
-#pragma unroll
-      for (int c = 0; c < kCh; ++c) {
-        sm.sa[slot + c] = pa[c];
-        sm.sh[slot + c] = ph[c];
-      }
-    }
-    __syncthreads();
-    float2 ah = make_float2(1.0f, 0.0f);
-    if (threadIdx.x < chans) compose(sm.sa, sm.sh, chans, p.geo.subs, false, threadIdx.x, &ah.x, &ah.y);
-    __syncthreads();
-    float st[kCh];
-#pragma unroll
-    for (int c = 0; c < kCh; ++c) {
-      st[c] = s.on ? enter(sm.sa[slot + c], sm.sh[slot + c], __ldg(p.saved + s.tile * p.channels + s.col * kCh + c))
-                   : 0.0f;
-    }
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-      float xv[kCh];
-      Q::unpack(*sm.slot(1, i), xv);
-      const float4 k4 = sm.keep[i * kThreads + threadIdx.x];
-      const float kv[kCh] = {k4.x, k4.y, k4.z, k4.w};
-      const int32_t seg = s.on ? ts.starts[sub * R + i] : -1;
-#pragma unroll
-      for (int c = 0; c < kCh; ++c) {
-        if (seg >= 0) st[c] = p.initial != nullptr ? __ldg(p.initial + seg * p.channels + s.col * kCh + c) : 0.0f;
-        q[i][c] = (st[c] - xv[c]) * (a[i][c] * kv[c]);
-        st[c] = fmaf(a[i][c], st[c], kv[c] * xv[c]);
-      }
-    }
-    if (ahead < tickets) {  // gate and x of the next tile into the slots just read
-      fetch_rows<T, 3>(p, ns, p.gate, sm, 0);
-      fetch_rows<T, 3>(p, ns, p.x, sm, 1);
-    }
-    fetch_commit();
-    fetch_wait<1>();  // grad of this tile
-
-    // e_t = a_t (d_t + e_{t+1}) from the last row of the thread to its first.
-    float pe[kCh];
-#pragma unroll
-    for (int c = 0; c < kCh; ++c) {
-      pa[c] = 1.0f;
-      pe[c] = 0.0f;
-    }
-#pragma unroll
-    for (int i = R - 1; i >= 0; --i) {
-      float dv[kCh];
-      Q::unpack(*sm.slot(2, i), dv);
-      const int32_t seg = s.on ? ts.ends[sub * R + i] : -1;
-      const bool inside = s.r0 + i >= ts.lo && s.r0 + i < ts.hi;
-      const bool restart = seg >= 0 || !inside;
-#pragma unroll
-      for (int c = 0; c < kCh; ++c) {
-        if (seg >= 0 && p.grad_final != nullptr) dv[c] += __ldg(p.grad_final + seg * p.channels + s.col * kCh + c);
-        pe[c] = inside ? a[i][c] * (restart ? dv[c] : dv[c] + pe[c]) : 0.0f;
-        pa[c] = (restart || pa[c] < 0.0f) ? -1.0f : pa[c] * a[i][c];
-      }
-    }
-    __syncthreads();  // the forward composition has been read
-    if (sub < p.geo.subs) {
-#pragma unroll
-      for (int c = 0; c < kCh; ++c) {
-        sm.sa[slot + c] = pa[c];
-        sm.sh[slot + c] = pe[c];
-      }
-    }
-    __syncthreads();
-    Chain chain(p, sm.parts, sm.state, s.part);
-    ah = make_float2(1.0f, 0.0f);
-    if (threadIdx.x < chans) compose(sm.sa, sm.sh, chans, p.geo.subs, true, threadIdx.x, &ah.x, &ah.y);
-    chain.publish(s.j, ah);
-    chain.enter_tile(s.j, p.geo.tiles - 1 - origin, ah);
-    if (s.on) {
-      float e[kCh];
-#pragma unroll
-      for (int c = 0; c < kCh; ++c) e[c] = enter(sm.sa[slot + c], sm.sh[slot + c], sm.state[lc * kCh + c]);
-#pragma unroll
-      for (int i = R - 1; i >= 0; --i) {
-        if (s.r0 + i < p.rows) {
-          const bool inside = s.r0 + i >= ts.lo && s.r0 + i < ts.hi;
-          const int32_t end = ts.ends[sub * R + i], seg = ts.starts[sub * R + i];
-          const float4 k4 = sm.keep[i * kThreads + threadIdx.x];
-          const float kv[kCh] = {k4.x, k4.y, k4.z, k4.w};
-          float dv[kCh], dx[kCh], dg[kCh];
-          Q::unpack(*sm.slot(2, i), dv);
-#pragma unroll
-          for (int c = 0; c < kCh; ++c) {
-            if (end >= 0) e[c] = p.grad_final != nullptr ? __ldg(p.grad_final + end * p.channels + s.col * kCh + c) : 0.0f;
-            const float delta = dv[c] + e[c];
-            e[c] = inside ? a[i][c] * delta : 0.0f;
-            dx[c] = inside ? kv[c] * delta : 0.0f;
-            dg[c] = inside ? delta * q[i][c] : 0.0f;
-          }
-          static_cast<typename Q::raw*>(p.dx)[(s.r0 + i) * p.geo.cols + s.col] = Q::pack(dx);
-          static_cast<typename Q::raw*>(p.dgate)[(s.r0 + i) * p.geo.cols + s.col] = Q::pack(dg);
-          if (seg >= 0 && p.dinitial != nullptr) {
-            *reinterpret_cast<float4*>(p.dinitial + seg * p.channels + s.col * kCh) = make_float4(e[0], e[1], e[2], e[3]);
-          }
-        }
-      }
-    }
-    if (ahead < tickets) fetch_rows<T, 3>(p, ns, p.grad, sm, 2);
-    fetch_commit();
-    ticket = ahead;
-    s = ns;
-  }
+  if (p.dinitial != nullptr) fill_empty(p, p.grad_final, p.dinitial);
 }
 
 template <class T>
@@ -740,59 +545,67 @@ int check_shape(const char* who, int64_t rows, int64_t channels, int64_t nseg, i
                 std::string(who) + ": need rows >= 0, segments >= 0, channels a positive multiple of 4, dtype fp32 or "
                                    "bf16");
   }
-  if (channels > (int64_t(1) << 20) || nseg >= (int64_t(1) << 31) || rows > (int64_t(1) << 40) ||
-      geometry(rows, channels, dtype).tiles * geometry(rows, channels, dtype).across >= (int64_t(1) << 31)) {
+  if (channels > (int64_t(1) << 20) || nseg >= (int64_t(1) << 31) - 1 || rows > (int64_t(1) << 40) ||
+      rows * channels > (int64_t(1) << 42)) {
     return fail(DGFX_ERR_UNSUPPORTED, std::string(who) + ": sizes out of range");
   }
   return DGFX_OK;
 }
 
-// Quads are loaded whole, fp32 states as 16-byte vectors.
+// Quads of x, gate, h and their gradients are loaded whole.
 bool quad_aligned(const void* p, int dtype) {
   return (reinterpret_cast<uintptr_t>(p) & (dtype == DGFX_F32 ? 15u : 7u)) == 0;
 }
 
-size_t carve(void* base, size_t cap, const Geometry& g, int64_t channels, Params* p, bool* ok) {
+// Chunk height: enough threads to fill the GPU (about 1024 per SM), at
+// least two blocks of rows, at most 256 rows (a taller chunk saves nothing: its
+// edge already costs under 1/8 of its rows where windows are short).
+int32_t chunk_rows_of(int64_t rows, int64_t channels) {
+  const int64_t full = static_cast<int64_t>(kSms) * 1024;
+  const int64_t want = ceil_div(rows * (channels / 2), full);
+  return static_cast<int32_t>(ceil_div(clamp64(want, 16, 256), kBlock) * kBlock);
+}
+
+size_t carve(void* base, size_t cap, int64_t rows, int64_t channels, Params* p, bool* ok) {
   Arena arena(base, cap);
-  const int64_t groups = ceil_div(g.tiles, kGroup), supers = ceil_div(g.tiles, kSuper);
-  p->tile_ah = arena.take<float2>(static_cast<size_t>(g.tiles) * channels);
-  p->group_ah = arena.take<float2>(static_cast<size_t>(groups) * channels);
-  p->super_state = arena.take<float>(static_cast<size_t>(supers) * channels);
-  p->clear_words = (g.tiles + groups + supers) * g.across + 2;
-  p->tile_flag = arena.take<uint32_t>(static_cast<size_t>(p->clear_words));
-  p->first_seg = arena.take<int32_t>(static_cast<size_t>(g.tiles));
-  p->origin = arena.take<int32_t>(static_cast<size_t>(g.tiles));
-  if (base != nullptr) {
-    p->group_flag = p->tile_flag + g.tiles * g.across;
-    p->super_flag = p->group_flag + groups * g.across;
-    p->counter = p->super_flag + supers * g.across;
-    p->aborted = p->counter + 1;
-  }
+  p->rows = rows;
+  p->channels = static_cast<int32_t>(channels);
+  p->pairs = static_cast<int32_t>(channels / 2);
+  p->chunk_rows = chunk_rows_of(rows, channels);
+  p->chunks = ceil_div(rows, p->chunk_rows);
+  p->groups = ceil_div(p->chunks, kLevel);
+  p->supers = ceil_div(p->groups, kLevel);
+  p->chunk_ah = arena.take<float4>(static_cast<size_t>(p->chunks) * p->pairs);
+  p->group_ah = arena.take<float4>(static_cast<size_t>(p->groups) * p->pairs);
+  p->super_ah = arena.take<float4>(static_cast<size_t>(p->supers) * p->pairs);
+  p->edge_seg = arena.take<int32_t>(static_cast<size_t>(p->chunks));
   *ok = arena.ok();
   return arena.used;
 }
 
-unsigned plan_grid(const Params& p) {
-  const int64_t items = std::max(std::max(p.clear_words, p.geo.tiles), p.nseg * 32);
-  return static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(ceil_div(items, 256), kSms * 8)));
-}
+unsigned grid_of(int64_t items) { return static_cast<unsigned>(std::max<int64_t>(1, ceil_div(items, kThreads))); }
 
-template <class T, bool BACKWARD>
-int launch(const Params& p, cudaStream_t stream) {
-  auto kernel = BACKWARD ? scan_backward_kernel<T> : scan_forward_kernel<T>;
-  const size_t smem = BACKWARD ? Smem<T, 3, true>::bytes(p.geo) : Smem<T, 2, false>::bytes(p.geo);
-  if (smem > 48 * 1024) {
-    static std::once_flag once[64];
-    int dev = 0;
-    DGFX_CUDA_TRY(cudaGetDevice(&dev));
-    cudaError_t err = cudaSuccess;
-    std::call_once(once[dev & 63], [&]() {
-      err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 112 * 1024);
-    });
-    DGFX_CUDA_TRY(err);
+template <class T>
+int launch(const Params& p, bool up, cudaStream_t stream) {
+  const unsigned grid = grid_of(p.chunks * p.pairs);
+  if (p.rows > 0) {
+    if (up) scan_chunk_up_kernel<T><<<grid, kThreads, 0, stream>>>(p);
+    else scan_chunk_kernel<T><<<grid, kThreads, 0, stream>>>(p);
+    // The forward pass has no edge behind the last chunk, the backward pass
+    // none above the first: those effects are not written, and no level that
+    // a chunk composes holds them.
+    if (p.groups > 1) {
+      scan_level_kernel<<<grid_of(p.groups * p.pairs), kThreads, 0, stream>>>(p.chunk_ah, p.chunks, p.pairs, up,
+                                                                             p.group_ah, p.groups);
+    }
+    if (p.supers > 1) {
+      scan_level_kernel<<<grid_of(p.supers * p.pairs), kThreads, 0, stream>>>(p.group_ah, p.groups, p.pairs, up,
+                                                                             p.super_ah, p.supers);
+    }
   }
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(p.geo.tiles * p.geo.across, 2 * kSms));
-  kernel<<<grid, kThreads, smem, stream>>>(p);
+  const unsigned apply = std::max(grid, grid_of(std::min<int64_t>(p.nseg, kSms * 2048)));  // segments without rows
+  if (up) scan_apply_up_kernel<T><<<apply, kThreads, 0, stream>>>(p);
+  else scan_apply_kernel<T><<<apply, kThreads, 0, stream>>>(p);
   DGFX_CUDA_TRY(cudaGetLastError());
   return DGFX_OK;
 }
@@ -802,14 +615,13 @@ int launch(const Params& p, cudaStream_t stream) {
 
 using namespace dgfx;
 
-extern "C" int dgfx_gated_scan_workspace_size(int64_t rows, int64_t channels, int dtype, size_t* workspace_bytes,
+extern "C" int dgfx_gated_scan_workspace_size(int64_t rows, int64_t channels, size_t* workspace_bytes,
                                               size_t* saved_bytes) {
-  DGFX_TRY(check_shape("dgfx_gated_scan_workspace_size", rows, channels, 0, dtype));
-  const Geometry g = geometry(rows, channels, dtype);
+  DGFX_TRY(check_shape("dgfx_gated_scan_workspace_size", rows, channels, 0, DGFX_F32));
   Params p{};
   bool ok;
-  if (workspace_bytes != nullptr) *workspace_bytes = carve(nullptr, 0, g, channels, &p, &ok);
-  if (saved_bytes != nullptr) *saved_bytes = static_cast<size_t>(g.tiles) * channels * sizeof(float);
+  if (workspace_bytes != nullptr) *workspace_bytes = carve(nullptr, 0, rows, channels, &p, &ok);
+  if (saved_bytes != nullptr) *saved_bytes = static_cast<size_t>(ceil_div(rows, kBlock)) * channels * sizeof(float);
   return DGFX_OK;
 }
 
@@ -823,16 +635,15 @@ extern "C" int dgfx_gated_scan(const void* d_x, const void* d_gate, int dtype, i
     return fail(DGFX_ERR_INVALID_ARGUMENT, "dgfx_gated_scan: null operand");
   }
   if (!quad_aligned(d_x, dtype) || !quad_aligned(d_gate, dtype) || !quad_aligned(d_h, dtype) ||
-      !quad_aligned(d_final, DGFX_F32)) {
+      !quad_aligned(d_initial, DGFX_F32) || !quad_aligned(d_final, DGFX_F32) || !quad_aligned(d_saved, DGFX_F32)) {
     return fail(DGFX_ERR_INVALID_ARGUMENT, "dgfx_gated_scan: operands must be aligned to 4 elements");
   }
   Params p{};
-  p.geo = geometry(rows, channels, dtype);
   bool ok = false;
-  carve(d_workspace, workspace_bytes, p.geo, channels, &p, &ok);
-  if (d_workspace == nullptr || !ok) return fail(DGFX_ERR_WORKSPACE, "dgfx_gated_scan: workspace too small");
-  p.err = dense_err_word();
-  if (p.err == nullptr) return fail(DGFX_ERR_CUDA, "dgfx_gated_scan: status word unavailable");
+  carve(d_workspace, workspace_bytes, rows, channels, &p, &ok);
+  if (rows > 0 && (d_workspace == nullptr || !ok)) {
+    return fail(DGFX_ERR_WORKSPACE, "dgfx_gated_scan: workspace too small");
+  }
   p.x = d_x;
   p.gate = d_gate;
   p.off = d_offsets;
@@ -840,13 +651,8 @@ extern "C" int dgfx_gated_scan(const void* d_x, const void* d_gate, int dtype, i
   p.h = d_h;
   p.final = d_final;
   p.save = d_saved;
-  p.rows = rows;
-  p.channels = channels;
   p.nseg = nseg;
-  scan_plan_kernel<<<plan_grid(p), 256, 0, stream>>>(p, d_initial, d_final);
-  DGFX_CUDA_TRY(cudaGetLastError());
-  if (rows == 0) return DGFX_OK;
-  return dtype == DGFX_F32 ? launch<float, false>(p, stream) : launch<__nv_bfloat16, false>(p, stream);
+  return dtype == DGFX_F32 ? launch<float>(p, false, stream) : launch<__nv_bfloat16>(p, false, stream);
 }
 
 extern "C" int dgfx_gated_scan_backward(const void* d_x, const void* d_gate, int dtype, int64_t rows, int64_t channels,
@@ -861,16 +667,17 @@ extern "C" int dgfx_gated_scan_backward(const void* d_x, const void* d_gate, int
     return fail(DGFX_ERR_INVALID_ARGUMENT, "dgfx_gated_scan_backward: null operand");
   }
   if (!quad_aligned(d_x, dtype) || !quad_aligned(d_gate, dtype) || !quad_aligned(d_grad_h, dtype) ||
-      !quad_aligned(d_dx, dtype) || !quad_aligned(d_dgate, dtype) || !quad_aligned(d_dinitial, DGFX_F32)) {
+      !quad_aligned(d_dx, dtype) || !quad_aligned(d_dgate, dtype) || !quad_aligned(d_initial, DGFX_F32) ||
+      !quad_aligned(d_saved, DGFX_F32) || !quad_aligned(d_grad_final, DGFX_F32) ||
+      !quad_aligned(d_dinitial, DGFX_F32)) {
     return fail(DGFX_ERR_INVALID_ARGUMENT, "dgfx_gated_scan_backward: operands must be aligned to 4 elements");
   }
   Params p{};
-  p.geo = geometry(rows, channels, dtype);
   bool ok = false;
-  carve(d_workspace, workspace_bytes, p.geo, channels, &p, &ok);
-  if (d_workspace == nullptr || !ok) return fail(DGFX_ERR_WORKSPACE, "dgfx_gated_scan_backward: workspace too small");
-  p.err = dense_err_word();
-  if (p.err == nullptr) return fail(DGFX_ERR_CUDA, "dgfx_gated_scan_backward: status word unavailable");
+  carve(d_workspace, workspace_bytes, rows, channels, &p, &ok);
+  if (rows > 0 && (d_workspace == nullptr || !ok)) {
+    return fail(DGFX_ERR_WORKSPACE, "dgfx_gated_scan_backward: workspace too small");
+  }
   p.x = d_x;
   p.gate = d_gate;
   p.off = d_offsets;
@@ -881,14 +688,8 @@ extern "C" int dgfx_gated_scan_backward(const void* d_x, const void* d_gate, int
   p.dgate = d_dgate;
   p.dinitial = d_dinitial;
   p.saved = d_saved;
-  p.rows = rows;
-  p.channels = channels;
   p.nseg = nseg;
-  p.up = 1;
-  scan_plan_kernel<<<plan_grid(p), 256, 0, stream>>>(p, d_grad_final, d_dinitial);
-  DGFX_CUDA_TRY(cudaGetLastError());
-  if (rows == 0) return DGFX_OK;
-  return dtype == DGFX_F32 ? launch<float, true>(p, stream) : launch<__nv_bfloat16, true>(p, stream);
+  return dtype == DGFX_F32 ? launch<float>(p, true, stream) : launch<__nv_bfloat16>(p, true, stream);
 }
 
 extern "C" int dgfx_gated_scan_step(const void* d_x, const void* d_gate, int dtype, int64_t n, int64_t channels,

@@ -108,8 +108,8 @@ def test_channels(cuda, c, dtype):
 
 
 def test_one_window_over_many_tiles(cuda):
-    """A window that crosses tiles, groups of 32 and supergroups of 1024 tiles
-    (64 rows of fp32 each at this width), short ones on either side."""
+    """A window that crosses chunks of 16 rows, groups of 32 chunks and supergroups
+    of 1024, short ones on either side."""
     off = _offsets([100, 70000, 50, 0, 3])
     x, gate, dh, h0, df = _inputs(70153, 64, 5, torch.float32, 12)
     _check(x, gate, off, h0, dh, df)
