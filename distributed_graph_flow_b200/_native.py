@@ -113,7 +113,7 @@ SIGNATURES = {
                                        _vp, _vp, _sz, _vp]),
     "dgfx_segment_group_norm_backward": (_int, [_vp, _vp, _int, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i32,
                                                 _vp, _vp, _vp, _vp, _sz, _vp]),
-    "dgfx_gated_scan_workspace_size": (_int, [_i64, _i64, ctypes.POINTER(_sz), ctypes.POINTER(_sz)]),
+    "dgfx_gated_scan_workspace_size": (_int, [_i64, _i64, _int, ctypes.POINTER(_sz), ctypes.POINTER(_sz)]),
     "dgfx_gated_scan": (_int, [_vp, _vp, _int, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "dgfx_gated_scan_backward": (_int, [_vp, _vp, _int, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                         _sz, _vp]),

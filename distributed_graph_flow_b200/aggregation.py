@@ -576,9 +576,9 @@ def segment_group_norm_backward(grad, x, offsets, mean, rstd, weight=None, bias=
     return dx, dw, db
 
 
-def _scan_sizes(rows: int, channels: int):
+def _scan_sizes(rows: int, channels: int, code: int):
     need, saved = ctypes.c_size_t(), ctypes.c_size_t()
-    _native.check(_native.lib().dgfx_gated_scan_workspace_size(rows, channels, ctypes.byref(need),
+    _native.check(_native.lib().dgfx_gated_scan_workspace_size(rows, channels, code, ctypes.byref(need),
                                                                ctypes.byref(saved)))
     return need.value, saved.value // 4
 
@@ -606,7 +606,7 @@ def gated_scan(x, gate, offsets, initial=None, return_sequence: bool = True, ret
     nseg = _layer_offsets(who, offsets)
     if initial is not None:
         _layer_input(who, "initial", initial, (nseg, channels), (torch.float32,))
-    need, saved_n = _scan_sizes(rows, channels)
+    need, saved_n = _scan_sizes(rows, channels, code)
     with _LayerLaunch(who, stream, x, gate, offsets, initial) as sh:
         h = torch.empty_like(x) if return_sequence else None
         final = torch.empty((nseg, channels), dtype=torch.float32, device=x.device)
@@ -635,7 +635,7 @@ def gated_scan_backward(grad, x, gate, offsets, saved, initial=None, grad_final=
     for name, t in (("initial", initial), ("grad_final", grad_final)):
         if t is not None:
             _layer_input(who, name, t, (nseg, channels), (torch.float32,))
-    need, saved_n = _scan_sizes(rows, channels)
+    need, saved_n = _scan_sizes(rows, channels, code)
     _layer_input(who, "saved", saved, (saved_n,), (torch.float32,))
     with _LayerLaunch(who, stream, x, grad, gate, offsets, saved, initial, grad_final) as sh:
         dx, dgate = torch.empty_like(x), torch.empty_like(gate)

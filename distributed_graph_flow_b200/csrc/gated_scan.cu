@@ -51,7 +51,9 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kCh = 4;     // channels per thread of the single step
-constexpr int kBlock = 8;  // rows loaded at a time; rows between saved states
+// Rows loaded at a time (32 bytes of each input); rows between saved states.
+template <class T>
+constexpr int kBlock = sizeof(T) == 2 ? 8 : 4;
 constexpr int kLevel = 32;
 constexpr int kSms = 148;
 
@@ -78,14 +80,33 @@ struct Pair<__nv_bfloat16> {
   __device__ static __forceinline__ raw zero() { return 0u; }
 };
 
-// a = sigmoid(g) and 1 - a, both to full relative precision: e^-|g| never
-// overflows, and neither comes from a subtraction.
+// a = sigmoid(g) and 1 - a = e^-g a, neither from a subtraction. The exponent
+// is held above -80, where a is 2e-35, so that e^-g stays finite (a maximum
+// that keeps NaN).
 __device__ __forceinline__ void gate_pair(float g, float* a, float* keep) {
-  const float e = __expf(-fabsf(g));
-  const float big = __fdividef(1.0f, 1.0f + e), small = e * big;
-  *a = g >= 0.0f ? big : small;
-  *keep = g >= 0.0f ? small : big;
+  float low, r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(low) : "f"(g), "f"(-80.0f));
+  const float e = __expf(-low);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  *a = r;
+  *keep = e * r;
 }
+
+// One row's coefficients and inputs for two channels.
+template <class T>
+struct Row {
+  float2 a, keep, x;
+  __device__ __forceinline__ Row(typename Pair<T>::raw gate, typename Pair<T>::raw in) {
+    const float2 g = Pair<T>::unpack(gate);
+    x = Pair<T>::unpack(in);
+    gate_pair(g.x, &a.x, &keep.x);
+    gate_pair(g.y, &a.y, &keep.y);
+  }
+  __device__ __forceinline__ void step(float2& h) const {
+    h.x = fmaf(a.x, h.x, keep.x * x.x);
+    h.y = fmaf(a.y, h.y, keep.y * x.y);
+  }
+};
 
 struct Params {
   const void* x;
@@ -139,14 +160,14 @@ struct Effect {
   }
   // Items `from`, from + dir, .. (n of them) of a table, in that order.
   __device__ void then_items(const float4* __restrict__ table, int64_t from, int dir, int64_t n, int64_t pitch) {
-    for (int64_t i = 0; i < n; i += 8) {
-      float4 t[8];
+    for (int64_t i = 0; i < n; i += 4) {
+      float4 t[4];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
+      for (int k = 0; k < 4; ++k) {
         if (i + k < n) t[k] = __ldg(table + (from + dir * (i + k)) * pitch);
       }
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
+      for (int k = 0; k < 4; ++k) {
         if (i + k < n) then(t[k]);
       }
     }
@@ -160,9 +181,32 @@ __device__ __forceinline__ void store2(float* base, int64_t row, int channels, i
   *reinterpret_cast<float2*>(base + row * channels + ch) = v;
 }
 
+// Chunk and pair of this thread (32-bit division where the grid allows).
+struct Spot {
+  int64_t j;
+  int pair, ch;
+  __device__ explicit Spot(const Params& p) {
+    const int64_t t = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+    if (t <= 0x7fffffff) {
+      const uint32_t q = static_cast<uint32_t>(t) / static_cast<uint32_t>(p.pairs);
+      j = q;
+      pair = static_cast<int>(static_cast<uint32_t>(t) - q * static_cast<uint32_t>(p.pairs));
+    } else {
+      j = t / p.pairs;
+      pair = static_cast<int>(t - j * p.pairs);
+    }
+    ch = 2 * pair;
+  }
+};
+
+// This thread's column of an input or output, from row r0.
 template <class T>
-__device__ __forceinline__ typename Pair<T>::raw load_pair(const void* base, int64_t row, int pairs, int pair) {
-  return __ldg(static_cast<const typename Pair<T>::raw*>(base) + row * pairs + pair);
+__device__ __forceinline__ const typename Pair<T>::raw* column(const void* base, const Params& p, int64_t r0, int pair) {
+  return static_cast<const typename Pair<T>::raw*>(base) + r0 * p.pairs + pair;
+}
+template <class T>
+__device__ __forceinline__ typename Pair<T>::raw* column(void* base, const Params& p, int64_t r0, int pair) {
+  return static_cast<typename Pair<T>::raw*>(base) + r0 * p.pairs + pair;
 }
 
 // ---------------------------------------------------------------------------
@@ -172,44 +216,42 @@ __device__ __forceinline__ typename Pair<T>::raw load_pair(const void* base, int
 // row of chunk j: it notes where that row stands and writes the effect of
 // chunk j - 1 on the segment that crosses the edge.
 template <class T>
-__global__ void __launch_bounds__(kThreads) scan_chunk_kernel(Params p) {
+__global__ void __launch_bounds__(kThreads, 4) scan_chunk_kernel(Params p) {
+  constexpr int B = kBlock<T>;
   using P = Pair<T>;
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  const int64_t j = t / p.pairs;
-  const int pair = static_cast<int>(t - j * p.pairs);
-  if (j >= p.chunks) return;
-  const int64_t edge = j * p.chunk_rows;
+  const Spot at(p);
+  if (at.j >= p.chunks) return;
+  const int64_t edge = at.j * p.chunk_rows;
   const int64_t seg = last_at_most(p.off, p.nseg, edge);
-  if (pair == 0) p.edge_seg[j] = static_cast<int32_t>(seg);
-  if (j == 0) return;
+  if (at.pair == 0) p.edge_seg[at.j] = static_cast<int32_t>(seg);
+  if (at.j == 0) return;
   Effect f;
   f.v = make_float4(-1.0f, 0.0f, -1.0f, 0.0f);
   if (seg >= 0 && seg < p.nseg) {
     const int64_t first = edge - p.chunk_rows, begin = __ldg(p.off + seg);
     const int64_t from = begin > first ? begin : first;
-    if (from < edge) {
+    const int n = static_cast<int>(edge - from);
+    if (n > 0) {
       float2 a = make_float2(1.0f, 1.0f), h = make_float2(0.0f, 0.0f);
-      if (begin >= first && p.initial != nullptr) h = load2(p.initial, seg, p.channels, 2 * pair);
-      for (int64_t r = from; r < edge; r += kBlock) {
-        typename P::raw g[kBlock], x[kBlock];
+      if (begin >= first && p.initial != nullptr) h = load2(p.initial, seg, p.channels, at.ch);
+      const auto* gp = column<T>(p.gate, p, from, at.pair);
+      const auto* xp = column<T>(p.x, p, from, at.pair);
+      for (int r = 0; r < n; r += B) {
+        typename P::raw g[B], x[B];
 #pragma unroll
-        for (int i = 0; i < kBlock; ++i) {
-          if (r + i < edge) {
-            g[i] = load_pair<T>(p.gate, r + i, p.pairs, pair);
-            x[i] = load_pair<T>(p.x, r + i, p.pairs, pair);
+        for (int i = 0; i < B; ++i) {
+          if (r + i < n) {
+            g[i] = __ldg(gp + (r + i) * p.pairs);
+            x[i] = __ldg(xp + (r + i) * p.pairs);
           }
         }
 #pragma unroll
-        for (int i = 0; i < kBlock; ++i) {
-          if (r + i < edge) {
-            const float2 gv = P::unpack(g[i]), xv = P::unpack(x[i]);
-            float2 av, kv;
-            gate_pair(gv.x, &av.x, &kv.x);
-            gate_pair(gv.y, &av.y, &kv.y);
-            h.x = fmaf(av.x, h.x, kv.x * xv.x);
-            h.y = fmaf(av.y, h.y, kv.y * xv.y);
-            a.x *= av.x;
-            a.y *= av.y;
+        for (int i = 0; i < B; ++i) {
+          if (r + i < n) {
+            const Row<T> row(g[i], x[i]);
+            row.step(h);
+            a.x *= row.a.x;
+            a.y *= row.a.y;
           }
         }
       }
@@ -217,63 +259,61 @@ __global__ void __launch_bounds__(kThreads) scan_chunk_kernel(Params p) {
       f.v = make_float4(began ? -1.0f : a.x, h.x, began ? -1.0f : a.y, h.y);
     }
   }
-  p.chunk_ah[(j - 1) * p.pairs + pair] = f.v;
+  p.chunk_ah[(at.j - 1) * p.pairs + at.pair] = f.v;
 }
 
 // Backward: thread (j, pair) looks at the edge above chunk j: the effect of
 // chunk j, upwards, on the segment that crosses it; and notes the last
 // segment with rows that begins at or before chunk j's last row.
 template <class T>
-__global__ void __launch_bounds__(kThreads) scan_chunk_up_kernel(Params p) {
+__global__ void __launch_bounds__(kThreads, 4) scan_chunk_up_kernel(Params p) {
+  constexpr int B = kBlock<T>;
   using P = Pair<T>;
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  const int64_t j = t / p.pairs;
-  const int pair = static_cast<int>(t - j * p.pairs);
-  if (j >= p.chunks) return;
-  const int64_t edge = j * p.chunk_rows;
+  const Spot at(p);
+  if (at.j >= p.chunks) return;
+  const int64_t edge = at.j * p.chunk_rows;
   const int64_t stop = edge + p.chunk_rows < p.rows ? edge + p.chunk_rows : p.rows;
-  if (pair == 0) {
+  if (at.pair == 0) {
     int64_t last = last_at_most(p.off, p.nseg, stop - 1);
     if (last == p.nseg) --last;
     while (last >= 0 && __ldg(p.off + last) >= __ldg(p.off + last + 1)) --last;
-    p.edge_seg[j] = static_cast<int32_t>(last);
+    p.edge_seg[at.j] = static_cast<int32_t>(last);
   }
-  if (j == 0) return;
+  if (at.j == 0) return;
   const int64_t seg = last_at_most(p.off, p.nseg, edge);
   Effect f;
   f.v = make_float4(-1.0f, 0.0f, -1.0f, 0.0f);
   if (seg >= 0 && seg < p.nseg && __ldg(p.off + seg) < edge) {
     const int64_t end = __ldg(p.off + seg + 1);
-    const int64_t to = end < stop ? end : stop;
+    const int n = static_cast<int>((end < stop ? end : stop) - edge);
     float2 a = make_float2(1.0f, 1.0f), e = make_float2(0.0f, 0.0f);
-    if (end <= stop && p.grad_final != nullptr) e = load2(p.grad_final, seg, p.channels, 2 * pair);
-    for (int64_t r = to; r > edge; r -= kBlock) {  // rows r - 1, r - 2, ..
-      typename P::raw g[kBlock], d[kBlock];
+    if (end <= stop && p.grad_final != nullptr) e = load2(p.grad_final, seg, p.channels, at.ch);
+    const auto* gp = column<T>(p.gate, p, edge, at.pair);
+    const auto* dp = column<T>(p.grad, p, edge, at.pair);
+    for (int r = n - 1; r >= 0; r -= B) {
+      typename P::raw g[B], d[B];
 #pragma unroll
-      for (int i = 0; i < kBlock; ++i) {
-        if (r - 1 - i >= edge) {
-          g[i] = load_pair<T>(p.gate, r - 1 - i, p.pairs, pair);
-          d[i] = p.grad != nullptr ? load_pair<T>(p.grad, r - 1 - i, p.pairs, pair) : P::zero();
+      for (int i = 0; i < B; ++i) {
+        if (r - i >= 0) {
+          g[i] = __ldg(gp + (r - i) * p.pairs);
+          d[i] = p.grad != nullptr ? __ldg(dp + (r - i) * p.pairs) : P::zero();
         }
       }
 #pragma unroll
-      for (int i = 0; i < kBlock; ++i) {
-        if (r - 1 - i >= edge) {
-          const float2 gv = P::unpack(g[i]), dv = P::unpack(d[i]);
-          float2 av, kv;
-          gate_pair(gv.x, &av.x, &kv.x);
-          gate_pair(gv.y, &av.y, &kv.y);
-          e.x = av.x * (dv.x + e.x);
-          e.y = av.y * (dv.y + e.y);
-          a.x *= av.x;
-          a.y *= av.y;
+      for (int i = 0; i < B; ++i) {
+        if (r - i >= 0) {
+          const Row<T> row(g[i], d[i]);
+          e.x = row.a.x * (row.x.x + e.x);
+          e.y = row.a.y * (row.x.y + e.y);
+          a.x *= row.a.x;
+          a.y *= row.a.y;
         }
       }
     }
     const bool ended = end <= stop;
     f.v = make_float4(ended ? -1.0f : a.x, e.x, ended ? -1.0f : a.y, e.y);
   }
-  p.chunk_ah[j * p.pairs + pair] = f.v;
+  p.chunk_ah[at.j * p.pairs + at.pair] = f.v;
 }
 
 // Effects of groups of kLevel items of the level below, in the order of the
@@ -326,26 +366,41 @@ __device__ __forceinline__ void fill_empty(const Params& p, const float* in, flo
 // ---------------------------------------------------------------------------
 // Apply kernels
 // ---------------------------------------------------------------------------
+// Both walk a chunk in blocks of kBlock rows, the next block's loads in
+// flight. A block that lies inside of one segment, with neither edge of it,
+// takes the plain path; any other is walked with its checks per row.
 template <class T>
-__global__ void __launch_bounds__(kThreads, 3) scan_apply_kernel(Params p) {
+__global__ void __launch_bounds__(kThreads, 4) scan_apply_kernel(Params p) {
+  constexpr int B = kBlock<T>;
   using P = Pair<T>;
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  const int64_t j = t / p.pairs;
-  const int pair = static_cast<int>(t - j * p.pairs), ch = 2 * pair;
-  if (j < p.chunks) {
-    const int64_t r0 = j * p.chunk_rows;
+  using raw = typename P::raw;
+  const Spot at(p);
+  if (at.j < p.chunks) {
+    const int64_t r0 = at.j * p.chunk_rows;
     const int n = static_cast<int>(p.rows - r0 < p.chunk_rows ? p.rows - r0 : p.chunk_rows);
-    typename P::raw g[kBlock], x[kBlock];
+    const raw* gp = column<T>(p.gate, p, r0, at.pair);
+    const raw* xp = column<T>(p.x, p, r0, at.pair);
+    raw* hp = p.h != nullptr ? column<T>(p.h, p, r0, at.pair) : nullptr;
+    auto fetch = [&](int b0, raw(&g)[B], raw(&x)[B]) {
+      if (b0 + B <= n) {
 #pragma unroll
-    for (int i = 0; i < kBlock; ++i) {
-      if (i < n) {
-        g[i] = load_pair<T>(p.gate, r0 + i, p.pairs, pair);
-        x[i] = load_pair<T>(p.x, r0 + i, p.pairs, pair);
+        for (int i = 0; i < B; ++i) {
+          g[i] = __ldg(gp + (b0 + i) * p.pairs);
+          x[i] = __ldg(xp + (b0 + i) * p.pairs);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+          g[i] = b0 + i < n ? __ldg(gp + (b0 + i) * p.pairs) : P::zero();
+          x[i] = b0 + i < n ? __ldg(xp + (b0 + i) * p.pairs) : P::zero();
+        }
       }
-    }
+    };
+    raw g[B], x[B];
+    fetch(0, g, x);
     // The current segment, the row (from r0) where it ends, and whether there
     // is one: rows before the first and behind the last have none.
-    int64_t seg = p.edge_seg[j];
+    int64_t seg = p.edge_seg[at.j];
     const int64_t hi = clamp64(__ldg(p.off + p.nseg), 0, p.rows);
     auto until = [&](int64_t row) { return static_cast<int>(clamp64(row - r0, 0, p.chunk_rows + 1)); };
     bool inside = seg >= 0 && seg < p.nseg;
@@ -354,48 +409,52 @@ __global__ void __launch_bounds__(kThreads, 3) scan_apply_kernel(Params p) {
     if (inside) {
       const int64_t begin = clamp64(__ldg(p.off + seg), 0, r0);
       limit = until(__ldg(p.off + seg + 1));
-      if (begin < r0) st = entering(p, j, begin / p.chunk_rows, pair, false);
-      else if (p.initial != nullptr) st = load2(p.initial, seg, p.channels, ch);
+      if (begin < r0) st = entering(p, at.j, begin / p.chunk_rows, at.pair, false);
+      else if (p.initial != nullptr) st = load2(p.initial, seg, p.channels, at.ch);
     } else {
       limit = seg < 0 ? until(__ldg(p.off)) : p.chunk_rows + 1;
     }
     if (limit == 0) limit = p.chunk_rows + 1;  // only where offsets do not ascend
-    for (int b0 = 0; b0 < n; b0 += kBlock) {
-      typename P::raw gn[kBlock], xn[kBlock];
-#pragma unroll
-      for (int i = 0; i < kBlock; ++i) {
-        if (b0 + kBlock + i < n) {
-          gn[i] = load_pair<T>(p.gate, r0 + b0 + kBlock + i, p.pairs, pair);
-          xn[i] = load_pair<T>(p.x, r0 + b0 + kBlock + i, p.pairs, pair);
-        }
+    float* save = p.save != nullptr ? p.save + r0 / B * p.channels + at.ch : nullptr;
+    for (int b0 = 0; b0 < n; b0 += B) {
+      raw gn[B], xn[B];
+      fetch(b0 + B, gn, xn);
+      if (save != nullptr) {
+        *reinterpret_cast<float2*>(save) = st;
+        save += p.channels;
       }
-      if (p.save != nullptr) store2(p.save, (r0 + b0) / kBlock, p.channels, ch, st);
+      if (inside && b0 + B < limit && b0 + B <= n) {
 #pragma unroll
-      for (int i = 0; i < kBlock; ++i) {
-        const int r = b0 + i;
-        if (r < n) {
-          const float2 gv = P::unpack(g[i]), xv = P::unpack(x[i]);
-          float2 av, kv;
-          gate_pair(gv.x, &av.x, &kv.x);
-          gate_pair(gv.y, &av.y, &kv.y);
-          st.x = inside ? fmaf(av.x, st.x, kv.x * xv.x) : 0.0f;
-          st.y = inside ? fmaf(av.y, st.y, kv.y * xv.y) : 0.0f;
-          if (p.h != nullptr) static_cast<typename P::raw*>(p.h)[(r0 + r) * p.pairs + pair] = P::pack(st);
-          if (r + 1 == limit) {  // this row is the segment's last: on to the next one with rows
-            if (inside && p.final != nullptr) store2(p.final, seg, p.channels, ch, st);
-            int64_t end = r0 + r + 1;
-            do {
-              ++seg;
-              if (seg < p.nseg) end = __ldg(p.off + seg + 1);
-            } while (seg < p.nseg && end <= r0 + r + 1);
-            inside = seg < p.nseg;
-            limit = inside ? until(end < hi ? end : hi) : p.chunk_rows + 1;
-            st = inside && p.initial != nullptr ? load2(p.initial, seg, p.channels, ch) : make_float2(0.0f, 0.0f);
+        for (int i = 0; i < B; ++i) {
+          const Row<T> row(g[i], x[i]);
+          row.step(st);
+          if (hp != nullptr) hp[(b0 + i) * p.pairs] = P::pack(st);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+          const int r = b0 + i;
+          if (r < n) {
+            const Row<T> row(g[i], x[i]);
+            row.step(st);
+            if (!inside) st = make_float2(0.0f, 0.0f);
+            if (hp != nullptr) hp[r * p.pairs] = P::pack(st);
+            if (r + 1 == limit) {  // this row is the segment's last: on to the next one with rows
+              if (inside && p.final != nullptr) store2(p.final, seg, p.channels, at.ch, st);
+              int64_t end = r0 + r + 1;
+              do {
+                ++seg;
+                if (seg < p.nseg) end = __ldg(p.off + seg + 1);
+              } while (seg < p.nseg && end <= r0 + r + 1);
+              inside = seg < p.nseg;
+              limit = inside ? until(end < hi ? end : hi) : p.chunk_rows + 1;
+              st = inside && p.initial != nullptr ? load2(p.initial, seg, p.channels, at.ch) : make_float2(0.0f, 0.0f);
+            }
           }
         }
       }
 #pragma unroll
-      for (int i = 0; i < kBlock; ++i) {
+      for (int i = 0; i < B; ++i) {
         g[i] = gn[i];
         x[i] = xn[i];
       }
@@ -406,107 +465,128 @@ __global__ void __launch_bounds__(kThreads, 3) scan_apply_kernel(Params p) {
 
 template <class T>
 __global__ void __launch_bounds__(kThreads, 2) scan_apply_up_kernel(Params p) {
+  constexpr int B = kBlock<T>;
   using P = Pair<T>;
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  const int64_t j = t / p.pairs;
-  const int pair = static_cast<int>(t - j * p.pairs), ch = 2 * pair;
-  if (j < p.chunks) {
-    const int64_t r0 = j * p.chunk_rows;
+  using raw = typename P::raw;
+  const Spot at(p);
+  if (at.j < p.chunks) {
+    const int64_t r0 = at.j * p.chunk_rows;
     const int n = static_cast<int>(p.rows - r0 < p.chunk_rows ? p.rows - r0 : p.chunk_rows);
     const int64_t lo64 = clamp64(__ldg(p.off), 0, p.rows), hi64 = clamp64(__ldg(p.off + p.nseg), lo64, p.rows);
     auto rel = [&](int64_t row) { return static_cast<int>(clamp64(row - r0, -1, p.chunk_rows + 1)); };
     const int lo = rel(lo64), hi = rel(hi64);
-    auto fetch = [&](int b0, typename P::raw(&g)[kBlock], typename P::raw(&x)[kBlock], typename P::raw(&d)[kBlock]) {
+    const raw* gp = column<T>(p.gate, p, r0, at.pair);
+    const raw* xp = column<T>(p.x, p, r0, at.pair);
+    const raw* dp = p.grad != nullptr ? column<T>(p.grad, p, r0, at.pair) : nullptr;
+    raw* dxp = column<T>(p.dx, p, r0, at.pair);
+    raw* dgp = column<T>(p.dgate, p, r0, at.pair);
+    auto fetch = [&](int b0, raw(&g)[B], raw(&x)[B], raw(&d)[B]) {
 #pragma unroll
-      for (int i = 0; i < kBlock; ++i) {
-        if (b0 + i < n) {
-          g[i] = load_pair<T>(p.gate, r0 + b0 + i, p.pairs, pair);
-          x[i] = load_pair<T>(p.x, r0 + b0 + i, p.pairs, pair);
-          d[i] = p.grad != nullptr ? load_pair<T>(p.grad, r0 + b0 + i, p.pairs, pair) : P::zero();
-        }
+      for (int i = 0; i < B; ++i) {
+        const bool there = b0 + i < n;
+        g[i] = there ? __ldg(gp + (b0 + i) * p.pairs) : P::zero();
+        x[i] = there ? __ldg(xp + (b0 + i) * p.pairs) : P::zero();
+        d[i] = there && dp != nullptr ? __ldg(dp + (b0 + i) * p.pairs) : P::zero();
       }
     };
-    typename P::raw g[kBlock], x[kBlock], d[kBlock];
-    int b0 = (n - 1) / kBlock * kBlock;
+    raw g[B], x[B], d[B];
+    int b0 = (n - 1) / B * B;
     fetch(b0, g, x, d);
-    float2 before = load2(p.saved, (r0 + b0) / kBlock, p.channels, ch);
+    const float* saved = p.saved + (r0 + b0) / B * p.channels + at.ch;
+    float2 before = __ldg(reinterpret_cast<const float2*>(saved));
     // The segment of the current row (with rows; -1 when none is left), its
     // first row and the row behind its last, from r0.
-    int64_t seg = p.edge_seg[j];
+    int64_t seg = p.edge_seg[at.j];
     int begin = seg >= 0 ? rel(__ldg(p.off + seg)) : -1;
     int end = seg >= 0 ? rel(__ldg(p.off + seg + 1)) : -1;
     float2 e = make_float2(0.0f, 0.0f);
     if (seg >= 0) {
       const int64_t end64 = clamp64(__ldg(p.off + seg + 1), 0, p.rows);
-      if (end64 > r0 + n) e = entering(p, j, (end64 - 1) / p.chunk_rows, pair, true);
+      if (end64 > r0 + n) e = entering(p, at.j, (end64 - 1) / p.chunk_rows, at.pair, true);
     }
-    for (; b0 >= 0; b0 -= kBlock) {
-      typename P::raw gn[kBlock], xn[kBlock], dn[kBlock];
+    for (; b0 >= 0; b0 -= B) {
+      raw gn[B], xn[B], dn[B];
       float2 before_next = make_float2(0.0f, 0.0f);
       if (b0 > 0) {
-        fetch(b0 - kBlock, gn, xn, dn);
-        before_next = load2(p.saved, (r0 + b0) / kBlock - 1, p.channels, ch);
+        fetch(b0 - B, gn, xn, dn);
+        saved -= p.channels;
+        before_next = __ldg(reinterpret_cast<const float2*>(saved));
       }
-      // Which rows of the block start a segment, and the segment of the first.
-      uint32_t starts = 0;
-      int64_t low = seg;
-      int b = begin;
-      while (low >= 0 && b >= b0) {
-        if (b < b0 + kBlock) starts |= 1u << (b - b0);
-        do {
-          --low;
-        } while (low >= 0 && __ldg(p.off + low) >= __ldg(p.off + low + 1));
-        b = low >= 0 ? rel(__ldg(p.off + low)) : -1;
-      }
-      // The forward states again: q = (h_{t-1} - x_t) a_t (1 - a_t).
-      float2 a[kBlock], keep[kBlock], q[kBlock];
       float2 st = before;
+      if (seg >= 0 && begin < b0 && end > b0 + B && b0 + B <= n) {
+        float2 a[B], keep[B], q[B];  // q = (h_{t-1} - x_t) a_t (1 - a_t), forward
 #pragma unroll
-      for (int i = 0; i < kBlock; ++i) {
-        if (b0 + i < n) {
+        for (int i = 0; i < B; ++i) {
+          const Row<T> row(g[i], x[i]);
+          a[i] = row.a;
+          keep[i] = row.keep;
+          q[i] = make_float2((st.x - row.x.x) * (row.a.x * row.keep.x), (st.y - row.x.y) * (row.a.y * row.keep.y));
+          row.step(st);
+        }
+#pragma unroll
+        for (int i = B - 1; i >= 0; --i) {
+          const float2 dv = P::unpack(d[i]);
+          const float2 delta = make_float2(dv.x + e.x, dv.y + e.y);
+          e = make_float2(a[i].x * delta.x, a[i].y * delta.y);
+          dxp[(b0 + i) * p.pairs] = P::pack(make_float2(keep[i].x * delta.x, keep[i].y * delta.y));
+          dgp[(b0 + i) * p.pairs] = P::pack(make_float2(q[i].x * delta.x, q[i].y * delta.y));
+        }
+      } else {
+        // Which rows of the block start a segment, and the segment before the
+        // first of them.
+        uint32_t starts = 0;
+        int64_t low = seg;
+        int b = begin;
+        while (low >= 0 && b >= b0) {
+          if (b < b0 + B) starts |= 1u << (b - b0);
+          do {
+            --low;
+          } while (low >= 0 && __ldg(p.off + low) >= __ldg(p.off + low + 1));
+          b = low >= 0 ? rel(__ldg(p.off + low)) : -1;
+        }
+        float2 a[B], keep[B], q[B];
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
           if ((starts >> i) & 1u) {
             do {
               ++low;
             } while (__ldg(p.off + low) >= __ldg(p.off + low + 1));
-            st = p.initial != nullptr ? load2(p.initial, low, p.channels, ch) : make_float2(0.0f, 0.0f);
+            st = p.initial != nullptr ? load2(p.initial, low, p.channels, at.ch) : make_float2(0.0f, 0.0f);
           }
-          const float2 gv = P::unpack(g[i]), xv = P::unpack(x[i]);
-          gate_pair(gv.x, &a[i].x, &keep[i].x);
-          gate_pair(gv.y, &a[i].y, &keep[i].y);
-          q[i].x = (st.x - xv.x) * (a[i].x * keep[i].x);
-          q[i].y = (st.y - xv.y) * (a[i].y * keep[i].y);
-          st.x = fmaf(a[i].x, st.x, keep[i].x * xv.x);
-          st.y = fmaf(a[i].y, st.y, keep[i].y * xv.y);
+          const Row<T> row(g[i], x[i]);
+          a[i] = row.a;
+          keep[i] = row.keep;
+          q[i] = make_float2((st.x - row.x.x) * (row.a.x * row.keep.x), (st.y - row.x.y) * (row.a.y * row.keep.y));
+          row.step(st);
+        }
+#pragma unroll
+        for (int i = B - 1; i >= 0; --i) {
+          const int r = b0 + i;
+          if (r < n) {
+            const bool inside = r >= lo && r < hi;
+            if (r + 1 == end) {
+              e = p.grad_final != nullptr ? load2(p.grad_final, seg, p.channels, at.ch) : make_float2(0.0f, 0.0f);
+            }
+            const float2 dv = P::unpack(d[i]);
+            const float2 delta = make_float2(dv.x + e.x, dv.y + e.y);
+            const float2 dx = make_float2(keep[i].x * delta.x, keep[i].y * delta.y);
+            const float2 dg = make_float2(q[i].x * delta.x, q[i].y * delta.y);
+            e = inside ? make_float2(a[i].x * delta.x, a[i].y * delta.y) : make_float2(0.0f, 0.0f);
+            dxp[r * p.pairs] = inside ? P::pack(dx) : P::zero();
+            dgp[r * p.pairs] = inside ? P::pack(dg) : P::zero();
+            if ((starts >> i) & 1u) {  // this row is the segment's first: on to the one before
+              if (p.dinitial != nullptr) store2(p.dinitial, seg, p.channels, at.ch, e);
+              do {
+                --seg;
+              } while (seg >= 0 && __ldg(p.off + seg) >= __ldg(p.off + seg + 1));
+              end = seg >= 0 ? r : -1;
+              begin = seg >= 0 ? rel(__ldg(p.off + seg)) : -1;
+            }
+          }
         }
       }
 #pragma unroll
-      for (int i = kBlock - 1; i >= 0; --i) {
-        const int r = b0 + i;
-        if (r < n) {
-          const bool inside = r >= lo && r < hi;
-          if (r + 1 == end) {
-            e = p.grad_final != nullptr ? load2(p.grad_final, seg, p.channels, ch) : make_float2(0.0f, 0.0f);
-          }
-          const float2 dv = P::unpack(d[i]);
-          const float2 delta = make_float2(dv.x + e.x, dv.y + e.y);
-          e.x = inside ? a[i].x * delta.x : 0.0f;
-          e.y = inside ? a[i].y * delta.y : 0.0f;
-          const float2 dx = make_float2(inside ? keep[i].x * delta.x : 0.0f, inside ? keep[i].y * delta.y : 0.0f);
-          const float2 dg = make_float2(inside ? q[i].x * delta.x : 0.0f, inside ? q[i].y * delta.y : 0.0f);
-          static_cast<typename P::raw*>(p.dx)[(r0 + r) * p.pairs + pair] = P::pack(dx);
-          static_cast<typename P::raw*>(p.dgate)[(r0 + r) * p.pairs + pair] = P::pack(dg);
-          if ((starts >> i) & 1u) {  // this row is the segment's first: on to the one before
-            if (p.dinitial != nullptr) store2(p.dinitial, seg, p.channels, ch, e);
-            do {
-              --seg;
-            } while (seg >= 0 && __ldg(p.off + seg) >= __ldg(p.off + seg + 1));
-            end = seg >= 0 ? r : -1;
-            begin = seg >= 0 ? rel(__ldg(p.off + seg)) : -1;
-          }
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < kBlock; ++i) {
+      for (int i = 0; i < B; ++i) {
         g[i] = gn[i];
         x[i] = xn[i];
         d[i] = dn[i];
@@ -563,7 +643,7 @@ bool quad_aligned(const void* p, int dtype) {
 int32_t chunk_rows_of(int64_t rows, int64_t channels) {
   const int64_t full = static_cast<int64_t>(kSms) * 1024;
   const int64_t want = ceil_div(rows * (channels / 2), full);
-  return static_cast<int32_t>(ceil_div(clamp64(want, 16, 256), kBlock) * kBlock);
+  return static_cast<int32_t>(ceil_div(clamp64(want, 16, 256), 8) * 8);
 }
 
 size_t carve(void* base, size_t cap, int64_t rows, int64_t channels, Params* p, bool* ok) {
@@ -615,13 +695,14 @@ int launch(const Params& p, bool up, cudaStream_t stream) {
 
 using namespace dgfx;
 
-extern "C" int dgfx_gated_scan_workspace_size(int64_t rows, int64_t channels, size_t* workspace_bytes,
+extern "C" int dgfx_gated_scan_workspace_size(int64_t rows, int64_t channels, int dtype, size_t* workspace_bytes,
                                               size_t* saved_bytes) {
-  DGFX_TRY(check_shape("dgfx_gated_scan_workspace_size", rows, channels, 0, DGFX_F32));
+  DGFX_TRY(check_shape("dgfx_gated_scan_workspace_size", rows, channels, 0, dtype));
   Params p{};
   bool ok;
   if (workspace_bytes != nullptr) *workspace_bytes = carve(nullptr, 0, rows, channels, &p, &ok);
-  if (saved_bytes != nullptr) *saved_bytes = static_cast<size_t>(ceil_div(rows, kBlock)) * channels * sizeof(float);
+  const int64_t block = dtype == DGFX_F32 ? kBlock<float> : kBlock<__nv_bfloat16>;
+  if (saved_bytes != nullptr) *saved_bytes = static_cast<size_t>(ceil_div(rows, block)) * channels * sizeof(float);
   return DGFX_OK;
 }
 

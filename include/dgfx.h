@@ -428,8 +428,8 @@ int dgfx_segment_group_norm_backward(const void* d_dy, const void* d_x, int dtyp
  * d_new_state [n, channels] (fp32; may be d_state itself) and the same values
  * in dtype in d_h.
  * ------------------------------------------------------------------------ */
-int dgfx_gated_scan_workspace_size(int64_t rows, int64_t channels, size_t* workspace_bytes,
-                                   size_t* saved_bytes);
+int dgfx_gated_scan_workspace_size(int64_t rows, int64_t channels, int dtype,
+                                   size_t* workspace_bytes, size_t* saved_bytes);
 int dgfx_gated_scan(const void* d_x, const void* d_gate, int dtype, int64_t rows,
                     int64_t channels, const int64_t* d_offsets, int64_t nseg,
                     const float* d_initial, void* d_h, float* d_final, float* d_saved,
