@@ -16,6 +16,8 @@
 // one, the next rows' loads in flight; neighbouring threads are neighbouring channels,
 // so loads and stores are whole rows, and nothing is shared between threads.
 //
+//   edge kernel    where each chunk's edge row stands among the segments;
+//                  outputs of the segments without rows.
 //   chunk kernel   what a chunk does to a state that passes through its last
 //                  row: (A, H), state -> A state + H. Only the segment that crosses
 //                  that edge matters, so only its rows in the chunk are read:
@@ -125,28 +127,10 @@ struct Params {
   float4* chunk_ah;    // (A, H, A, H) of two channels: [chunks, pairs]
   float4* group_ah;    // [groups, pairs]
   float4* super_ah;    // [supergroups, pairs]
-  int32_t* edge_seg;   // per chunk: where its first (backward: last) row stands among the segments
+  int32_t* edge_seg;   // per chunk: where its first (backward: last) row stands among the segments [chunks]
   int64_t rows, nseg, chunks, groups, supers;
-  int32_t channels, pairs, chunk_rows;
+  int32_t channels, pairs, chunk_rows, chunk_shift;  // chunk_rows = 1 << chunk_shift
 };
-
-// The largest i in [0, n] with off[i] <= row, -1 if there is none: eight-way,
-// the probes of a round independent of one another.
-__device__ __forceinline__ int64_t last_at_most(const int64_t* __restrict__ off, int64_t n, int64_t row) {
-  int64_t lo = -1, hi = n + 1;
-  while (hi - lo > 1) {
-    const int64_t step = (hi - lo + 7) >> 3;
-    int below = 0;
-#pragma unroll
-    for (int k = 1; k < 8; ++k) {
-      const int64_t q = lo + step * k;
-      below += q < hi && __ldg(off + q) <= row;
-    }
-    lo += step * below;
-    hi = lo + step < hi ? lo + step : hi;
-  }
-  return lo;
-}
 
 // (A, H) of two channels.
 struct Effect {
@@ -210,106 +194,144 @@ __device__ __forceinline__ typename Pair<T>::raw* column(void* base, const Param
 }
 
 // ---------------------------------------------------------------------------
+// Edge kernel: a warp per segment
+// ---------------------------------------------------------------------------
+// Forward, edge_seg[j] = the segment of chunk j's first row: -1 before the
+// first segment, nseg behind the last. Backward, the last segment with rows
+// that begins at or before chunk j's last row, -1 if there is none. Segments without
+// rows get their state or gradient of it: out[s] = in[s] (0 without `in`).
+__global__ void __launch_bounds__(kThreads) scan_edge_kernel(Params p, int up, const float* __restrict__ in,
+                                                             float* __restrict__ out) {
+  const int64_t threads = static_cast<int64_t>(gridDim.x) * kThreads;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  const int lane = threadIdx.x & 31;
+  const int64_t lo = clamp64(__ldg(p.off), 0, p.rows), hi = clamp64(__ldg(p.off + p.nseg), lo, p.rows);
+  for (int64_t j = t; j < p.chunks; j += threads) {
+    const int64_t first = j << p.chunk_shift, next = first + p.chunk_rows;
+    if (up) {
+      if ((next < p.rows ? next : p.rows) <= lo || lo == hi) p.edge_seg[j] = -1;
+    } else if (first < lo || first >= hi) {
+      p.edge_seg[j] = first < lo ? -1 : static_cast<int32_t>(p.nseg);
+    }
+  }
+  for (int64_t s = t >> 5; s < p.nseg; s += threads >> 5) {
+    const int64_t b = clamp64(__ldg(p.off + s), lo, hi), e = clamp64(__ldg(p.off + s + 1), b, hi);
+    if (b == e) {
+      if (out != nullptr) {
+        for (int c = 2 * lane; c < p.channels; c += 64) {
+          store2(out, s, p.channels, c, in != nullptr ? load2(in, s, p.channels, c) : make_float2(0.0f, 0.0f));
+        }
+      }
+    } else if (up) {
+      // Chunks whose last row lies in [b, e); of the last segment with rows,
+      // also the chunks behind it.
+      for (int64_t j = (b >> p.chunk_shift) + lane; j < p.chunks; j += 32) {
+        const int64_t next = (j + 1) << p.chunk_shift;
+        if (e != hi && (next < p.rows ? next : p.rows) > e) break;
+        p.edge_seg[j] = static_cast<int32_t>(s);
+      }
+    } else {
+      for (int64_t j = ((b + p.chunk_rows - 1) >> p.chunk_shift) + lane; (j << p.chunk_shift) < e; j += 32) {
+        p.edge_seg[j] = static_cast<int32_t>(s);
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
 // Chunk kernels
 // ---------------------------------------------------------------------------
-// Forward: thread (j, pair) looks at the edge below chunk j - 1, the first
-// row of chunk j: it notes where that row stands and writes the effect of
-// chunk j - 1 on the segment that crosses the edge.
+// Calls f for n rows from `gate` and `in` on (null: zeros), `pitch` apart, in
+// order; the next block's loads are on their way while this one's run.
+template <class T, class F>
+__device__ __forceinline__ void walk(const typename Pair<T>::raw* gate, const typename Pair<T>::raw* in, int pitch, int n,
+                                     F f) {
+  constexpr int B = kBlock<T>;
+  using raw = typename Pair<T>::raw;
+  raw g[B], x[B];
+  auto fetch = [&](int r, raw(&gv)[B], raw(&xv)[B]) {
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+      const bool there = r + i < n;
+      gv[i] = there ? __ldg(gate + (r + i) * pitch) : Pair<T>::zero();
+      xv[i] = there && in != nullptr ? __ldg(in + (r + i) * pitch) : Pair<T>::zero();
+    }
+  };
+  fetch(0, g, x);
+  for (int r = 0; r < n; r += B) {
+    raw gn[B], xn[B];
+    fetch(r + B, gn, xn);
+    if (r + B <= n) {
+#pragma unroll
+      for (int i = 0; i < B; ++i) f(Row<T>(g[i], x[i]));
+    } else {
+#pragma unroll
+      for (int i = 0; i < B; ++i) {
+        if (r + i < n) f(Row<T>(g[i], x[i]));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+      g[i] = gn[i];
+      x[i] = xn[i];
+    }
+  }
+}
+
+// Forward: thread (j, pair) writes the effect of chunk j on the segment that
+// crosses its lower edge, the first row of chunk j + 1.
 template <class T>
 __global__ void __launch_bounds__(kThreads, 4) scan_chunk_kernel(Params p) {
-  constexpr int B = kBlock<T>;
-  using P = Pair<T>;
   const Spot at(p);
-  if (at.j >= p.chunks) return;
-  const int64_t edge = at.j * p.chunk_rows;
-  const int64_t seg = last_at_most(p.off, p.nseg, edge);
-  if (at.pair == 0) p.edge_seg[at.j] = static_cast<int32_t>(seg);
-  if (at.j == 0) return;
+  if (at.j + 1 >= p.chunks) return;
+  const int64_t first = at.j << p.chunk_shift, edge = first + p.chunk_rows;
+  // Clamped here and below: offsets that do not ascend leave anything.
+  const int64_t seg = clamp64(__ldg(p.edge_seg + at.j + 1), -1, p.nseg);
   Effect f;
   f.v = make_float4(-1.0f, 0.0f, -1.0f, 0.0f);
   if (seg >= 0 && seg < p.nseg) {
-    const int64_t first = edge - p.chunk_rows, begin = __ldg(p.off + seg);
-    const int64_t from = begin > first ? begin : first;
+    const int64_t begin = __ldg(p.off + seg);
+    const int64_t from = clamp64(begin, first, edge);
     const int n = static_cast<int>(edge - from);
     if (n > 0) {
       float2 a = make_float2(1.0f, 1.0f), h = make_float2(0.0f, 0.0f);
       if (begin >= first && p.initial != nullptr) h = load2(p.initial, seg, p.channels, at.ch);
-      const auto* gp = column<T>(p.gate, p, from, at.pair);
-      const auto* xp = column<T>(p.x, p, from, at.pair);
-      for (int r = 0; r < n; r += B) {
-        typename P::raw g[B], x[B];
-#pragma unroll
-        for (int i = 0; i < B; ++i) {
-          if (r + i < n) {
-            g[i] = __ldg(gp + (r + i) * p.pairs);
-            x[i] = __ldg(xp + (r + i) * p.pairs);
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < B; ++i) {
-          if (r + i < n) {
-            const Row<T> row(g[i], x[i]);
-            row.step(h);
-            a.x *= row.a.x;
-            a.y *= row.a.y;
-          }
-        }
-      }
+      walk<T>(column<T>(p.gate, p, from, at.pair), column<T>(p.x, p, from, at.pair), p.pairs, n, [&](const Row<T>& row) {
+        row.step(h);
+        a.x *= row.a.x;
+        a.y *= row.a.y;
+      });
       const bool began = begin >= first;
       f.v = make_float4(began ? -1.0f : a.x, h.x, began ? -1.0f : a.y, h.y);
     }
   }
-  p.chunk_ah[(at.j - 1) * p.pairs + at.pair] = f.v;
+  p.chunk_ah[at.j * p.pairs + at.pair] = f.v;
 }
 
-// Backward: thread (j, pair) looks at the edge above chunk j: the effect of
-// chunk j, upwards, on the segment that crosses it; and notes the last
-// segment with rows that begins at or before chunk j's last row.
+// Backward: the effect of chunk j, upwards, on the segment that crosses its
+// upper edge.
 template <class T>
 __global__ void __launch_bounds__(kThreads, 4) scan_chunk_up_kernel(Params p) {
-  constexpr int B = kBlock<T>;
-  using P = Pair<T>;
   const Spot at(p);
-  if (at.j >= p.chunks) return;
-  const int64_t edge = at.j * p.chunk_rows;
+  if (at.j >= p.chunks || at.j == 0) return;
+  const int64_t edge = at.j << p.chunk_shift;
   const int64_t stop = edge + p.chunk_rows < p.rows ? edge + p.chunk_rows : p.rows;
-  if (at.pair == 0) {
-    int64_t last = last_at_most(p.off, p.nseg, stop - 1);
-    if (last == p.nseg) --last;
-    while (last >= 0 && __ldg(p.off + last) >= __ldg(p.off + last + 1)) --last;
-    p.edge_seg[at.j] = static_cast<int32_t>(last);
-  }
-  if (at.j == 0) return;
-  const int64_t seg = last_at_most(p.off, p.nseg, edge);
+  // The segment of the last row above the edge, if it goes on below it.
+  const int64_t seg = clamp64(__ldg(p.edge_seg + at.j - 1), -1, p.nseg - 1);
   Effect f;
   f.v = make_float4(-1.0f, 0.0f, -1.0f, 0.0f);
-  if (seg >= 0 && seg < p.nseg && __ldg(p.off + seg) < edge) {
+  if (seg >= 0 && __ldg(p.off + seg + 1) > edge) {
     const int64_t end = __ldg(p.off + seg + 1);
-    const int n = static_cast<int>((end < stop ? end : stop) - edge);
+    const int n = static_cast<int>(clamp64(end, edge, stop) - edge);
     float2 a = make_float2(1.0f, 1.0f), e = make_float2(0.0f, 0.0f);
     if (end <= stop && p.grad_final != nullptr) e = load2(p.grad_final, seg, p.channels, at.ch);
-    const auto* gp = column<T>(p.gate, p, edge, at.pair);
-    const auto* dp = column<T>(p.grad, p, edge, at.pair);
-    for (int r = n - 1; r >= 0; r -= B) {
-      typename P::raw g[B], d[B];
-#pragma unroll
-      for (int i = 0; i < B; ++i) {
-        if (r - i >= 0) {
-          g[i] = __ldg(gp + (r - i) * p.pairs);
-          d[i] = p.grad != nullptr ? __ldg(dp + (r - i) * p.pairs) : P::zero();
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < B; ++i) {
-        if (r - i >= 0) {
-          const Row<T> row(g[i], d[i]);
-          e.x = row.a.x * (row.x.x + e.x);
-          e.y = row.a.y * (row.x.y + e.y);
-          a.x *= row.a.x;
-          a.y *= row.a.y;
-        }
-      }
-    }
+    const auto* dp = p.grad != nullptr ? column<T>(p.grad, p, edge + n - 1, at.pair) : nullptr;
+    walk<T>(column<T>(p.gate, p, edge + n - 1, at.pair), dp, -p.pairs, n, [&](const Row<T>& row) {
+      e.x = row.a.x * (row.x.x + e.x);
+      e.y = row.a.y * (row.x.y + e.y);
+      a.x *= row.a.x;
+      a.y *= row.a.y;
+    });
     const bool ended = end <= stop;
     f.v = make_float4(ended ? -1.0f : a.x, e.x, ended ? -1.0f : a.y, e.y);
   }
@@ -351,18 +373,6 @@ __device__ __forceinline__ float2 entering(const Params& p, int64_t j, int64_t o
   return make_float2(f.v.y, f.v.w);
 }
 
-// out[s] = in[s] (0 without `in`) for the segments without rows, one thread
-// per segment.
-__device__ __forceinline__ void fill_empty(const Params& p, const float* in, float* out) {
-  const int64_t threads = static_cast<int64_t>(gridDim.x) * kThreads;
-  for (int64_t s = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; s < p.nseg; s += threads) {
-    if (__ldg(p.off + s) < __ldg(p.off + s + 1)) continue;
-    for (int c = 0; c < p.channels; c += 2) {
-      store2(out, s, p.channels, c, in != nullptr ? load2(in, s, p.channels, c) : make_float2(0.0f, 0.0f));
-    }
-  }
-}
-
 // ---------------------------------------------------------------------------
 // Apply kernels
 // ---------------------------------------------------------------------------
@@ -376,7 +386,7 @@ __global__ void __launch_bounds__(kThreads, 4) scan_apply_kernel(Params p) {
   using raw = typename P::raw;
   const Spot at(p);
   if (at.j < p.chunks) {
-    const int64_t r0 = at.j * p.chunk_rows;
+    const int64_t r0 = at.j << p.chunk_shift;
     const int n = static_cast<int>(p.rows - r0 < p.chunk_rows ? p.rows - r0 : p.chunk_rows);
     const raw* gp = column<T>(p.gate, p, r0, at.pair);
     const raw* xp = column<T>(p.x, p, r0, at.pair);
@@ -400,7 +410,7 @@ __global__ void __launch_bounds__(kThreads, 4) scan_apply_kernel(Params p) {
     fetch(0, g, x);
     // The current segment, the row (from r0) where it ends, and whether there
     // is one: rows before the first and behind the last have none.
-    int64_t seg = p.edge_seg[at.j];
+    int64_t seg = clamp64(__ldg(p.edge_seg + at.j), -1, p.nseg);
     const int64_t hi = clamp64(__ldg(p.off + p.nseg), 0, p.rows);
     auto until = [&](int64_t row) { return static_cast<int>(clamp64(row - r0, 0, p.chunk_rows + 1)); };
     bool inside = seg >= 0 && seg < p.nseg;
@@ -409,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, 4) scan_apply_kernel(Params p) {
     if (inside) {
       const int64_t begin = clamp64(__ldg(p.off + seg), 0, r0);
       limit = until(__ldg(p.off + seg + 1));
-      if (begin < r0) st = entering(p, at.j, begin / p.chunk_rows, at.pair, false);
+      if (begin < r0) st = entering(p, at.j, begin >> p.chunk_shift, at.pair, false);
       else if (p.initial != nullptr) st = load2(p.initial, seg, p.channels, at.ch);
     } else {
       limit = seg < 0 ? until(__ldg(p.off)) : p.chunk_rows + 1;
@@ -460,7 +470,6 @@ __global__ void __launch_bounds__(kThreads, 4) scan_apply_kernel(Params p) {
       }
     }
   }
-  if (p.final != nullptr) fill_empty(p, p.initial, p.final);
 }
 
 template <class T>
@@ -470,7 +479,7 @@ __global__ void __launch_bounds__(kThreads, 2) scan_apply_up_kernel(Params p) {
   using raw = typename P::raw;
   const Spot at(p);
   if (at.j < p.chunks) {
-    const int64_t r0 = at.j * p.chunk_rows;
+    const int64_t r0 = at.j << p.chunk_shift;
     const int n = static_cast<int>(p.rows - r0 < p.chunk_rows ? p.rows - r0 : p.chunk_rows);
     const int64_t lo64 = clamp64(__ldg(p.off), 0, p.rows), hi64 = clamp64(__ldg(p.off + p.nseg), lo64, p.rows);
     auto rel = [&](int64_t row) { return static_cast<int>(clamp64(row - r0, -1, p.chunk_rows + 1)); };
@@ -496,13 +505,13 @@ __global__ void __launch_bounds__(kThreads, 2) scan_apply_up_kernel(Params p) {
     float2 before = __ldg(reinterpret_cast<const float2*>(saved));
     // The segment of the current row (with rows; -1 when none is left), its
     // first row and the row behind its last, from r0.
-    int64_t seg = p.edge_seg[at.j];
+    int64_t seg = clamp64(__ldg(p.edge_seg + at.j), -1, p.nseg - 1);
     int begin = seg >= 0 ? rel(__ldg(p.off + seg)) : -1;
     int end = seg >= 0 ? rel(__ldg(p.off + seg + 1)) : -1;
     float2 e = make_float2(0.0f, 0.0f);
     if (seg >= 0) {
       const int64_t end64 = clamp64(__ldg(p.off + seg + 1), 0, p.rows);
-      if (end64 > r0 + n) e = entering(p, at.j, (end64 - 1) / p.chunk_rows, at.pair, true);
+      if (end64 > r0 + n) e = entering(p, at.j, (end64 - 1) >> p.chunk_shift, at.pair, true);
     }
     for (; b0 >= 0; b0 -= B) {
       raw gn[B], xn[B], dn[B];
@@ -594,7 +603,6 @@ __global__ void __launch_bounds__(kThreads, 2) scan_apply_up_kernel(Params p) {
       before = before_next;
     }
   }
-  if (p.dinitial != nullptr) fill_empty(p, p.grad_final, p.dinitial);
 }
 
 template <class T>
@@ -637,13 +645,15 @@ bool quad_aligned(const void* p, int dtype) {
   return (reinterpret_cast<uintptr_t>(p) & (dtype == DGFX_F32 ? 15u : 7u)) == 0;
 }
 
-// Chunk height: enough threads to fill the GPU (about 1024 per SM), at
-// least two blocks of rows, at most 256 rows (a taller chunk saves nothing: its
-// edge already costs under 1/8 of its rows where windows are short).
-int32_t chunk_rows_of(int64_t rows, int64_t channels) {
+// Chunk height (its logarithm): at least 16 rows, at most 256 (a taller chunk
+// saves little: the rows that its edge makes the chunk kernel read are already
+// few where windows are short), and about 1024 threads per SM in between.
+int32_t chunk_shift_of(int64_t rows, int64_t channels) {
   const int64_t full = static_cast<int64_t>(kSms) * 1024;
-  const int64_t want = ceil_div(rows * (channels / 2), full);
-  return static_cast<int32_t>(ceil_div(clamp64(want, 16, 256), 8) * 8);
+  const int64_t want = rows * (channels / 2) / full;
+  int32_t shift = 4;
+  while (shift < 8 && (int64_t(1) << shift) < want) ++shift;
+  return shift;
 }
 
 size_t carve(void* base, size_t cap, int64_t rows, int64_t channels, Params* p, bool* ok) {
@@ -651,7 +661,8 @@ size_t carve(void* base, size_t cap, int64_t rows, int64_t channels, Params* p, 
   p->rows = rows;
   p->channels = static_cast<int32_t>(channels);
   p->pairs = static_cast<int32_t>(channels / 2);
-  p->chunk_rows = chunk_rows_of(rows, channels);
+  p->chunk_shift = chunk_shift_of(rows, channels);
+  p->chunk_rows = 1 << p->chunk_shift;
   p->chunks = ceil_div(rows, p->chunk_rows);
   p->groups = ceil_div(p->chunks, kLevel);
   p->supers = ceil_div(p->groups, kLevel);
@@ -668,7 +679,9 @@ unsigned grid_of(int64_t items) { return static_cast<unsigned>(std::max<int64_t>
 template <class T>
 int launch(const Params& p, bool up, cudaStream_t stream) {
   const unsigned grid = grid_of(p.chunks * p.pairs);
-  if (p.rows > 0) {
+  const unsigned edges = grid_of(std::max(p.chunks, std::min<int64_t>(p.nseg * 32, kSms * 2048)));
+  scan_edge_kernel<<<edges, kThreads, 0, stream>>>(p, up, up ? p.grad_final : p.initial, up ? p.dinitial : p.final);
+  if (p.chunks > 1) {
     if (up) scan_chunk_up_kernel<T><<<grid, kThreads, 0, stream>>>(p);
     else scan_chunk_kernel<T><<<grid, kThreads, 0, stream>>>(p);
     // The forward pass has no edge behind the last chunk, the backward pass
@@ -683,9 +696,10 @@ int launch(const Params& p, bool up, cudaStream_t stream) {
                                                                              p.super_ah, p.supers);
     }
   }
-  const unsigned apply = std::max(grid, grid_of(std::min<int64_t>(p.nseg, kSms * 2048)));  // segments without rows
-  if (up) scan_apply_up_kernel<T><<<apply, kThreads, 0, stream>>>(p);
-  else scan_apply_kernel<T><<<apply, kThreads, 0, stream>>>(p);
+  if (p.chunks > 0) {
+    if (up) scan_apply_up_kernel<T><<<grid, kThreads, 0, stream>>>(p);
+    else scan_apply_kernel<T><<<grid, kThreads, 0, stream>>>(p);
+  }
   DGFX_CUDA_TRY(cudaGetLastError());
   return DGFX_OK;
 }
