@@ -86,12 +86,11 @@ struct Pair<__nv_bfloat16> {
 // is held above -80, where a is 2e-35, so that e^-g stays finite (a maximum
 // that keeps NaN).
 __device__ __forceinline__ void gate_pair(float g, float* a, float* keep) {
-  float low, r;
+  float low;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(low) : "f"(g), "f"(-80.0f));
-  const float e = __expf(-low);
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
-  *a = r;
-  *keep = e * r;
+  const float e = exp_f(-low);
+  *a = rcp_f(1.0f + e);
+  *keep = e * *a;
 }
 
 // One row's coefficients and inputs for two channels.
@@ -249,25 +248,26 @@ __device__ __forceinline__ void walk(const typename Pair<T>::raw* gate, const ty
   constexpr int B = kBlock<T>;
   using raw = typename Pair<T>::raw;
   raw g[B], x[B];
-  auto fetch = [&](int r, raw(&gv)[B], raw(&xv)[B]) {
+  auto fetch = [&](int left, raw(&gv)[B], raw(&xv)[B]) {  // the next block, `left` rows from the end
 #pragma unroll
     for (int i = 0; i < B; ++i) {
-      const bool there = r + i < n;
-      gv[i] = there ? __ldg(gate + (r + i) * pitch) : Pair<T>::zero();
-      xv[i] = there && in != nullptr ? __ldg(in + (r + i) * pitch) : Pair<T>::zero();
+      gv[i] = i < left ? __ldg(gate + i * pitch) : Pair<T>::zero();
+      xv[i] = i < left && in != nullptr ? __ldg(in + i * pitch) : Pair<T>::zero();
     }
+    gate += B * pitch;
+    if (in != nullptr) in += B * pitch;
   };
-  fetch(0, g, x);
-  for (int r = 0; r < n; r += B) {
+  fetch(n, g, x);
+  for (int left = n; left > 0; left -= B) {
     raw gn[B], xn[B];
-    fetch(r + B, gn, xn);
-    if (r + B <= n) {
+    fetch(left - B, gn, xn);
+    if (left >= B) {
 #pragma unroll
       for (int i = 0; i < B; ++i) f(Row<T>(g[i], x[i]));
     } else {
 #pragma unroll
       for (int i = 0; i < B; ++i) {
-        if (r + i < n) f(Row<T>(g[i], x[i]));
+        if (i < left) f(Row<T>(g[i], x[i]));
       }
     }
 #pragma unroll
@@ -391,23 +391,25 @@ __global__ void __launch_bounds__(kThreads, 4) scan_apply_kernel(Params p) {
     const raw* gp = column<T>(p.gate, p, r0, at.pair);
     const raw* xp = column<T>(p.x, p, r0, at.pair);
     raw* hp = p.h != nullptr ? column<T>(p.h, p, r0, at.pair) : nullptr;
-    auto fetch = [&](int b0, raw(&g)[B], raw(&x)[B]) {
-      if (b0 + B <= n) {
+    auto fetch = [&](int left, raw(&g)[B], raw(&x)[B]) {  // the next block, `left` rows from the end
+      if (left >= B) {
 #pragma unroll
         for (int i = 0; i < B; ++i) {
-          g[i] = __ldg(gp + (b0 + i) * p.pairs);
-          x[i] = __ldg(xp + (b0 + i) * p.pairs);
+          g[i] = __ldg(gp + i * p.pairs);
+          x[i] = __ldg(xp + i * p.pairs);
         }
       } else {
 #pragma unroll
         for (int i = 0; i < B; ++i) {
-          g[i] = b0 + i < n ? __ldg(gp + (b0 + i) * p.pairs) : P::zero();
-          x[i] = b0 + i < n ? __ldg(xp + (b0 + i) * p.pairs) : P::zero();
+          g[i] = i < left ? __ldg(gp + i * p.pairs) : P::zero();
+          x[i] = i < left ? __ldg(xp + i * p.pairs) : P::zero();
         }
       }
+      gp += B * p.pairs;
+      xp += B * p.pairs;
     };
     raw g[B], x[B];
-    fetch(0, g, x);
+    fetch(n, g, x);
     // The current segment, the row (from r0) where it ends, and whether there
     // is one: rows before the first and behind the last have none.
     int64_t seg = clamp64(__ldg(p.edge_seg + at.j), -1, p.nseg);
@@ -428,7 +430,7 @@ __global__ void __launch_bounds__(kThreads, 4) scan_apply_kernel(Params p) {
     float* save = p.save != nullptr ? p.save + r0 / B * p.channels + at.ch : nullptr;
     for (int b0 = 0; b0 < n; b0 += B) {
       raw gn[B], xn[B];
-      fetch(b0 + B, gn, xn);
+      fetch(n - b0 - B, gn, xn);
       if (save != nullptr) {
         *reinterpret_cast<float2*>(save) = st;
         save += p.channels;
@@ -438,7 +440,7 @@ __global__ void __launch_bounds__(kThreads, 4) scan_apply_kernel(Params p) {
         for (int i = 0; i < B; ++i) {
           const Row<T> row(g[i], x[i]);
           row.step(st);
-          if (hp != nullptr) hp[(b0 + i) * p.pairs] = P::pack(st);
+          if (hp != nullptr) hp[i * p.pairs] = P::pack(st);
         }
       } else {
 #pragma unroll
@@ -448,7 +450,7 @@ __global__ void __launch_bounds__(kThreads, 4) scan_apply_kernel(Params p) {
             const Row<T> row(g[i], x[i]);
             row.step(st);
             if (!inside) st = make_float2(0.0f, 0.0f);
-            if (hp != nullptr) hp[r * p.pairs] = P::pack(st);
+            if (hp != nullptr) hp[i * p.pairs] = P::pack(st);
             if (r + 1 == limit) {  // this row is the segment's last: on to the next one with rows
               if (inside && p.final != nullptr) store2(p.final, seg, p.channels, at.ch, st);
               int64_t end = r0 + r + 1;
@@ -463,6 +465,7 @@ __global__ void __launch_bounds__(kThreads, 4) scan_apply_kernel(Params p) {
           }
         }
       }
+      if (hp != nullptr) hp += B * p.pairs;
 #pragma unroll
       for (int i = 0; i < B; ++i) {
         g[i] = gn[i];
@@ -484,23 +487,25 @@ __global__ void __launch_bounds__(kThreads, 2) scan_apply_up_kernel(Params p) {
     const int64_t lo64 = clamp64(__ldg(p.off), 0, p.rows), hi64 = clamp64(__ldg(p.off + p.nseg), lo64, p.rows);
     auto rel = [&](int64_t row) { return static_cast<int>(clamp64(row - r0, -1, p.chunk_rows + 1)); };
     const int lo = rel(lo64), hi = rel(hi64);
-    const raw* gp = column<T>(p.gate, p, r0, at.pair);
-    const raw* xp = column<T>(p.x, p, r0, at.pair);
-    const raw* dp = p.grad != nullptr ? column<T>(p.grad, p, r0, at.pair) : nullptr;
-    raw* dxp = column<T>(p.dx, p, r0, at.pair);
-    raw* dgp = column<T>(p.dgate, p, r0, at.pair);
-    auto fetch = [&](int b0, raw(&g)[B], raw(&x)[B], raw(&d)[B]) {
+    int b0 = (n - 1) / B * B;
+    const raw* gp = column<T>(p.gate, p, r0 + b0, at.pair);
+    const raw* xp = column<T>(p.x, p, r0 + b0, at.pair);
+    const raw* dp = p.grad != nullptr ? column<T>(p.grad, p, r0 + b0, at.pair) : nullptr;
+    raw* dxp = column<T>(p.dx, p, r0 + b0, at.pair);
+    raw* dgp = column<T>(p.dgate, p, r0 + b0, at.pair);
+    auto fetch = [&](int left, raw(&g)[B], raw(&x)[B], raw(&d)[B]) {  // a block, `left` rows from the end
 #pragma unroll
       for (int i = 0; i < B; ++i) {
-        const bool there = b0 + i < n;
-        g[i] = there ? __ldg(gp + (b0 + i) * p.pairs) : P::zero();
-        x[i] = there ? __ldg(xp + (b0 + i) * p.pairs) : P::zero();
-        d[i] = there && dp != nullptr ? __ldg(dp + (b0 + i) * p.pairs) : P::zero();
+        g[i] = i < left ? __ldg(gp + i * p.pairs) : P::zero();
+        x[i] = i < left ? __ldg(xp + i * p.pairs) : P::zero();
+        d[i] = i < left && dp != nullptr ? __ldg(dp + i * p.pairs) : P::zero();
       }
+      gp -= B * p.pairs;
+      xp -= B * p.pairs;
+      if (dp != nullptr) dp -= B * p.pairs;
     };
     raw g[B], x[B], d[B];
-    int b0 = (n - 1) / B * B;
-    fetch(b0, g, x, d);
+    fetch(n - b0, g, x, d);
     const float* saved = p.saved + (r0 + b0) / B * p.channels + at.ch;
     float2 before = __ldg(reinterpret_cast<const float2*>(saved));
     // The segment of the current row (with rows; -1 when none is left), its
@@ -517,7 +522,7 @@ __global__ void __launch_bounds__(kThreads, 2) scan_apply_up_kernel(Params p) {
       raw gn[B], xn[B], dn[B];
       float2 before_next = make_float2(0.0f, 0.0f);
       if (b0 > 0) {
-        fetch(b0 - B, gn, xn, dn);
+        fetch(B, gn, xn, dn);
         saved -= p.channels;
         before_next = __ldg(reinterpret_cast<const float2*>(saved));
       }
@@ -537,8 +542,8 @@ __global__ void __launch_bounds__(kThreads, 2) scan_apply_up_kernel(Params p) {
           const float2 dv = P::unpack(d[i]);
           const float2 delta = make_float2(dv.x + e.x, dv.y + e.y);
           e = make_float2(a[i].x * delta.x, a[i].y * delta.y);
-          dxp[(b0 + i) * p.pairs] = P::pack(make_float2(keep[i].x * delta.x, keep[i].y * delta.y));
-          dgp[(b0 + i) * p.pairs] = P::pack(make_float2(q[i].x * delta.x, q[i].y * delta.y));
+          dxp[i * p.pairs] = P::pack(make_float2(keep[i].x * delta.x, keep[i].y * delta.y));
+          dgp[i * p.pairs] = P::pack(make_float2(q[i].x * delta.x, q[i].y * delta.y));
         }
       } else {
         // Which rows of the block start a segment, and the segment before the
@@ -581,8 +586,8 @@ __global__ void __launch_bounds__(kThreads, 2) scan_apply_up_kernel(Params p) {
             const float2 dx = make_float2(keep[i].x * delta.x, keep[i].y * delta.y);
             const float2 dg = make_float2(q[i].x * delta.x, q[i].y * delta.y);
             e = inside ? make_float2(a[i].x * delta.x, a[i].y * delta.y) : make_float2(0.0f, 0.0f);
-            dxp[r * p.pairs] = inside ? P::pack(dx) : P::zero();
-            dgp[r * p.pairs] = inside ? P::pack(dg) : P::zero();
+            dxp[i * p.pairs] = inside ? P::pack(dx) : P::zero();
+            dgp[i * p.pairs] = inside ? P::pack(dg) : P::zero();
             if ((starts >> i) & 1u) {  // this row is the segment's first: on to the one before
               if (p.dinitial != nullptr) store2(p.dinitial, seg, p.channels, at.ch, e);
               do {
@@ -594,6 +599,8 @@ __global__ void __launch_bounds__(kThreads, 2) scan_apply_up_kernel(Params p) {
           }
         }
       }
+      dxp -= B * p.pairs;
+      dgp -= B * p.pairs;
 #pragma unroll
       for (int i = 0; i < B; ++i) {
         g[i] = gn[i];

@@ -9,8 +9,21 @@
 
 namespace dgfx {
 
+// e^x and 1 / x by the special function unit, subnormal numbers flushed (the
+// plain intrinsics spend as many instructions again on keeping them).
+__device__ __forceinline__ float exp_f(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.4426950408889634f));
+  return r;
+}
+__device__ __forceinline__ float rcp_f(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 // 1 / (1 + e^-z) without overflow at either end: e^-z = inf gives 0.
-__device__ __forceinline__ float sigmoid_f(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
+__device__ __forceinline__ float sigmoid_f(float z) { return rcp_f(1.0f + exp_f(-z)); }
 
 // Activations (DGFX_ACT_*) and their derivatives in fp32. gelu is the exact
 // form z Phi(z) = z (1 + erf(z / sqrt 2)) / 2. relu'(0) = 0. relu compares
@@ -37,7 +50,7 @@ __device__ __forceinline__ void act_both_f(float z, float* value, float* slope) 
   } else if (ACT == DGFX_ACT_GELU) {
     const float cdf = 0.5f + 0.5f * erff(z * 0.70710678118654752f);
     *value = z * cdf;
-    *slope = cdf + z * 0.39894228040143268f * __expf(-0.5f * z * z);
+    *slope = cdf + z * 0.39894228040143268f * exp_f(-0.5f * z * z);
   } else if (ACT == DGFX_ACT_SIGMOID) {
     const float s = sigmoid_f(z);
     *value = s;
