@@ -9,23 +9,22 @@
 //   dx = rstd (w dz - S1 / n - xhat S2 / n),  S1 = sum w dz,
 //   S2 = sum w dz xhat (over (s, g)),  dw_c = sum dz xhat,  db_c = sum dz.
 //
-// Bound by HBM. Short segments (a sampled graph) are read once: a team of
-// threads holds the whole segment in registers, 32 KB per 256 threads, takes
-// the sums and writes the result. A team is the smallest power of two of
-// threads (32 .. 512, at least a row) that holds twice the average segment,
-// so many small segments share a block. Longer segments are listed (in row
-// order) and go through two more kernels: the first reads row tiles and
+// Bound by HBM. A short segment (a sampled graph) is the work of a team of
+// threads: it reads the segment for the sums and again for the result, the second
+// time from L1. A team is the smallest power of two of threads (32 .. 512,
+// at least a row) that reads the average segment in a few steps, so many
+// small segments share a block. Segments of more than eight steps are listed (in
+// row order) and go through two more kernels: the first reads row tiles and
 // leaves a mean and a centred sum of squares per tile and group, which the
 // block that finishes a segment's last tile merges; the second applies them,
 // tiles in reverse order, so that what the first read last is still in L2.
-// When no segment can be long (all rows fit a team) only the first kernel is launched.
+// When no segment can be that long only the first kernel is launched.
 //
-// Thread t of a team holds the quad (4 channels) t mod Q of every (team / Q)-th
+// Thread t of a team takes the quad (4 channels) t mod Q of every (team / Q)-th
 // row, Q = C / 4: loads are whole rows and a thread's channels never change,
 // so weights and the sums for dw and db stay in registers. Squares are summed
-// around a mean (two passes over registers, or pairwise merges of means and
-// centred squares along the rows of a tile), never as sum x^2 - mean^2. All sums are
-// fp32 in an order fixed by the sizes: results do not change from run to
+// around a value of the segment, then around the means, never as sum x^2 -
+// mean^2. All sums are fp32 in an order fixed by the sizes: results do not change from run to
 // run. Rows outside [off[0], off[nseg]) are written as zeros and their inputs
 // are never used.
 #include <algorithm>
@@ -39,9 +38,9 @@ namespace {
 constexpr int kSms = 148;
 constexpr int kCh = 4;
 
-// Rows of a segment one thread holds (quads of bf16 take half the registers).
+// Rows loaded at a time: 128 bytes per thread in all.
 template <class T>
-constexpr int kHold = sizeof(T) == 2 ? 16 : 8;
+constexpr int kAhead = sizeof(T) == 2 ? 16 : 8;
 
 struct Params {
   const void* x;
@@ -60,13 +59,14 @@ struct Params {
   unsigned long long* long_counter;
   unsigned int* blocks_done;
   int32_t* long_slot;
+  longlong2* long_span;  // first row, rows
   int32_t* long_seg;
   int32_t* long_base;
   int32_t* long_done;
   float2* tile_sums;
   float2* seg_sums;  // backward: S1 / n and S2 / n per long segment and group
   int64_t rows, nseg;
-  int64_t hold_rows;  // rows a team holds in registers
+  int64_t loop_rows;  // rows of the longest segment that one team takes
   int64_t tile_rows;
   int64_t max_long, max_tiles;  // room of the list and of tile_sums
   int32_t channels, groups, quads;
@@ -145,7 +145,7 @@ struct Affine {
   __device__ Affine(const Params& p, const Place& at) {
 #pragma unroll
     for (int c = 0; c < kCh; ++c) {
-      const int ch = at.col * kCh + c;
+      const int ch = at.on ? at.col * kCh + c : 0;
       w[c] = p.weight != nullptr ? __ldg(p.weight + ch) : 1.0f;
       b[c] = p.bias != nullptr ? __ldg(p.bias + ch) : 0.0f;
     }
@@ -177,9 +177,10 @@ __device__ __forceinline__ void zero_outside(const Params& p, int64_t lo, int64_
 }
 
 // A long segment notes itself in the slot of its first row: segments of more
-// than hold_rows rows begin at least that far apart, so no two share a slot.
+// than loop_rows rows begin at least that far apart, so no two share a slot.
 __device__ __forceinline__ void note_long(const Params& p, int64_t s, int64_t begin) {
-  p.long_slot[begin / (p.hold_rows + 1)] = static_cast<int32_t>(s) + 1;
+  p.long_slot[begin / (p.loop_rows + 1)] = static_cast<int32_t>(s) + 1;
+  __threadfence();  // before this block counts as done
 }
 
 // The last block of a short-segment kernel to get here turns the slots into
@@ -187,7 +188,6 @@ __device__ __forceinline__ void note_long(const Params& p, int64_t s, int64_t be
 // with each one's first tile. Every thread of every block calls it.
 __device__ __forceinline__ void list_longs(const Params& p, int64_t lo, int64_t hi, float* smem) {
   __shared__ int last;
-  __threadfence();
   __syncthreads();
   if (threadIdx.x == 0) last = atomicAdd(p.blocks_done, 1u) == gridDim.x - 1;
   __syncthreads();
@@ -209,6 +209,8 @@ __device__ __forceinline__ void list_longs(const Params& p, int64_t lo, int64_t 
     const int32_t s = __ldcg(p.long_slot + i);
     if (s == 0) continue;
     const int64_t base = static_cast<int64_t>(at & 0xffffffffull);
+    const int64_t b = clamp64(p.off[s - 1], lo, hi), e = clamp64(p.off[s], b, hi);
+    p.long_span[at >> 32] = make_longlong2(b, e - b);
     p.long_seg[at >> 32] = s - 1;
     // Ascending offsets fit; others stay inside of the tables.
     p.long_base[at >> 32] = static_cast<int32_t>(base < p.max_tiles ? base : p.max_tiles);
@@ -243,13 +245,153 @@ __device__ __forceinline__ int find_long(const int32_t* base, int count, int til
   return lo;
 }
 
+// This thread's share of rows [begin, end): `mine` rows of its lane from
+// element `first` on, `pitch` elements (quads) apart.
+struct Share {
+  int64_t first;
+  int mine, pitch;
+  __device__ Share(const Params& p, const Place& at, int64_t begin, int64_t end) {
+    first = (begin + at.rl) * p.quads + at.col;
+    const int n = static_cast<int>(end - begin);
+    mine = at.on && n > at.rl ? (n - at.rl + at.per_pass - 1) / at.per_pass : 0;
+    pitch = at.per_pass * p.quads;
+  }
+};
+
+// Calls f(quad of x) or f(quad of x, quad of d) for `left` <= N rows, all
+// loads first.
+template <class T, int N, class F>
+__device__ __forceinline__ void few_rows(const typename Quad<T>::raw* x, int pitch, int left, F f) {
+  typename Quad<T>::raw v[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = i < left ? __ldg(x + i * pitch) : Quad<T>::zero();
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (i < left) f(v[i]);
+  }
+}
+template <class T, int N, class F>
+__device__ __forceinline__ void few_rows(const typename Quad<T>::raw* x, const typename Quad<T>::raw* d, int pitch, int left,
+                                         F f) {
+  typename Quad<T>::raw v[N], w[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    v[i] = i < left ? __ldg(x + i * pitch) : Quad<T>::zero();
+    w[i] = i < left ? __ldg(d + i * pitch) : Quad<T>::zero();
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (i < left) f(v[i], w[i]);
+  }
+}
+
+// The same for a share's rows in order, kAhead loads at a time.
+template <class T, class F>
+__device__ __forceinline__ void each_row(const Share& sh, const void* base, F f) {
+  constexpr int B = kAhead<T>;
+  using raw = typename Quad<T>::raw;
+  const raw* x = static_cast<const raw*>(base) + sh.first;
+  int left = sh.mine;
+  for (; left >= B; left -= B) {
+    raw v[B];
+#pragma unroll
+    for (int i = 0; i < B; ++i) v[i] = __ldg(x + i * sh.pitch);
+    x += B * sh.pitch;
+#pragma unroll
+    for (int i = 0; i < B; ++i) f(v[i]);
+  }
+  if (left > B / 4) few_rows<T, B - 1>(x, sh.pitch, left, f);
+  else if (left > 0) few_rows<T, B / 4>(x, sh.pitch, left, f);
+}
+template <class T, class F>
+__device__ __forceinline__ void each_row(const Share& sh, const void* base, const void* other, F f) {
+  constexpr int B = kAhead<T> / 2;
+  using raw = typename Quad<T>::raw;
+  const raw* x = static_cast<const raw*>(base) + sh.first;
+  const raw* d = static_cast<const raw*>(other) + sh.first;
+  int left = sh.mine;
+  for (; left >= B; left -= B) {
+    raw v[B], w[B];
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+      v[i] = __ldg(x + i * sh.pitch);
+      w[i] = __ldg(d + i * sh.pitch);
+    }
+    x += B * sh.pitch;
+    d += B * sh.pitch;
+#pragma unroll
+    for (int i = 0; i < B; ++i) f(v[i], w[i]);
+  }
+  if (left > B / 4) few_rows<T, B - 1>(x, d, sh.pitch, left, f);
+  else if (left > 0) few_rows<T, B / 4>(x, d, sh.pitch, left, f);
+}
+
+// Mean and centred squares of this thread's channels over its share. The
+// sums run around the share's first row x0: with d = x - x0, the centred squares
+// are sum d^2 - (sum d)^2 / n. What that loses is at most about n 2^-24 of
+// sum d^2, and as x0 is one of the values, n (x0 - mean)^2 summed over the
+// threads is at most n times the segment's own centred squares: a relative error of n 2^-24,
+// n the rows of a thread, however far the mean is from zero.
+struct RowStats {
+  float mean[kCh], m2[kCh], have;
+};
+
+template <class T>
+__device__ __forceinline__ RowStats row_stats(const Params& p, const Share& sh) {
+  using Q = Quad<T>;
+  RowStats s = {};
+  if (sh.mine == 0) return s;
+  float x0[kCh];
+  bool first = true;
+  each_row<T>(sh, p.x, [&](const typename Q::raw& v) {
+    float f[kCh];
+    Q::unpack(v, f);
+#pragma unroll
+    for (int c = 0; c < kCh; ++c) {
+      if (first) x0[c] = f[c];
+      const float d = f[c] - x0[c];
+      s.mean[c] += d;
+      s.m2[c] += d * d;
+    }
+    first = false;
+  });
+  s.have = static_cast<float>(sh.mine);
+  const float inv = 1.0f / s.have;
+#pragma unroll
+  for (int c = 0; c < kCh; ++c) {
+    const float d = s.mean[c] * inv;
+    const float m2 = s.m2[c] - s.mean[c] * d;
+    s.m2[c] = m2 < 0.0f ? 0.0f : m2;
+    s.mean[c] = x0[c] + d;
+  }
+  return s;
+}
+
+// y of a share's rows from their statistics.
+template <class T, int ACT>
+__device__ __forceinline__ void apply_rows(const Params& p, const Share& sh, const Affine& af, const float (&mu)[kCh],
+                                           const float (&rs)[kCh]) {
+  using Q = Quad<T>;
+  if (sh.mine == 0) return;
+  float scale[kCh];
+#pragma unroll
+  for (int c = 0; c < kCh; ++c) scale[c] = rs[c] * af.w[c];
+  typename Q::raw* y = static_cast<typename Q::raw*>(p.y) + sh.first;
+  each_row<T>(sh, p.x, [&](const typename Q::raw& v) {
+    float f[kCh];
+    Q::unpack(v, f);
+#pragma unroll
+    for (int c = 0; c < kCh; ++c) f[c] = act_f<ACT>(fmaf(f[c] - mu[c], scale[c], af.b[c]));
+    *y = Q::pack(f);
+    y += sh.pitch;
+  });
+}
+
 // ---------------------------------------------------------------------------
 // Forward
 // ---------------------------------------------------------------------------
 template <class T, int ACT>
-__global__ void __launch_bounds__(512, 2) norm_forward_kernel(Params p) {
-  using Q = Quad<T>;
-  constexpr int U = kHold<T>;
+__global__ void __maxnreg__(64) norm_forward_kernel(Params p) {
   extern __shared__ float smem[];
   const int in_block = threadIdx.x / p.team, t = threadIdx.x - in_block * p.team, bar = 1 + in_block;
   const Place at(p, t, p.team);
@@ -257,70 +399,37 @@ __global__ void __launch_bounds__(512, 2) norm_forward_kernel(Params p) {
   float* red = smem + in_block * (p.team * p.split + p.groups);
   float* gsum = red + p.team * p.split;
   const int64_t lo = clamp64(p.off[0], 0, p.rows), hi = clamp64(p.off[p.nseg], lo, p.rows);
-  zero_outside<T>(p, lo, hi);
   const int cg = p.channels / p.groups;
+  const Affine af(p, at);
   const int teams = blockDim.x / p.team;
   for (int64_t s = static_cast<int64_t>(blockIdx.x) * teams + in_block; s < p.nseg;
        s += static_cast<int64_t>(gridDim.x) * teams) {
     const int64_t begin = clamp64(p.off[s], lo, hi), end = clamp64(p.off[s + 1], begin, hi);
-    if (end - begin > p.hold_rows) {
+    if (end - begin > p.loop_rows) {
       if (t == 0) note_long(p, s, begin);
       continue;
     }
     const int n = static_cast<int>(end - begin);
-    // This thread's rows: begin + rl + u per_pass for u < mine.
-    const int mine = at.on && n > at.rl ? (n - at.rl + at.per_pass - 1) / at.per_pass : 0;
-    const int step = at.per_pass * p.quads;
-    const int64_t at0 = (begin + at.rl) * p.quads + at.col;
-    const typename Q::raw* px = static_cast<const typename Q::raw*>(p.x) + at0;
-    typename Q::raw v[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) v[u] = u < mine ? __ldg(px + u * step) : Q::zero();
     const float inv = n > 0 ? 1.0f / (static_cast<float>(n) * static_cast<float>(cg)) : 0.0f;
-    float acc[1][kCh] = {};
+    float mu[kCh], rs[kCh], acc[1][kCh] = {};
+    const Share sh(p, at, begin, end);
+    const RowStats rst = row_stats<T>(p, sh);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {  // rows past the end hold zeros
-      float f[kCh];
-      Q::unpack(v[u], f);
-#pragma unroll
-      for (int c = 0; c < kCh; ++c) acc[0][c] += f[c];
-    }
+    for (int c = 0; c < kCh; ++c) acc[0][c] = rst.have * rst.mean[c];
     group_sums<1>(p, acc, at, t, p.team, bar, red, gsum);
-    float mu[kCh];
     each_group(p, at, g0, [&](int c, int g) {
       mu[c] = at.on ? gsum[g] * inv : 0.0f;
-      acc[0][c] = 0.0f;
+      const float d = rst.mean[c] - mu[c];
+      acc[0][c] = rst.m2[c] + rst.have * d * d;
     });
     for (int g = t; g < p.groups; g += p.team) p.mean[s * p.groups + g] = gsum[g] * inv;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (u < mine) {
-        float f[kCh];
-        Q::unpack(v[u], f);
-#pragma unroll
-        for (int c = 0; c < kCh; ++c) acc[0][c] += (f[c] - mu[c]) * (f[c] - mu[c]);
-      }
-    }
     // Its first barrier also ends the reads of gsum above.
     group_sums<1>(p, acc, at, t, p.team, bar, red, gsum);
-    float rs[kCh];
     each_group(p, at, g0, [&](int c, int g) { rs[c] = at.on ? rsqrtf(gsum[g] * inv + p.eps) : 0.0f; });
     for (int g = t; g < p.groups; g += p.team) p.rstd[s * p.groups + g] = rsqrtf(gsum[g] * inv + p.eps);
-    if (mine > 0) {
-      const Affine af(p, at);
-      typename Q::raw* py = static_cast<typename Q::raw*>(p.y) + at0;
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (u < mine) {
-          float f[kCh];
-          Q::unpack(v[u], f);
-#pragma unroll
-          for (int c = 0; c < kCh; ++c) f[c] = act_f<ACT>((f[c] - mu[c]) * rs[c] * af.w[c] + af.b[c]);
-          py[u * step] = Q::pack(f);
-        }
-      }
-    }
+    apply_rows<T, ACT>(p, sh, af, mu, rs);
   }
+  zero_outside<T>(p, lo, hi);
   if (p.long_counter != nullptr) list_longs(p, lo, hi, smem);
 }
 
@@ -333,9 +442,9 @@ struct Tile {
     first = __ldg(p.long_base + entry);
     count_tiles = (entry + 1 < all.count ? __ldg(p.long_base + entry + 1) : all.tiles) - first;
     seg = __ldg(p.long_seg + entry);
-    const int64_t lo = clamp64(p.off[0], 0, p.rows), hi = clamp64(p.off[p.nseg], lo, p.rows);
-    const int64_t b = clamp64(p.off[seg], lo, hi), e = clamp64(p.off[seg + 1], b, hi);
-    rows_of_seg = e - b;
+    const longlong2 span = __ldg(p.long_span + entry);
+    const int64_t b = span.x, e = b + span.y;
+    rows_of_seg = span.y;
     begin = b + static_cast<int64_t>(tile - first) * p.tile_rows;
     end = begin + p.tile_rows < e ? begin + p.tile_rows : e;
   }
@@ -353,10 +462,41 @@ __device__ __forceinline__ bool last_tile(const Params& p, const Tile& tile, int
   return last;
 }
 
+// Adds term(tile's sums, first tile's sums, last tile?) over a segment's
+// tiles, for each group, and hands the total to done(group, total, first
+// tile's sums). The whole block calls; the order of the additions is fixed.
+template <class F, class D>
+__device__ __forceinline__ void merge_tiles(const Params& p, const Tile& tl, F term, D done) {
+  __shared__ float2 part[512];
+  const float2* sums = p.tile_sums + static_cast<int64_t>(tl.first) * p.groups;
+  for (int g0 = 0; g0 < p.groups; g0 += blockDim.x) {
+    const int width = min(p.groups - g0, static_cast<int>(blockDim.x)), lanes = blockDim.x / width;
+    const int lane = threadIdx.x / width, g = g0 + threadIdx.x - lane * width;
+    float2 total = make_float2(0.0f, 0.0f), s0 = total;
+    if (lane < lanes) {
+      s0 = __ldcg(sums + g);
+#pragma unroll 8
+      for (int k = lane; k < tl.count_tiles; k += lanes) {
+        const float2 t = term(__ldcg(sums + static_cast<int64_t>(k) * p.groups + g), s0, k == tl.count_tiles - 1);
+        total.x += t.x;
+        total.y += t.y;
+      }
+    }
+    part[threadIdx.x] = total;
+    __syncthreads();
+    if (lane == 0) {
+      for (int k = 1; k < lanes; ++k) {
+        total.x += part[k * width + threadIdx.x].x;
+        total.y += part[k * width + threadIdx.x].y;
+      }
+      done(g, total, s0);
+    }
+    __syncthreads();
+  }
+}
+
 template <class T>
 __global__ void __maxnreg__(64) norm_tile_stats_kernel(Params p) {
-  using Q = Quad<T>;
-  constexpr int B = 4;  // rows loaded at a time
   extern __shared__ float smem[];
   __shared__ int flag;
   float* red = smem;
@@ -368,60 +508,15 @@ __global__ void __maxnreg__(64) norm_tile_stats_kernel(Params p) {
   const int cg = p.channels / p.groups;
   for (int tile = blockIdx.x; tile < all.tiles; tile += gridDim.x) {
     const Tile tl(p, all, tile);
-    // Mean and centred squares of this thread's rows, merged B rows at a time
-    // (Chan, Golub and LeVeque, "Updating formulae and a pairwise algorithm
-    // for computing sample variances", 1979).
-    float mean[kCh] = {}, m2[kCh] = {}, have = 0.0f;
-    if (at.on) {
-      const int64_t step = at.per_pass;
-      for (int64_t r = tl.begin + at.rl; r < tl.end; r += B * step) {
-        typename Q::raw v[B];
-        int k = 0;
-#pragma unroll
-        for (int i = 0; i < B; ++i) {
-          if (r + i * step < tl.end) {
-            v[i] = load_quad<T>(p, p.x, r + i * step, at.col);
-            ++k;
-          } else {
-            v[i] = Q::zero();
-          }
-        }
-        const float kf = static_cast<float>(k);
-        const float ik = k == B ? 1.0f / B : 1.0f / kf;
-        const float all = have + kf, share = kf / all;
-        float sum[kCh] = {}, sq[kCh] = {}, f[B][kCh];
-#pragma unroll
-        for (int i = 0; i < B; ++i) {
-          Q::unpack(v[i], f[i]);
-#pragma unroll
-          for (int c = 0; c < kCh; ++c) sum[c] += f[i][c];
-        }
-#pragma unroll
-        for (int c = 0; c < kCh; ++c) sum[c] *= ik;
-#pragma unroll
-        for (int i = 0; i < B; ++i) {
-          if (i < k) {
-#pragma unroll
-            for (int c = 0; c < kCh; ++c) sq[c] += (f[i][c] - sum[c]) * (f[i][c] - sum[c]);
-          }
-        }
-#pragma unroll
-        for (int c = 0; c < kCh; ++c) {
-          const float d = sum[c] - mean[c];
-          mean[c] += d * share;
-          m2[c] += sq[c] + d * d * (have * share);
-        }
-        have = all;
-      }
-    }
+    const RowStats rst = row_stats<T>(p, Share(p, at, tl.begin, tl.end));
     const float n_tile = static_cast<float>(tl.end - tl.begin) * static_cast<float>(cg);
     float acc[1][kCh];
 #pragma unroll
-    for (int c = 0; c < kCh; ++c) acc[0][c] = have * mean[c];
+    for (int c = 0; c < kCh; ++c) acc[0][c] = rst.have * rst.mean[c];
     group_sums<1>(p, acc, at, threadIdx.x, threads, 1, red, gsum);
     each_group(p, at, g0, [&](int c, int g) {
-      const float d = at.on ? mean[c] - gsum[g] / n_tile : 0.0f;
-      acc[0][c] = m2[c] + have * d * d;
+      const float d = at.on ? rst.mean[c] - gsum[g] / n_tile : 0.0f;
+      acc[0][c] = rst.m2[c] + rst.have * d * d;
     });
     for (int g = threadIdx.x; g < p.groups; g += threads) {
       p.tile_sums[static_cast<int64_t>(tile) * p.groups + g].x = gsum[g] / n_tile;
@@ -431,29 +526,23 @@ __global__ void __maxnreg__(64) norm_tile_stats_kernel(Params p) {
       p.tile_sums[static_cast<int64_t>(tile) * p.groups + g].y = gsum[g];
     }
     if (last_tile(p, tl, &flag)) {
-      // Merge the segment's tiles, a warp per group.
-      const int lane = threadIdx.x & 31;
+      // Merge the segment's tiles around the first tile's mean m0, as the
+      // threads did their rows.
       const float n_all = static_cast<float>(tl.rows_of_seg) * static_cast<float>(cg);
       const float n_full = static_cast<float>(p.tile_rows) * static_cast<float>(cg);
       const float n_last = static_cast<float>(tl.rows_of_seg - (tl.count_tiles - 1) * p.tile_rows) * static_cast<float>(cg);
-      for (int g = threadIdx.x >> 5; g < p.groups; g += threads >> 5) {
-        const float2* sums = p.tile_sums + static_cast<int64_t>(tl.first) * p.groups + g;
-        float m = 0.0f;
-        for (int k = lane; k < tl.count_tiles; k += 32) {
-          m += (k == tl.count_tiles - 1 ? n_last : n_full) * __ldcg(&sums[static_cast<int64_t>(k) * p.groups].x);
-        }
-        m = warp_reduce_sum(m) / n_all;
-        float q = 0.0f;
-        for (int k = lane; k < tl.count_tiles; k += 32) {
-          const float2 s = __ldcg(&sums[static_cast<int64_t>(k) * p.groups]);
-          q += s.y + (k == tl.count_tiles - 1 ? n_last : n_full) * (s.x - m) * (s.x - m);
-        }
-        q = warp_reduce_sum(q) / n_all;
-        if (lane == 0) {
-          p.mean[tl.seg * p.groups + g] = m;
-          p.rstd[tl.seg * p.groups + g] = rsqrtf(q + p.eps);
-        }
-      }
+      merge_tiles(
+          p, tl,
+          [&](float2 s, float2 s0, bool last) {
+            const float d = s.x - s0.x, n = last ? n_last : n_full;
+            return make_float2(n * d, s.y + n * d * d);
+          },
+          [&](int g, float2 sum, float2 s0) {
+            const float d = sum.x / n_all;
+            const float m2 = sum.y - sum.x * d;
+            p.mean[tl.seg * p.groups + g] = s0.x + d;
+            p.rstd[tl.seg * p.groups + g] = rsqrtf((m2 < 0.0f ? 0.0f : m2) / n_all + p.eps);
+          });
     }
     __syncthreads();
   }
@@ -461,8 +550,6 @@ __global__ void __maxnreg__(64) norm_tile_stats_kernel(Params p) {
 
 template <class T, int ACT>
 __global__ void __maxnreg__(64) norm_tile_apply_kernel(Params p) {
-  using Q = Quad<T>;
-  constexpr int B = 8;
   const Place at(p, threadIdx.x, blockDim.x);
   const int g0 = at.col * kCh / (p.channels / p.groups);
   const Affine af(p, at);
@@ -475,41 +562,23 @@ __global__ void __maxnreg__(64) norm_tile_apply_kernel(Params p) {
       mu[c] = __ldg(p.mean + tl.seg * p.groups + g);
       rs[c] = __ldg(p.rstd + tl.seg * p.groups + g);
     });
-    const int64_t step = at.per_pass;
-    for (int64_t r = tl.begin + at.rl; r < tl.end; r += B * step) {
-      typename Q::raw v[B];
-#pragma unroll
-      for (int i = 0; i < B; ++i) {
-        v[i] = Q::zero();
-        if (r + i * step < tl.end) v[i] = load_quad<T>(p, p.x, r + i * step, at.col);
-      }
-#pragma unroll
-      for (int i = 0; i < B; ++i) {
-        if (r + i * step < tl.end) {
-          float f[kCh];
-          Q::unpack(v[i], f);
-#pragma unroll
-          for (int c = 0; c < kCh; ++c) f[c] = act_f<ACT>((f[c] - mu[c]) * rs[c] * af.w[c] + af.b[c]);
-          store_quad<T>(p, r + i * step, at.col, f);
-        }
-      }
-    }
+    apply_rows<T, ACT>(p, Share(p, at, tl.begin, tl.end), af, mu, rs);
   }
 }
 
 // ---------------------------------------------------------------------------
 // Backward
 // ---------------------------------------------------------------------------
-// xhat, and w dz rounded before any subtraction, the same value in the sums
-// and in dx: a segment of one value then cancels to zero exactly.
+// xhat and dz. dz and w dz are rounded before any sum or subtraction, the same
+// values in the sums and in dx: a segment of one value then cancels to zero
+// exactly.
 template <int ACT>
 __device__ __forceinline__ void grad_terms(float x, float dy, float mu, float rs, float w, float b, float* xhat,
-                                           float* dz, float* wdz) {
+                                           float* dz) {
   *xhat = (x - mu) * rs;
   float v, slope;
   act_both_f<ACT>(*xhat * w + b, &v, &slope);
   *dz = __fmul_rn(dy, slope);
-  *wdz = __fmul_rn(*dz, w);
 }
 
 // This block's sums for dw and db over its threads, in order, to its slot.
@@ -535,10 +604,57 @@ __device__ __forceinline__ void write_partial(const Params& p, const float (&dwb
   }
 }
 
+// A share's sums for dw and db (added to dwb), and from them its part of the
+// group sums: sum w dz xhat and sum w dz are w times those, channel by channel.
 template <class T, int ACT>
-__global__ void __launch_bounds__(512, 1) norm_backward_kernel(Params p) {
+__device__ __forceinline__ void grad_sums(const Params& p, const Share& sh, const float (&mu)[kCh], const float (&rs)[kCh],
+                                          const Affine& af, float (&acc)[2][kCh], float (&dwb)[2][kCh]) {
   using Q = Quad<T>;
-  constexpr int U = kHold<T>;
+  float dw[kCh] = {}, db[kCh] = {};  // these rows', so that long sums stay pairwise
+  each_row<T>(sh, p.x, p.dy, [&](const typename Q::raw& v, const typename Q::raw& d) {
+    float f[kCh], g[kCh];
+    Q::unpack(v, f);
+    Q::unpack(d, g);
+#pragma unroll
+    for (int c = 0; c < kCh; ++c) {
+      float xh, dz;
+      grad_terms<ACT>(f[c], g[c], mu[c], rs[c], af.w[c], af.b[c], &xh, &dz);
+      dw[c] += dz * xh;
+      db[c] += dz;
+    }
+  });
+#pragma unroll
+  for (int c = 0; c < kCh; ++c) {
+    dwb[0][c] += dw[c];
+    dwb[1][c] += db[c];
+    acc[0][c] = __fmul_rn(db[c], af.w[c]);
+    acc[1][c] = __fmul_rn(dw[c], af.w[c]);
+  }
+}
+
+// dx of a share's rows from their group's sums (divided by n).
+template <class T, int ACT>
+__device__ __forceinline__ void grad_rows(const Params& p, const Share& sh, const float (&mu)[kCh], const float (&rs)[kCh],
+                                          const Affine& af, const float (&s1)[kCh], const float (&s2)[kCh]) {
+  using Q = Quad<T>;
+  typename Q::raw* dx = static_cast<typename Q::raw*>(p.y) + sh.first;
+  each_row<T>(sh, p.x, p.dy, [&](const typename Q::raw& v, const typename Q::raw& d) {
+    float f[kCh], g[kCh];
+    Q::unpack(v, f);
+    Q::unpack(d, g);
+#pragma unroll
+    for (int c = 0; c < kCh; ++c) {
+      float xh, dz;
+      grad_terms<ACT>(f[c], g[c], mu[c], rs[c], af.w[c], af.b[c], &xh, &dz);
+      f[c] = rs[c] * (__fmul_rn(dz, af.w[c]) - s1[c] - xh * s2[c]);
+    }
+    *dx = Q::pack(f);
+    dx += sh.pitch;
+  });
+}
+
+template <class T, int ACT>
+__global__ void __maxnreg__(80) norm_backward_kernel(Params p) {
   extern __shared__ float smem[];
   const int in_block = threadIdx.x / p.team, t = threadIdx.x - in_block * p.team, bar = 1 + in_block;
   const Place at(p, t, p.team);
@@ -546,7 +662,6 @@ __global__ void __launch_bounds__(512, 1) norm_backward_kernel(Params p) {
   float* red = smem + in_block * 2 * (p.team * p.split + p.groups);
   float* gsum = red + 2 * p.team * p.split;
   const int64_t lo = clamp64(p.off[0], 0, p.rows), hi = clamp64(p.off[p.nseg], lo, p.rows);
-  zero_outside<T>(p, lo, hi);
   const Affine af(p, at);
   const int cg = p.channels / p.groups;
   const int teams = blockDim.x / p.team;
@@ -555,70 +670,30 @@ __global__ void __launch_bounds__(512, 1) norm_backward_kernel(Params p) {
        s += static_cast<int64_t>(gridDim.x) * teams) {
     const int64_t begin = clamp64(p.off[s], lo, hi), end = clamp64(p.off[s + 1], begin, hi);
     if (begin == end) continue;
-    if (end - begin > p.hold_rows) {
+    if (end - begin > p.loop_rows) {
       if (t == 0) note_long(p, s, begin);
       continue;
     }
     const int n = static_cast<int>(end - begin);
-    const int mine = at.on && n > at.rl ? (n - at.rl + at.per_pass - 1) / at.per_pass : 0;
-    const int step = at.per_pass * p.quads;
-    const int64_t at0 = (begin + at.rl) * p.quads + at.col;
-    const typename Q::raw* px = static_cast<const typename Q::raw*>(p.x) + at0;
-    const typename Q::raw* pd = static_cast<const typename Q::raw*>(p.dy) + at0;
-    typename Q::raw v[U], d[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      v[u] = u < mine ? __ldg(px + u * step) : Q::zero();
-      d[u] = u < mine ? __ldg(pd + u * step) : Q::zero();
-    }
     const float inv = 1.0f / (static_cast<float>(n) * static_cast<float>(cg));
     float mu[kCh], rs[kCh], acc[2][kCh] = {};
     each_group(p, at, g0, [&](int c, int g) {
       mu[c] = at.on ? __ldg(p.mean + s * p.groups + g) : 0.0f;
       rs[c] = at.on ? __ldg(p.rstd + s * p.groups + g) : 0.0f;
     });
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (u < mine) {
-        float f[kCh], g[kCh];
-        Q::unpack(v[u], f);
-        Q::unpack(d[u], g);
-#pragma unroll
-        for (int c = 0; c < kCh; ++c) {
-          float xh, dz, wdz;
-          grad_terms<ACT>(f[c], g[c], mu[c], rs[c], af.w[c], af.b[c], &xh, &dz, &wdz);
-          dwb[0][c] += dz * xh;
-          dwb[1][c] += dz;
-          acc[0][c] += wdz;
-          acc[1][c] += wdz * xh;
-        }
-      }
-    }
+    const Share sh(p, at, begin, end);
+    grad_sums<T, ACT>(p, sh, mu, rs, af, acc, dwb);
     group_sums<2>(p, acc, at, t, p.team, bar, red, gsum);
-    if (mine > 0) {
+    if (sh.mine > 0) {
       float s1[kCh], s2[kCh];
-      typename Q::raw* py = static_cast<typename Q::raw*>(p.y) + at0;
       each_group(p, at, g0, [&](int c, int g) {
         s1[c] = gsum[g] * inv;
         s2[c] = gsum[p.groups + g] * inv;
       });
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (u < mine) {
-          float f[kCh], g[kCh];
-          Q::unpack(v[u], f);
-          Q::unpack(d[u], g);
-#pragma unroll
-          for (int c = 0; c < kCh; ++c) {
-            float xh, dz, wdz;
-            grad_terms<ACT>(f[c], g[c], mu[c], rs[c], af.w[c], af.b[c], &xh, &dz, &wdz);
-            f[c] = rs[c] * (wdz - s1[c] - xh * s2[c]);
-          }
-          py[u * step] = Q::pack(f);
-        }
-      }
+      grad_rows<T, ACT>(p, sh, mu, rs, af, s1, s2);
     }
   }
+  zero_outside<T>(p, lo, hi);
   write_partial(p, dwb, at, teams, in_block, smem, blockIdx.x);
   if (p.long_counter != nullptr) {
     __syncthreads();
@@ -628,8 +703,6 @@ __global__ void __launch_bounds__(512, 1) norm_backward_kernel(Params p) {
 
 template <class T, int ACT>
 __global__ void __maxnreg__(80) norm_tile_grad_kernel(Params p) {
-  using Q = Quad<T>;
-  constexpr int B = 4;
   extern __shared__ float smem[];
   __shared__ int flag;
   float* red = smem;
@@ -648,63 +721,18 @@ __global__ void __maxnreg__(80) norm_tile_grad_kernel(Params p) {
       mu[c] = at.on ? __ldg(p.mean + tl.seg * p.groups + g) : 0.0f;
       rs[c] = at.on ? __ldg(p.rstd + tl.seg * p.groups + g) : 0.0f;
     });
-    if (at.on) {
-      float dwt[2][kCh] = {};  // this tile's, so that long sums stay pairwise
-      const int64_t step = at.per_pass;
-      for (int64_t r = tl.begin + at.rl; r < tl.end; r += B * step) {
-        typename Q::raw v[B], d[B];
-#pragma unroll
-        for (int i = 0; i < B; ++i) {
-          v[i] = Q::zero();
-          d[i] = Q::zero();
-          if (r + i * step < tl.end) {
-            v[i] = load_quad<T>(p, p.x, r + i * step, at.col);
-            d[i] = load_quad<T>(p, p.dy, r + i * step, at.col);
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < B; ++i) {
-          if (r + i * step < tl.end) {
-            float f[kCh], g[kCh];
-            Q::unpack(v[i], f);
-            Q::unpack(d[i], g);
-#pragma unroll
-            for (int c = 0; c < kCh; ++c) {
-              float xh, dz, wdz;
-              grad_terms<ACT>(f[c], g[c], mu[c], rs[c], af.w[c], af.b[c], &xh, &dz, &wdz);
-              dwt[0][c] += dz * xh;
-              dwt[1][c] += dz;
-              acc[0][c] += wdz;
-              acc[1][c] += wdz * xh;
-            }
-          }
-        }
-      }
-#pragma unroll
-      for (int c = 0; c < kCh; ++c) {
-        dwb[0][c] += dwt[0][c];
-        dwb[1][c] += dwt[1][c];
-      }
-    }
+    grad_sums<T, ACT>(p, Share(p, at, tl.begin, tl.end), mu, rs, af, acc, dwb);
     group_sums<2>(p, acc, at, threadIdx.x, threads, 1, red, gsum);
     for (int g = threadIdx.x; g < p.groups; g += threads) {
       p.tile_sums[static_cast<int64_t>(tile) * p.groups + g] = make_float2(gsum[g], gsum[p.groups + g]);
     }
     if (last_tile(p, tl, &flag)) {
-      const int lane = threadIdx.x & 31;
       const float n_all = static_cast<float>(tl.rows_of_seg) * static_cast<float>(cg);
-      for (int g = threadIdx.x >> 5; g < p.groups; g += threads >> 5) {
-        const float2* sums = p.tile_sums + static_cast<int64_t>(tl.first) * p.groups + g;
-        float a = 0.0f, b = 0.0f;
-        for (int k = lane; k < tl.count_tiles; k += 32) {
-          const float2 s = __ldcg(&sums[static_cast<int64_t>(k) * p.groups]);
-          a += s.x;
-          b += s.y;
-        }
-        a = warp_reduce_sum(a) / n_all;
-        b = warp_reduce_sum(b) / n_all;
-        if (lane == 0) p.seg_sums[static_cast<int64_t>(tl.entry) * p.groups + g] = make_float2(a, b);
-      }
+      merge_tiles(
+          p, tl, [](float2 s, float2, bool) { return s; },
+          [&](int g, float2 sum, float2) {
+            p.seg_sums[static_cast<int64_t>(tl.entry) * p.groups + g] = make_float2(sum.x / n_all, sum.y / n_all);
+          });
     }
     __syncthreads();
   }
@@ -713,8 +741,6 @@ __global__ void __maxnreg__(80) norm_tile_grad_kernel(Params p) {
 
 template <class T, int ACT>
 __global__ void __maxnreg__(80) norm_tile_grad_apply_kernel(Params p) {
-  using Q = Quad<T>;
-  constexpr int B = 4;
   const Place at(p, threadIdx.x, blockDim.x);
   const int g0 = at.col * kCh / (p.channels / p.groups);
   const Affine af(p, at);
@@ -730,34 +756,7 @@ __global__ void __maxnreg__(80) norm_tile_grad_apply_kernel(Params p) {
       s1[c] = s.x;
       s2[c] = s.y;
     });
-    const int64_t step = at.per_pass;
-    for (int64_t r = tl.begin + at.rl; r < tl.end; r += B * step) {
-      typename Q::raw v[B], d[B];
-#pragma unroll
-      for (int i = 0; i < B; ++i) {
-        v[i] = Q::zero();
-        d[i] = Q::zero();
-        if (r + i * step < tl.end) {
-          v[i] = load_quad<T>(p, p.x, r + i * step, at.col);
-          d[i] = load_quad<T>(p, p.dy, r + i * step, at.col);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < B; ++i) {
-        if (r + i * step < tl.end) {
-          float f[kCh], g[kCh];
-          Q::unpack(v[i], f);
-          Q::unpack(d[i], g);
-#pragma unroll
-          for (int c = 0; c < kCh; ++c) {
-            float xh, dz, wdz;
-            grad_terms<ACT>(f[c], g[c], mu[c], rs[c], af.w[c], af.b[c], &xh, &dz, &wdz);
-            f[c] = rs[c] * (wdz - s1[c] - xh * s2[c]);
-          }
-          store_quad<T>(p, r + i * step, at.col, f);
-        }
-      }
-    }
+    grad_rows<T, ACT>(p, Share(p, at, tl.begin, tl.end), mu, rs, af, s1, s2);
   }
 }
 
@@ -787,7 +786,7 @@ __global__ void __launch_bounds__(256) norm_params_kernel(const float* __restric
 // ---------------------------------------------------------------------------
 struct Plan {
   int32_t quads, team, threads, split, grid, tile_threads, tile_grid;
-  int64_t hold_rows, tile_rows, max_long, max_tiles;
+  int64_t loop_rows, tile_rows, max_long, max_tiles;
   bool longs;  // whether a segment can be too long for a team
 };
 
@@ -805,24 +804,33 @@ int make_plan(const char* who, int64_t rows, int64_t channels, int64_t groups, i
     return fail(DGFX_ERR_UNSUPPORTED,
                 std::string(who) + ": rows of at most 4096 bytes, fewer than 2^36 rows and 2^31 segments");
   }
-  const int hold = dtype == DGFX_F32 ? kHold<float> : kHold<__nv_bfloat16>;
   pl->quads = static_cast<int32_t>(channels / kCh);
   pl->split = channels / groups % kCh == 0 ? 1 : kCh;
+  // A team grows while the average segment takes it more than four steps of
+  // kAhead rows per thread, or more than two as long as the teams do not fill
+  // the GPU: more threads for the same segment repeat the fixed work of its
+  // sums. It takes segments of up to eight steps; longer ones would hold up
+  // their block.
+  const int ahead = (dtype == DGFX_F32 ? kAhead<float> : kAhead<__nv_bfloat16>) / 2;
   const int64_t average = nseg > 0 ? ceil_div(rows, nseg) : 1;
+  auto step_rows = [&](int team) { return static_cast<int64_t>(team / pl->quads) * ahead; };
   int team = 32;
-  while (team < 512 && (team < pl->quads || static_cast<int64_t>(team / pl->quads) * hold < 2 * average)) team *= 2;
+  while (team < 512 && (team < pl->quads || 4 * step_rows(team) < average ||
+                        (nseg * team < kSms * 768 && 2 * step_rows(team) < average))) {
+    team *= 2;
+  }
   pl->team = team;
   pl->threads = std::max(team, 256);
-  pl->hold_rows = static_cast<int64_t>(team / pl->quads) * hold;
-  pl->longs = rows > pl->hold_rows;
-  const int per_sm = backward ? (pl->threads == 512 ? 1 : 2) : (pl->threads == 512 ? 2 : 4);
+  pl->loop_rows = 8 * step_rows(team);
+  pl->longs = rows > pl->loop_rows;
+  const int per_sm = (backward ? 3 : 4) * 256 / pl->threads;
   pl->grid = static_cast<int32_t>(
       std::max<int64_t>(1, std::min<int64_t>(ceil_div(nseg * team, pl->threads), kSms * per_sm)));
   if (nseg == 0) pl->grid = kSms;
   pl->tile_threads = pl->quads > 256 ? 512 : 256;
   pl->tile_grid = kSms * (backward ? 3 : 4) / (pl->tile_threads / 256);
-  pl->tile_rows = std::max<int64_t>(pl->hold_rows, ceil_div(rows, kSms * 16));
-  pl->max_long = rows / (pl->hold_rows + 1) + 1;
+  pl->tile_rows = std::max<int64_t>(2 * step_rows(team), ceil_div(rows, kSms * 8));
+  pl->max_long = rows / (pl->loop_rows + 1) + 1;
   pl->max_tiles = ceil_div(rows, pl->tile_rows) + pl->max_long;
   return DGFX_OK;
 }
@@ -830,6 +838,7 @@ int make_plan(const char* who, int64_t rows, int64_t channels, int64_t groups, i
 struct Work {
   unsigned long long* counter;
   unsigned int* blocks;
+  longlong2* span;
   int32_t *slot, *seg, *base, *done;
   float2 *tile_sums, *seg_sums;
   float* partial;
@@ -847,6 +856,7 @@ Work carve(void* ws, size_t cap, const Plan& pl, int64_t channels, int64_t group
     w.slot = a.take<int32_t>(static_cast<size_t>(pl.max_long));
     w.done = a.take<int32_t>(static_cast<size_t>(pl.max_long));
     w.clear_bytes = a.used;
+    w.span = a.take<longlong2>(static_cast<size_t>(pl.max_long));
     w.seg = a.take<int32_t>(static_cast<size_t>(pl.max_long));
     w.base = a.take<int32_t>(static_cast<size_t>(pl.max_long));
     w.tile_sums = a.take<float2>(static_cast<size_t>(pl.max_tiles) * groups);
@@ -867,7 +877,7 @@ Params make_params(const Plan& pl, const Work& w, int64_t rows, int64_t channels
   p.quads = pl.quads;
   p.team = pl.team;
   p.split = pl.split;
-  p.hold_rows = pl.hold_rows;
+  p.loop_rows = pl.loop_rows;
   p.tile_rows = pl.tile_rows;
   p.max_long = pl.max_long;
   p.max_tiles = pl.max_tiles;
@@ -875,6 +885,7 @@ Params make_params(const Plan& pl, const Work& w, int64_t rows, int64_t channels
   p.long_counter = w.counter;
   p.blocks_done = w.blocks;
   p.long_slot = w.slot;
+  p.long_span = w.span;
   p.long_seg = w.seg;
   p.long_base = w.base;
   p.long_done = w.done;
