@@ -223,9 +223,29 @@ def stream_handle(stream=None) -> int:
     return int(s.cuda_stream)
 
 
+def current_device() -> int:
+    """Index of the current CUDA device (-1 without one), without the cost of
+    torch.cuda.current_device where torch offers the bare query."""
+    import torch
+
+    if not torch.cuda.is_initialized():
+        return torch.cuda.current_device() if torch.cuda.is_available() else -1
+    return torch._C._cuda_getDevice() if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device()
+
+
+def raw_stream(device: int) -> int:
+    """Handle of the current stream of a device, without building a Stream
+    object where torch offers the bare query."""
+    import torch
+
+    if hasattr(torch._C, "_cuda_getCurrentRawStream"):
+        return torch._C._cuda_getCurrentRawStream(device)
+    return int(torch.cuda.current_stream(device).cuda_stream)
+
+
 def ptr(t) -> Optional[int]:
     """Device pointer of a torch tensor (None passes NULL)."""
-    return None if t is None else int(t.data_ptr())
+    return None if t is None else t.data_ptr()
 
 
 def elem_ptr(t, i: int) -> int:

@@ -15,7 +15,10 @@ in fp32; inputs/outputs are fp32 or bf16.
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional
+
+import torch
 
 from distributed_graph_flow_b200 import _native
 
@@ -327,74 +330,70 @@ def batch_mean_aggregate(batch, features, out=None, stream=None):
 # the segments of a merged batch, gated recurrence over ragged windows.
 # ---------------------------------------------------------------------------
 def _activation_code(who: str, activation: str) -> int:
-    if activation not in _native.ACTIVATIONS:
+    code = _native.ACTIVATIONS.get(activation)
+    if code is None:
         raise ValueError(f"{who}: unknown activation {activation!r}; expected one of {sorted(_native.ACTIVATIONS)}")
-    return _native.ACTIVATIONS[activation]
+    return code
 
 
-def _layer_input(who: str, name: str, t, shape, dtypes) -> int:
-    """Checks one operand (type, shape with None for any extent, contiguity)
-    and returns its dtype code."""
-    import torch
+def _short(dtype) -> str:
+    return str(dtype).replace("torch.", "")
 
-    codes = {torch.float32: _native.F32, torch.bfloat16: _native.BF16}
-    allowed = [d for d in codes if d in dtypes]
-    if t.dtype not in allowed:
-        raise ValueError(f"{who}: {name} must be " + " or ".join(str(a).replace("torch.", "") for a in allowed))
-    if t.dim() != len(shape) or any(w is not None and int(n) != int(w) for n, w in zip(t.shape, shape)):
-        want = ", ".join("any" if w is None else str(int(w)) for w in shape)
-        raise ValueError(f"{who}: {name} is {list(t.shape)}, expected [{want}]")
+
+def _layer_operand(who: str, name: str, t, shape, dtype) -> None:
+    """Checks one operand: type, shape, contiguity."""
+    if t.dtype is not dtype:
+        raise ValueError(f"{who}: {name} must be {_short(dtype)}")
+    if t.shape != shape:
+        raise ValueError(f"{who}: {name} is {list(t.shape)}, expected {list(shape)}")
     if not t.is_contiguous():
         raise ValueError(f"{who}: {name} must be contiguous")
-    return codes[t.dtype]
+
+
+def _layer_matrix(who: str, name: str, t, dtype):
+    """Checks a matrix whose extents are free and returns them."""
+    shape = t.shape
+    if len(shape) != 2:
+        raise ValueError(f"{who}: {name} is {list(shape)}, expected a matrix")
+    _layer_operand(who, name, t, shape, dtype)
+    return shape
+
+
+def _layer_input(who: str, x):
+    """Checks the main input [rows, channels] (float32 or bfloat16); (rows, channels, dtype code)."""
+    code = _native.BF16 if x.dtype is torch.bfloat16 else _native.F32
+    if code == _native.F32 and x.dtype is not torch.float32:
+        raise ValueError(f"{who}: x must be float32 or bfloat16")
+    rows, channels = _layer_matrix(who, "x", x, x.dtype)
+    return rows, channels, code
 
 
 def _layer_offsets(who: str, offsets) -> int:
     """Checks segment offsets (int64 [segments + 1]) and returns the number of segments."""
-    import torch
-
-    if offsets.dtype != torch.int64 or offsets.dim() != 1 or int(offsets.numel()) < 1 or not offsets.is_contiguous():
+    if offsets.dtype is not torch.int64 or offsets.dim() != 1 or offsets.numel() < 1 or not offsets.is_contiguous():
         raise ValueError(f"{who}: offsets must be a contiguous int64 vector of segments + 1 values")
-    return int(offsets.numel()) - 1
+    return offsets.numel() - 1
 
 
-class _LayerLaunch:
-    """Device and stream of one call: every operand on one CUDA device, which
-    becomes the current one; allocations inside belong to the call's stream,
-    and operands used on a stream other than the current one are recorded on
-    it, so that their memory is not handed out while the call still runs."""
+class _LayerGuard:
+    """Device and stream of a call that does not run where the caller stands:
+    the operands' device becomes the current one and ``stream`` the current
+    stream, so that allocations inside belong to it; the operands are recorded on it, so
+    that their memory is not handed out while the call still runs."""
 
-    def __init__(self, who: str, stream, *operands):
-        torch = _native.require_cuda()
-        operands = [t for t in operands if t is not None]
-        self.device = operands[0].device
-        if self.device.type != "cuda" or any(t.device != self.device for t in operands):
-            raise ValueError(f"{who}: all tensors must be on one CUDA device, got "
-                             + ", ".join(sorted({str(t.device) for t in operands})))
-        self._guards = []
-        if self.device.index != torch.cuda.current_device():
-            self._guards.append(torch.cuda.device(self.device))
-        self._stream = stream
-        self._operands = operands
+    def __init__(self, who: str, stream, device: int, operands):
+        if stream is not None and stream.device_index != device:
+            raise ValueError(f"{who}: the stream belongs to cuda:{stream.device_index}, the tensors to cuda:{device}")
+        self._guards = [torch.cuda.device(device)]
+        if stream is not None:
+            self._guards.append(torch.cuda.stream(stream))
+            for t in operands:
+                if t is not None:
+                    t.record_stream(stream)
 
-    def __enter__(self) -> int:
-        import torch
-
+    def __enter__(self):
         for g in self._guards:
             g.__enter__()
-        current = torch.cuda.current_stream()
-        if self._stream is None or self._stream == current:
-            return int(current.cuda_stream)
-        if self._stream.device != self.device:
-            for g in reversed(self._guards):
-                g.__exit__(None, None, None)
-            raise ValueError(f"the stream belongs to {self._stream.device}, the tensors to {self.device}")
-        for t in self._operands:
-            t.record_stream(self._stream)
-        inner = torch.cuda.stream(self._stream)
-        inner.__enter__()
-        self._guards.append(inner)
-        return int(self._stream.cuda_stream)
 
     def __exit__(self, *exc):
         for g in reversed(self._guards):
@@ -402,29 +401,57 @@ class _LayerLaunch:
         return False
 
 
-def _layer_workspace(device, nbytes: int):
-    import torch
+def _layer_guard(who: str, stream, *operands):
+    """None when the call runs on the current device and stream as it is, else
+    the guard to run it under. Refuses operands that are not on one CUDA
+    device."""
+    device = operands[0].get_device()
+    for t in operands:
+        if t is not None and (t.get_device() != device or device < 0):
+            _native.require_cuda()
+            raise ValueError(f"{who}: all tensors must be on one CUDA device, got "
+                             + ", ".join(sorted({str(o.device) for o in operands if o is not None})))
+    if device == _native.current_device() and (stream is None or stream.cuda_stream == _native.raw_stream(device)):
+        return None
+    return _LayerGuard(who, stream, device, operands)
 
+
+def _layer_workspace(device, nbytes: int):
     return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(function: str, *sizes) -> int:
+    """A *_workspace_size query (a function of the sizes alone)."""
+    need = ctypes.c_size_t()
+    _native.check(getattr(_native.lib(), function)(*sizes, ctypes.byref(need)))
+    return need.value
+
+
+@functools.lru_cache(maxsize=1024)
+def _scan_sizes(rows: int, channels: int, code: int):
+    need, saved = ctypes.c_size_t(), ctypes.c_size_t()
+    _native.check(_native.lib().dgfx_gated_scan_workspace_size(rows, channels, code, ctypes.byref(need),
+                                                               ctypes.byref(saved)))
+    return need.value, saved.value // 4
 
 
 def _gated_operands(who: str, x1, x2, w_gate, w_up, b_gate, b_up):
     """Checks the operands of the gated dense layer; (m, k1, k2, n)."""
-    import torch
-
-    bf16 = (torch.bfloat16,)
-    _layer_input(who, "x1", x1, (None, None), bf16)
-    m, k1 = int(x1.shape[0]), int(x1.shape[1])
+    m, k1 = _layer_matrix(who, "x1", x1, torch.bfloat16)
     k2 = 0
     if x2 is not None:
-        _layer_input(who, "x2", x2, (m, None), bf16)
-        k2 = int(x2.shape[1])
-    _layer_input(who, "w_gate", w_gate, (None, k1 + k2), bf16)
-    n = int(w_gate.shape[0])
-    _layer_input(who, "w_up", w_up, (n, k1 + k2), bf16)
-    for name, t in (("b_gate", b_gate), ("b_up", b_up)):
-        if t is not None:
-            _layer_input(who, name, t, (n,), (torch.float32,))
+        m2, k2 = _layer_matrix(who, "x2", x2, torch.bfloat16)
+        if m2 != m:
+            raise ValueError(f"{who}: x2 is {list(x2.shape)}, expected {m} rows")
+    n, k = _layer_matrix(who, "w_gate", w_gate, torch.bfloat16)
+    if k != k1 + k2:
+        raise ValueError(f"{who}: w_gate is {list(w_gate.shape)}, expected {k1 + k2} columns")
+    _layer_operand(who, "w_up", w_up, (n, k), torch.bfloat16)
+    if b_gate is not None:
+        _layer_operand(who, "b_gate", b_gate, (n,), torch.float32)
+    if b_up is not None:
+        _layer_operand(who, "b_up", b_up, (n,), torch.float32)
     return m, k1, k2, n
 
 
@@ -439,27 +466,23 @@ def gated_dense_concat(x1, x2, w_gate, w_up, b_gate=None, b_up=None, activation:
     contiguous. activation: silu, gelu (erf form), relu, sigmoid or none. fp32
     accumulation, one rounding to bfloat16. ``dense_check`` reports pipeline
     timeouts of this call too."""
-    import torch
-
     who = "gated_dense_concat"
     m, k1, k2, n = _gated_operands(who, x1, x2, w_gate, w_up, b_gate, b_up)
     act = _activation_code(who, activation)
     if out is not None:
-        _layer_input(who, "out", out, (m, n), (torch.bfloat16,))
-    _gated_sizes(k1, k2, m, n)
-    with _LayerLaunch(who, stream, x1, x2, w_gate, w_up, b_gate, b_up, out) as sh:
-        if out is None:
-            out = torch.empty((m, n), dtype=torch.bfloat16, device=x1.device)
-        _native.check(_native.lib().dgfx_gated_dense_concat_bf16(
-            _native.ptr(x1), k1, _native.ptr(x2), k2, m, _native.ptr(w_gate), _native.ptr(w_up), _native.ptr(b_gate),
-            _native.ptr(b_up), n, act, _native.ptr(out), sh))
+        _layer_operand(who, "out", out, (m, n), torch.bfloat16)
+    _workspace_bytes("dgfx_gated_dense_concat_backward_workspace_size", k1, k2, m, n)  # refuses sizes before devices
+    guard = _layer_guard(who, stream, x1, x2, w_gate, w_up, b_gate, b_up, out)
+    if guard is not None:
+        with guard:
+            return gated_dense_concat(x1, x2, w_gate, w_up, b_gate, b_up, activation, out)
+    if out is None:
+        out = torch.empty((m, n), dtype=torch.bfloat16, device=x1.device)
+    ptr = _native.ptr
+    _native.check(_native.lib().dgfx_gated_dense_concat_bf16(
+        ptr(x1), k1, ptr(x2), k2, m, ptr(w_gate), ptr(w_up), ptr(b_gate), ptr(b_up), n, act, ptr(out),
+        _native.raw_stream(x1.get_device())))
     return out
-
-
-def _gated_sizes(k1: int, k2: int, m: int, n: int) -> int:
-    need = ctypes.c_size_t()
-    _native.check(_native.lib().dgfx_gated_dense_concat_backward_workspace_size(k1, k2, m, n, ctypes.byref(need)))
-    return need.value
 
 
 def gated_dense_concat_backward(grad, x1, x2, w_gate, w_up, b_gate=None, b_up=None, activation: str = "silu",
@@ -472,25 +495,27 @@ def gated_dense_concat_backward(grad, x1, x2, w_gate, w_up, b_gate=None, b_up=No
     follow; the bias gradients (float32) are summed before that rounding.
     need_input=False skips dx1 and dx2, need_weight=False dw_gate and dw_up
     (returned as None). Sums run in a fixed order."""
-    import torch
-
     who = "gated_dense_concat_backward"
     m, k1, k2, n = _gated_operands(who, x1, x2, w_gate, w_up, b_gate, b_up)
-    _layer_input(who, "grad", grad, (m, n), (torch.bfloat16,))
+    _layer_operand(who, "grad", grad, (m, n), torch.bfloat16)
     act = _activation_code(who, activation)
-    need = _gated_sizes(k1, k2, m, n)
-    with _LayerLaunch(who, stream, x1, x2, w_gate, w_up, b_gate, b_up, grad) as sh:
-        dx1 = torch.empty_like(x1) if need_input else None
-        dx2 = torch.empty_like(x2) if need_input and x2 is not None else None
-        dwg = torch.empty_like(w_gate) if need_weight else None
-        dwu = torch.empty_like(w_up) if need_weight else None
-        dbg = None if b_gate is None else torch.empty_like(b_gate)
-        dbu = None if b_up is None else torch.empty_like(b_up)
-        ws = _layer_workspace(x1.device, need)
-        _native.check(_native.lib().dgfx_gated_dense_concat_backward_bf16(
-            _native.ptr(grad), _native.ptr(x1), k1, _native.ptr(x2), k2, m, _native.ptr(w_gate), _native.ptr(w_up),
-            _native.ptr(b_gate), _native.ptr(b_up), n, act, _native.ptr(dx1), _native.ptr(dx2), _native.ptr(dwg),
-            _native.ptr(dwu), _native.ptr(dbg), _native.ptr(dbu), _native.ptr(ws), need, sh))
+    need = _workspace_bytes("dgfx_gated_dense_concat_backward_workspace_size", k1, k2, m, n)
+    guard = _layer_guard(who, stream, x1, x2, w_gate, w_up, b_gate, b_up, grad)
+    if guard is not None:
+        with guard:
+            return gated_dense_concat_backward(grad, x1, x2, w_gate, w_up, b_gate, b_up, activation, need_input,
+                                               need_weight)
+    dx1 = torch.empty_like(x1) if need_input else None
+    dx2 = torch.empty_like(x2) if need_input and x2 is not None else None
+    dwg = torch.empty_like(w_gate) if need_weight else None
+    dwu = torch.empty_like(w_up) if need_weight else None
+    dbg = None if b_gate is None else torch.empty_like(b_gate)
+    dbu = None if b_up is None else torch.empty_like(b_up)
+    ws = _layer_workspace(x1.device, need)
+    ptr = _native.ptr
+    _native.check(_native.lib().dgfx_gated_dense_concat_backward_bf16(
+        ptr(grad), ptr(x1), k1, ptr(x2), k2, m, ptr(w_gate), ptr(w_up), ptr(b_gate), ptr(b_up), n, act, ptr(dx1),
+        ptr(dx2), ptr(dwg), ptr(dwu), ptr(dbg), ptr(dbu), ptr(ws), need, _native.raw_stream(x1.get_device())))
     return dx1, dx2, dwg, dwu, dbg, dbu
 
 
@@ -511,31 +536,30 @@ def segment_group_norm(x, offsets, groups: int, weight=None, bias=None, eps: flo
     (a merged batch's spare capacity) give zeros and are never used, whatever they
     hold. Returns (y, mean, rstd); mean and rstd, float32 [segments, groups],
     are what ``segment_group_norm_backward`` takes."""
-    import torch
-
     who = "segment_group_norm"
-    code = _layer_input(who, "x", x, (None, None), (torch.float32, torch.bfloat16))
-    rows, channels = int(x.shape[0]), int(x.shape[1])
+    rows, channels, code = _layer_input(who, x)
     nseg = _layer_offsets(who, offsets)
     act = _activation_code(who, activation)
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None:
-            _layer_input(who, name, t, (channels,), (torch.float32,))
-    lib = _native.lib()
-    need = ctypes.c_size_t()
-    _native.check(lib.dgfx_segment_group_norm_workspace_size(rows, channels, int(groups), nseg, code, 0,
-                                                             ctypes.byref(need)))
+    if weight is not None:
+        _layer_operand(who, "weight", weight, (channels,), torch.float32)
+    if bias is not None:
+        _layer_operand(who, "bias", bias, (channels,), torch.float32)
+    groups = int(groups)
+    need = _workspace_bytes("dgfx_segment_group_norm_workspace_size", rows, channels, groups, nseg, code, 0)
     if not eps > 0:
         raise ValueError(f"{who}: eps must be positive")
-    with _LayerLaunch(who, stream, x, offsets, weight, bias) as sh:
-        y = torch.empty_like(x)
-        mean = torch.empty((nseg, int(groups)), dtype=torch.float32, device=x.device)
-        rstd = torch.empty_like(mean)
-        ws = _layer_workspace(x.device, need.value)
-        _native.check(lib.dgfx_segment_group_norm(
-            _native.ptr(x), code, rows, channels, int(groups), _native.ptr(offsets), nseg, _native.ptr(weight),
-            _native.ptr(bias), float(eps), act, _native.ptr(y), _native.ptr(mean), _native.ptr(rstd), _native.ptr(ws),
-            need.value, sh))
+    guard = _layer_guard(who, stream, x, offsets, weight, bias)
+    if guard is not None:
+        with guard:
+            return segment_group_norm(x, offsets, groups, weight, bias, eps, activation)
+    y = torch.empty_like(x)
+    mean = torch.empty((nseg, groups), dtype=torch.float32, device=x.device)
+    rstd = torch.empty_like(mean)
+    ws = _layer_workspace(x.device, need) if need else None
+    ptr = _native.ptr
+    _native.check(_native.lib().dgfx_segment_group_norm(
+        ptr(x), code, rows, channels, groups, ptr(offsets), nseg, ptr(weight), ptr(bias), eps, act, ptr(y), ptr(mean),
+        ptr(rstd), ptr(ws), need, _native.raw_stream(x.get_device())))
     return y, mean, rstd
 
 
@@ -546,41 +570,33 @@ def segment_group_norm_backward(grad, x, offsets, mean, rstd, weight=None, bias=
     x's type, dweight and dbias are float32 sums over all segments (None for
     a weight or bias that is None), in a fixed order. Rows outside of every
     segment get zeros, and what grad holds there is not used."""
-    import torch
-
     who = "segment_group_norm_backward"
-    code = _layer_input(who, "x", x, (None, None), (torch.float32, torch.bfloat16))
-    rows, channels = int(x.shape[0]), int(x.shape[1])
-    _layer_input(who, "grad", grad, x.shape, (x.dtype,))
+    rows, channels, code = _layer_input(who, x)
+    _layer_operand(who, "grad", grad, x.shape, x.dtype)
     nseg = _layer_offsets(who, offsets)
     act = _activation_code(who, activation)
-    _layer_input(who, "mean", mean, (nseg, None), (torch.float32,))
-    groups = int(mean.shape[1])
-    _layer_input(who, "rstd", rstd, (nseg, groups), (torch.float32,))
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None:
-            _layer_input(who, name, t, (channels,), (torch.float32,))
-    lib = _native.lib()
-    need = ctypes.c_size_t()
-    _native.check(lib.dgfx_segment_group_norm_workspace_size(rows, channels, groups, nseg, code, 1,
-                                                             ctypes.byref(need)))
-    with _LayerLaunch(who, stream, grad, x, offsets, mean, rstd, weight, bias) as sh:
-        dx = torch.empty_like(x)
-        dw = None if weight is None else torch.empty_like(weight)
-        db = None if bias is None else torch.empty_like(bias)
-        ws = _layer_workspace(x.device, need.value)
-        _native.check(lib.dgfx_segment_group_norm_backward(
-            _native.ptr(grad), _native.ptr(x), code, rows, channels, groups, _native.ptr(offsets), nseg,
-            _native.ptr(mean), _native.ptr(rstd), _native.ptr(weight), _native.ptr(bias), act, _native.ptr(dx),
-            _native.ptr(dw), _native.ptr(db), _native.ptr(ws), need.value, sh))
+    segments, groups = _layer_matrix(who, "mean", mean, torch.float32)
+    if segments != nseg:
+        raise ValueError(f"{who}: mean is {list(mean.shape)}, expected {nseg} rows")
+    _layer_operand(who, "rstd", rstd, (nseg, groups), torch.float32)
+    if weight is not None:
+        _layer_operand(who, "weight", weight, (channels,), torch.float32)
+    if bias is not None:
+        _layer_operand(who, "bias", bias, (channels,), torch.float32)
+    need = _workspace_bytes("dgfx_segment_group_norm_workspace_size", rows, channels, groups, nseg, code, 1)
+    guard = _layer_guard(who, stream, grad, x, offsets, mean, rstd, weight, bias)
+    if guard is not None:
+        with guard:
+            return segment_group_norm_backward(grad, x, offsets, mean, rstd, weight, bias, activation)
+    dx = torch.empty_like(x)
+    dw = None if weight is None else torch.empty_like(weight)
+    db = None if bias is None else torch.empty_like(bias)
+    ws = _layer_workspace(x.device, need)
+    ptr = _native.ptr
+    _native.check(_native.lib().dgfx_segment_group_norm_backward(
+        ptr(grad), ptr(x), code, rows, channels, groups, ptr(offsets), nseg, ptr(mean), ptr(rstd), ptr(weight),
+        ptr(bias), act, ptr(dx), ptr(dw), ptr(db), ptr(ws), need, _native.raw_stream(x.get_device())))
     return dx, dw, db
-
-
-def _scan_sizes(rows: int, channels: int, code: int):
-    need, saved = ctypes.c_size_t(), ctypes.c_size_t()
-    _native.check(_native.lib().dgfx_gated_scan_workspace_size(rows, channels, code, ctypes.byref(need),
-                                                               ctypes.byref(saved)))
-    return need.value, saved.value // 4
 
 
 def gated_scan(x, gate, offsets, initial=None, return_sequence: bool = True, return_saved: bool = False, stream=None):
@@ -597,24 +613,25 @@ def gated_scan(x, gate, offsets, initial=None, return_sequence: bool = True, ret
     after each segment's last row (its initial state if it has no rows).
     States are float32 throughout. return_sequence=False skips h (returned as
     None); return_saved=True appends what ``gated_scan_backward`` takes."""
-    import torch
-
     who = "gated_scan"
-    code = _layer_input(who, "x", x, (None, None), (torch.float32, torch.bfloat16))
-    rows, channels = int(x.shape[0]), int(x.shape[1])
-    _layer_input(who, "gate", gate, x.shape, (x.dtype,))
+    rows, channels, code = _layer_input(who, x)
+    _layer_operand(who, "gate", gate, x.shape, x.dtype)
     nseg = _layer_offsets(who, offsets)
     if initial is not None:
-        _layer_input(who, "initial", initial, (nseg, channels), (torch.float32,))
+        _layer_operand(who, "initial", initial, (nseg, channels), torch.float32)
     need, saved_n = _scan_sizes(rows, channels, code)
-    with _LayerLaunch(who, stream, x, gate, offsets, initial) as sh:
-        h = torch.empty_like(x) if return_sequence else None
-        final = torch.empty((nseg, channels), dtype=torch.float32, device=x.device)
-        saved = torch.empty(saved_n, dtype=torch.float32, device=x.device) if return_saved else None
-        ws = _layer_workspace(x.device, need)
-        _native.check(_native.lib().dgfx_gated_scan(
-            _native.ptr(x), _native.ptr(gate), code, rows, channels, _native.ptr(offsets), nseg, _native.ptr(initial),
-            _native.ptr(h), _native.ptr(final), _native.ptr(saved), _native.ptr(ws), need, sh))
+    guard = _layer_guard(who, stream, x, gate, offsets, initial)
+    if guard is not None:
+        with guard:
+            return gated_scan(x, gate, offsets, initial, return_sequence, return_saved)
+    h = torch.empty_like(x) if return_sequence else None
+    final = torch.empty((nseg, channels), dtype=torch.float32, device=x.device)
+    saved = torch.empty(saved_n, dtype=torch.float32, device=x.device) if return_saved else None
+    ws = _layer_workspace(x.device, need)
+    ptr = _native.ptr
+    _native.check(_native.lib().dgfx_gated_scan(
+        ptr(x), ptr(gate), code, rows, channels, ptr(offsets), nseg, ptr(initial), ptr(h), ptr(final), ptr(saved),
+        ptr(ws), need, _native.raw_stream(x.get_device())))
     return (h, final, saved) if return_saved else (h, final)
 
 
@@ -623,28 +640,29 @@ def gated_scan_backward(grad, x, gate, offsets, saved, initial=None, grad_final=
     of h (None: zeros) and of final (None: zeros), the forward inputs and
     ``saved``. dinitial is None where initial is. Rows outside of every
     segment get zeros."""
-    import torch
-
     who = "gated_scan_backward"
-    code = _layer_input(who, "x", x, (None, None), (torch.float32, torch.bfloat16))
-    rows, channels = int(x.shape[0]), int(x.shape[1])
-    _layer_input(who, "gate", gate, x.shape, (x.dtype,))
+    rows, channels, code = _layer_input(who, x)
+    _layer_operand(who, "gate", gate, x.shape, x.dtype)
     if grad is not None:
-        _layer_input(who, "grad", grad, x.shape, (x.dtype,))
+        _layer_operand(who, "grad", grad, x.shape, x.dtype)
     nseg = _layer_offsets(who, offsets)
-    for name, t in (("initial", initial), ("grad_final", grad_final)):
-        if t is not None:
-            _layer_input(who, name, t, (nseg, channels), (torch.float32,))
+    if initial is not None:
+        _layer_operand(who, "initial", initial, (nseg, channels), torch.float32)
+    if grad_final is not None:
+        _layer_operand(who, "grad_final", grad_final, (nseg, channels), torch.float32)
     need, saved_n = _scan_sizes(rows, channels, code)
-    _layer_input(who, "saved", saved, (saved_n,), (torch.float32,))
-    with _LayerLaunch(who, stream, x, grad, gate, offsets, saved, initial, grad_final) as sh:
-        dx, dgate = torch.empty_like(x), torch.empty_like(gate)
-        dinitial = None if initial is None else torch.empty_like(initial)
-        ws = _layer_workspace(x.device, need)
-        _native.check(_native.lib().dgfx_gated_scan_backward(
-            _native.ptr(x), _native.ptr(gate), code, rows, channels, _native.ptr(offsets), nseg, _native.ptr(initial),
-            _native.ptr(saved), _native.ptr(grad), _native.ptr(grad_final), _native.ptr(dx), _native.ptr(dgate),
-            _native.ptr(dinitial), _native.ptr(ws), need, sh))
+    _layer_operand(who, "saved", saved, (saved_n,), torch.float32)
+    guard = _layer_guard(who, stream, x, grad, gate, offsets, saved, initial, grad_final)
+    if guard is not None:
+        with guard:
+            return gated_scan_backward(grad, x, gate, offsets, saved, initial, grad_final)
+    dx, dgate = torch.empty_like(x), torch.empty_like(gate)
+    dinitial = None if initial is None else torch.empty_like(initial)
+    ws = _layer_workspace(x.device, need)
+    ptr = _native.ptr
+    _native.check(_native.lib().dgfx_gated_scan_backward(
+        ptr(x), ptr(gate), code, rows, channels, ptr(offsets), nseg, ptr(initial), ptr(saved), ptr(grad),
+        ptr(grad_final), ptr(dx), ptr(dgate), ptr(dinitial), ptr(ws), need, _native.raw_stream(x.get_device())))
     return dx, dgate, dinitial
 
 
@@ -653,19 +671,19 @@ def gated_scan_step(x, gate, state, out_state=None, stream=None):
     state' = a state + (1 - a) x with a = sigmoid(gate). x and gate [n, C],
     state float32 [n, C]; returns (h, state'), h in x's type. out_state may be
     ``state`` itself, which is then updated in place."""
-    import torch
-
     who = "gated_scan_step"
-    code = _layer_input(who, "x", x, (None, None), (torch.float32, torch.bfloat16))
-    n, channels = int(x.shape[0]), int(x.shape[1])
-    _layer_input(who, "gate", gate, x.shape, (x.dtype,))
-    _layer_input(who, "state", state, (n, channels), (torch.float32,))
+    n, channels, code = _layer_input(who, x)
+    _layer_operand(who, "gate", gate, x.shape, x.dtype)
+    _layer_operand(who, "state", state, (n, channels), torch.float32)
     if out_state is not None:
-        _layer_input(who, "out_state", out_state, (n, channels), (torch.float32,))
-    with _LayerLaunch(who, stream, x, gate, state, out_state) as sh:
-        h = torch.empty_like(x)
-        new_state = torch.empty_like(state) if out_state is None else out_state
-        _native.check(_native.lib().dgfx_gated_scan_step(
-            _native.ptr(x), _native.ptr(gate), code, n, channels, _native.ptr(state), _native.ptr(h),
-            _native.ptr(new_state), sh))
+        _layer_operand(who, "out_state", out_state, (n, channels), torch.float32)
+    guard = _layer_guard(who, stream, x, gate, state, out_state)
+    if guard is not None:
+        with guard:
+            return gated_scan_step(x, gate, state, out_state)
+    h = torch.empty_like(x)
+    new_state = torch.empty_like(state) if out_state is None else out_state
+    ptr = _native.ptr
+    _native.check(_native.lib().dgfx_gated_scan_step(
+        ptr(x), ptr(gate), code, n, channels, ptr(state), ptr(h), ptr(new_state), _native.raw_stream(x.get_device())))
     return h, new_state

@@ -810,7 +810,8 @@ int make_plan(const char* who, int64_t rows, int64_t channels, int64_t groups, i
   // kAhead rows per thread, or more than two as long as the teams do not fill
   // the GPU: more threads for the same segment repeat the fixed work of its
   // sums. It takes segments of up to eight steps; longer ones would hold up
-  // their block.
+  // their block. Only where 24 steps cover all rows it takes any: two more
+  // launches would cost as much.
   const int ahead = (dtype == DGFX_F32 ? kAhead<float> : kAhead<__nv_bfloat16>) / 2;
   const int64_t average = nseg > 0 ? ceil_div(rows, nseg) : 1;
   auto step_rows = [&](int team) { return static_cast<int64_t>(team / pl->quads) * ahead; };
@@ -821,7 +822,7 @@ int make_plan(const char* who, int64_t rows, int64_t channels, int64_t groups, i
   }
   pl->team = team;
   pl->threads = std::max(team, 256);
-  pl->loop_rows = 8 * step_rows(team);
+  pl->loop_rows = rows <= 24 * step_rows(team) ? rows : 8 * step_rows(team);
   pl->longs = rows > pl->loop_rows;
   const int per_sm = (backward ? 3 : 4) * 256 / pl->threads;
   pl->grid = static_cast<int32_t>(
