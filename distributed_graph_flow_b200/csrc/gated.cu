@@ -12,7 +12,7 @@
 // accumulate in fp32.
 //
 // One kernel body, four kinds of tile (128 rows by up to 256 accumulator
-// columns, K-blocks of 64):
+// columns per CTA, K-blocks of 64):
 //   kForward  A = X (K-major), B = BN rows of Wg above BN rows of Wu: one MMA
 //             gives the tile's g and u side by side in TMEM, and the
 //             epilogue writes h; neither projection leaves the SM.
@@ -24,11 +24,17 @@
 //   kWeights  dW: A = D, B = X, both MN-major (the contraction runs down the
 //             rows of both); the rows are split over CTAs, whose fp32
 //             tiles are added in order by gated_finish_kernel.
-// Warps: 0 TMA producer, 1 TMEM owner and MMA issuer, 2-9 epilogue (two per
-// TMEM lane quarter, half of the columns each). Two accumulators: the
-// epilogue of a tile runs beside the products of the next. Every wait is
+// Tiles of 256 columns run on pairs of CTAs (cta_group::2, 256 rows per
+// pair): each CTA loads its own A rows and half of B (for kForward one of
+// them Wg, the other Wu), so a K-block brings 32 KB into an SM instead of
+// 48, which with the operand reads is what its shared memory can carry at
+// the full MMA rate. Smaller products use single CTAs and 128 or 64 columns,
+// to spread over the SMs.
+// Warps: 0 TMA producer, 1 TMEM owner and MMA issuer (the pair's leader
+// issues), then the epilogue warps: four, two or one per TMEM lane quarter and group of columns.
+// Two accumulators: the epilogue of a tile runs beside the products of the next. Every wait is
 // bounded and latched in the status word of dgfx_dense_check; on expiry the roles leave,
-// copies and MMAs are drained and TMEM is freed. No multicast, no clusters.
+// copies and MMAs are drained and TMEM is freed. No multicast loads.
 #include <algorithm>
 
 #include "layer_math.cuh"
@@ -37,12 +43,8 @@
 namespace dgfx {
 namespace {
 
-constexpr int kBM = 128;
+constexpr int kBM = 128;  // rows per CTA
 constexpr int kBK = 64;
-constexpr int kStages = 4;
-constexpr int kEpilogueWarps = 8;
-constexpr int kThreads = 64 + 32 * kEpilogueWarps;
-constexpr uint32_t kStageOut = 4096;  // staging bytes per epilogue warp
 
 enum { kForward = 0, kGates = 1, kInput = 2, kWeights = 3 };
 
@@ -54,7 +56,7 @@ struct Args {
   int64_t m;
   int32_t n, k1, k2;
   int32_t kb1, kb_total;  // K-blocks of the first operand pair, of both
-  int32_t n_tiles, ctas_per_n;
+  int32_t n_tiles, units_per_n;
   int32_t cb1;        // kWeights: column blocks of X1
   int32_t kb_split;   // kWeights: K-blocks per split
   int32_t act;
@@ -63,18 +65,25 @@ struct Args {
   const __nv_bfloat16* dh;
   __nv_bfloat16* out;    // h, D, or dX1
   __nv_bfloat16* out2;   // dX2
-  float* partial;        // kGates: [4 ctas_per_n, 2 N] bias sums; kWeights: [splits, 2 N, K]
+  float* partial;        // kGates: [4 slots, 2 N] bias sums; kWeights: [splits, 2 N, K]
   unsigned int* err;
 };
 
-template <int NACC>
+// Per CTA. NACC accumulator columns; 256 of them on a pair of CTAs.
+template <int KIND, int NACC>
 struct Layout {
+  static constexpr int kGroup = NACC == 256 ? 2 : 1;            // CTAs that share a tile
+  static constexpr int kEpilogueWarps = NACC == 256 ? 16 : 8;
+  static constexpr int kThreads = 64 + 32 * kEpilogueWarps;
   static constexpr uint32_t kA = kBM * kBK * 2;
-  static constexpr uint32_t kB = NACC * kBK * 2;
+  static constexpr uint32_t kB = NACC / kGroup * kBK * 2;
   static constexpr uint32_t kStage = kA + kB;
+  static constexpr uint32_t kOutWarp = KIND == kGates ? 4096 : 2048;  // staging bytes per epilogue warp
+  static constexpr int kStages = NACC != 256 ? 4 : (KIND == kGates ? 5 : 6);
   static constexpr uint32_t kTmemCols = 2 * NACC;
-  static constexpr size_t kBytes = static_cast<size_t>(kStages) * kStage + kEpilogueWarps * kStageOut +
+  static constexpr size_t kBytes = static_cast<size_t>(kStages) * kStage + kEpilogueWarps * kOutWarp +
                                    NACC * sizeof(float) /* biases */ + 1024 /* align */ + 256 /* barriers */;
+  static_assert(kBytes <= 232448, "shared memory of a CTA");
 };
 
 // Two 16-column pieces of the accumulators (all 32 lanes of this warp's
@@ -142,43 +151,44 @@ __device__ __forceinline__ float transpose_sum(float (&v)[32]) {
   return v[0];
 }
 
-// The tiles of one CTA. Kinds with a fixed column block per CTA walk down the
-// row blocks; kWeights has one tile and one range of K-blocks.
-template <int KIND>
+// The tiles of one CTA or pair (`unit`). Kinds with a fixed column block per
+// unit walk down the row blocks; kWeights has one tile and one range of K-blocks.
+template <int KIND, int GROUP>
 struct Walk {
-  int32_t nb, m_tiles, step, mb;
+  int32_t unit, rank, nb, m_tiles, step, mb;
   int32_t kb_begin, kb_end;
   __device__ Walk(const Args& p) {
+    rank = GROUP == 2 ? static_cast<int32_t>(cluster_rank()) : 0;
+    unit = static_cast<int32_t>(blockIdx.x) / GROUP;
+    nb = unit % p.n_tiles;
     if (KIND == kWeights) {
-      nb = static_cast<int32_t>(blockIdx.x) % p.n_tiles;  // output tile
-      const int32_t split = static_cast<int32_t>(blockIdx.x) / p.n_tiles;
       m_tiles = 1;
       step = 1;
       mb = 0;
-      kb_begin = split * p.kb_split;
+      kb_begin = unit / p.n_tiles * p.kb_split;
       kb_end = min(kb_begin + p.kb_split, p.kb_total);
     } else {
-      nb = static_cast<int32_t>(blockIdx.x) % p.n_tiles;
-      mb = static_cast<int32_t>(blockIdx.x) / p.n_tiles;
-      step = p.ctas_per_n;
-      m_tiles = static_cast<int32_t>((p.m + kBM - 1) / kBM);
+      mb = unit / p.n_tiles;
+      step = p.units_per_n;
+      m_tiles = static_cast<int32_t>((p.m + kBM * GROUP - 1) / (kBM * GROUP));
       kb_begin = 0;
       kb_end = p.kb_total;
     }
   }
+  // First row of this CTA in row block mb.
+  __device__ int32_t row(int32_t mb_) const { return (mb_ * GROUP + rank) * kBM; }
 };
 
-// kWeights: output tile `t` -> half (0 gate, 1 up), its first row n0, the
-// operand and first column of X, and that column in K.
+// kWeights: output tile `t` -> its first row in [dWg; dWu], the operand and
+// first column of X, and that column in K.
 struct WeightTile {
-  int32_t half, n0, col0, kcol0, kcols;
+  int32_t row0, col0, kcol0, kcols;
   bool second;
-  __device__ WeightTile(const Args& p, int32_t t, int nacc) {
-    const int32_t row_blocks = (p.n + kBM - 1) / kBM;
-    const int32_t col_blocks = p.n_tiles / (2 * row_blocks);
+  __device__ WeightTile(const Args& p, int32_t t, int tile_rows, int nacc) {
+    const int32_t row_blocks = (2 * p.n + tile_rows - 1) / tile_rows;
+    const int32_t col_blocks = p.n_tiles / row_blocks;
     const int32_t rb = t / col_blocks, cb = t - rb * col_blocks;
-    half = rb / row_blocks;
-    n0 = (rb - half * row_blocks) * kBM;
+    row0 = rb * tile_rows;
     second = cb >= p.cb1;
     col0 = (second ? cb - p.cb1 : cb) * nacc;
     kcol0 = (second ? p.k1 : 0) + col0;
@@ -186,34 +196,48 @@ struct WeightTile {
   }
 };
 
+template <int GROUP>
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, uint32_t bar, int32_t x, int32_t y) {
+  if (GROUP == 2) tma_load_2d_pair(dst, map, bar, x, y);
+  else tma_load_2d(dst, map, bar, x, y);
+}
+
 template <int KIND, int NACC>
-__device__ __forceinline__ void load_stage(const Maps& maps, const Args& p, const Walk<KIND>& w, int32_t mb, int32_t kb,
-                                           uint32_t a_dst, uint32_t bar) {
-  constexpr int BN = NACC / 2;
-  const uint32_t b_dst = a_dst + Layout<NACC>::kA;
+__device__ __forceinline__ void load_stage(const Maps& maps, const Args& p, const Walk<KIND, Layout<KIND, NACC>::kGroup>& w,
+                                           int32_t mb, int32_t kb, uint32_t a_dst, uint32_t bar) {
+  using L = Layout<KIND, NACC>;
+  constexpr int G = L::kGroup;
+  const uint32_t b_dst = a_dst + L::kA;
   if (KIND == kForward || KIND == kGates) {
+    constexpr int BN = NACC / 2;
     const bool first = kb < p.kb1;
     const int32_t x = (first ? kb : kb - p.kb1) * kBK;
-    tma_load_2d(a_dst, first ? &maps.a1 : &maps.a2, bar, x, mb * kBM);
-    tma_load_2d(b_dst, first ? &maps.b1 : &maps.b2, bar, x, w.nb * BN);
-    tma_load_2d(b_dst + BN * kBK * 2, first ? &maps.b3 : &maps.b4, bar, x, w.nb * BN);
+    load_box<G>(a_dst, first ? &maps.a1 : &maps.a2, bar, x, w.row(mb));
+    const CUtensorMap* gate = first ? &maps.b1 : &maps.b2;
+    const CUtensorMap* up = first ? &maps.b3 : &maps.b4;
+    if (G == 2) {
+      load_box<G>(b_dst, w.rank == 0 ? gate : up, bar, x, w.nb * BN);
+    } else {
+      load_box<G>(b_dst, gate, bar, x, w.nb * BN);
+      load_box<G>(b_dst + BN * kBK * 2, up, bar, x, w.nb * BN);
+    }
   } else if (KIND == kInput) {
     const bool first = kb < p.kb1;
     const int32_t x = (first ? kb : kb - p.kb1) * kBK;
-    tma_load_2d(a_dst, first ? &maps.a1 : &maps.a2, bar, x, mb * kBM);
+    load_box<G>(a_dst, first ? &maps.a1 : &maps.a2, bar, x, w.row(mb));
 #pragma unroll
-    for (int j = 0; j < NACC / 64; ++j) {
-      tma_load_2d(b_dst + j * 8192, first ? &maps.b1 : &maps.b2, bar, w.nb * NACC + j * 64, x);
+    for (int j = 0; j < NACC / G / 64; ++j) {
+      load_box<G>(b_dst + j * 8192, first ? &maps.b1 : &maps.b2, bar, w.nb * NACC + w.rank * (NACC / G) + j * 64, x);
     }
   } else {
-    const WeightTile t(p, w.nb, NACC);
+    const WeightTile t(p, w.nb, kBM * G, NACC);
 #pragma unroll
     for (int j = 0; j < kBM / 64; ++j) {
-      tma_load_2d(a_dst + j * 8192, &maps.a1, bar, t.half * p.n + t.n0 + j * 64, kb * kBK);
+      load_box<G>(a_dst + j * 8192, &maps.a1, bar, t.row0 + w.rank * kBM + j * 64, kb * kBK);
     }
 #pragma unroll
-    for (int j = 0; j < NACC / 64; ++j) {
-      tma_load_2d(b_dst + j * 8192, t.second ? &maps.b2 : &maps.b1, bar, t.col0 + j * 64, kb * kBK);
+    for (int j = 0; j < NACC / G / 64; ++j) {
+      load_box<G>(b_dst + j * 8192, t.second ? &maps.b2 : &maps.b1, bar, t.col0 + w.rank * (NACC / G) + j * 64, kb * kBK);
     }
   }
 }
@@ -235,32 +259,33 @@ __device__ __forceinline__ void store_bf16(const uint8_t* stage, __nv_bfloat16* 
 }
 
 template <int KIND, int NACC>
-__global__ void __launch_bounds__(kThreads, 1) gated_kernel(const __grid_constant__ Maps maps, const Args p) {
-  using L = Layout<NACC>;
-  constexpr int BN = NACC / 2;
+__device__ __forceinline__ void gated_body(const Maps& maps, const Args& p) {
+  using L = Layout<KIND, NACC>;
+  constexpr int G = L::kGroup, BN = NACC / 2, S = L::kStages;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  // 128-byte swizzled tiles need 1024-byte aligned shared addresses.
+  // 128-byte swizzled tiles need 1024-byte aligned shared addresses (the same
+  // offset in both CTAs of a pair).
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  uint8_t* out_stage = smem + kStages * L::kStage;
-  float* biases = reinterpret_cast<float*>(out_stage + kEpilogueWarps * kStageOut);
+  uint8_t* out_stage = smem + S * L::kStage;
+  float* biases = reinterpret_cast<float*>(out_stage + L::kEpilogueWarps * L::kOutWarp);
   uint64_t* bars = reinterpret_cast<uint64_t*>(biases + NACC);
-  // bars: full[kStages], empty[kStages], acc_full[2], acc_empty[2], drain
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 5);
+  // bars: full[S], empty[S], acc_full[2], acc_empty[2], drain
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S + 5);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + kStages);
-  const uint32_t accf0 = smem_u32(bars + 2 * kStages), acce0 = smem_u32(bars + 2 * kStages + 2);
-  const uint32_t drain = smem_u32(bars + 2 * kStages + 4);
+  const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + S);
+  const uint32_t accf0 = smem_u32(bars + 2 * S), acce0 = smem_u32(bars + 2 * S + 2);
+  const uint32_t drain = smem_u32(bars + 2 * S + 4);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const Walk<KIND> w(p);
+  const Walk<KIND, G> w(p);
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) {
+    for (int s = 0; s < S; ++s) {
       mbar_init(full0 + 8 * s, 1);
       mbar_init(empty0 + 8 * s, 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(accf0 + 8 * b, 1);
-      mbar_init(acce0 + 8 * b, kEpilogueWarps);
+      mbar_init(acce0 + 8 * b, G * L::kEpilogueWarps);
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -268,25 +293,35 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const __grid_constan
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   if (KIND == kForward || KIND == kGates) {
-    for (int i = threadIdx.x; i < NACC; i += kThreads) {
+    for (int i = threadIdx.x; i < NACC; i += L::kThreads) {
       const int32_t col = w.nb * BN + (i < BN ? i : i - BN);
       const float* b = i < BN ? p.b_gate : p.b_up;
       biases[i] = b != nullptr && col < p.n ? b[col] : 0.0f;
     }
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                 "r"(L::kTmemCols)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if (G == 2) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                   "r"(L::kTmemCols)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                   "r"(L::kTmemCols)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
   }
   tc_fence_before();
   __syncthreads();
+  if (G == 2) cluster_sync();  // the peer's barriers are ready
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
   if (warp == 0) {
     if (lane == 0) {
+      // Loads report to the leader's barriers.
+      const uint32_t report0 = G == 2 ? map_rank(full0, 0) : full0;
       int s = 0;
       uint32_t ph = 0;
       uint32_t issued = 0;  // stages with a load issued in the current ring pass
@@ -297,10 +332,10 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const __grid_constan
             ok = false;
             break;
           }
-          mbar_arrive_expect_tx(full0 + 8 * s, L::kStage);
-          load_stage<KIND, NACC>(maps, p, w, mb, kb, smem_u32(smem + s * L::kStage), full0 + 8 * s);
+          if (w.rank == 0) mbar_arrive_expect_tx(full0 + 8 * s, G * L::kStage);
+          load_stage<KIND, NACC>(maps, p, w, mb, kb, smem_u32(smem + s * L::kStage), report0 + 8 * s);
           issued |= 1u << s;
-          if (++s == kStages) {
+          if (++s == S) {
             s = 0;
             ph ^= 1u;
             issued = 0;
@@ -309,7 +344,10 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const __grid_constan
       }
       if (!ok) {
         // Drain: every stage loaded in this pass completes its transaction.
-        for (int j = 0; j < kStages; ++j) {
+        // The second CTA of a pair cannot see it and gives its copies time.
+        const uint64_t t1 = now_ns();
+        while (w.rank != 0 && now_ns() - t1 < 10000000ull) __nanosleep(1000);
+        for (int j = 0; j < S && w.rank == 0; ++j) {
           if (issued & (1u << j)) {
             const uint64_t t0 = now_ns();
             while (!mbar_test(full0 + 8 * j, ph) && now_ns() - t0 < kWaitNs) __nanosleep(100);
@@ -319,11 +357,15 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const __grid_constan
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (lane == 0 && w.rank == 0) {
       constexpr bool kAMn = KIND == kWeights, kBMn = KIND == kWeights || KIND == kInput;
-      constexpr uint32_t idesc = idesc_bf16(kBM, NACC, kAMn, kBMn);
+      constexpr uint32_t idesc = idesc_bf16(kBM * G, NACC, kAMn, kBMn);
       // A K step of 16: 32 bytes inside the swizzle atom, or 16 rows of 128.
       constexpr uint32_t kAStep = kAMn ? 2048 >> 4 : 32 >> 4, kBStep = kBMn ? 2048 >> 4 : 32 >> 4;
+      auto commit = [](uint32_t bar) {
+        if (G == 2) mma_commit_pair(bar);
+        else mma_commit(bar);
+      };
       int s = 0;
       uint32_t ph = 0;
       int b = 0;
@@ -345,17 +387,19 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const __grid_constan
           const uint64_t bdesc = kBMn ? smem_desc_sw128_mn(a_addr + L::kA) : smem_desc_sw128(a_addr + L::kA);
 #pragma unroll
           for (int k = 0; k < kBK / 16; ++k) {
-            mma_bf16(d_tmem, adesc + kAStep * k, bdesc + kBStep * k, idesc, (kb != w.kb_begin || k != 0) ? 1u : 0u);
+            const uint32_t accumulate = (kb != w.kb_begin || k != 0) ? 1u : 0u;
+            if (G == 2) mma_bf16_pair(d_tmem, adesc + kAStep * k, bdesc + kBStep * k, idesc, accumulate);
+            else mma_bf16(d_tmem, adesc + kAStep * k, bdesc + kBStep * k, idesc, accumulate);
           }
           any = true;
-          mma_commit(empty0 + 8 * s);
-          if (++s == kStages) {
+          commit(empty0 + 8 * s);
+          if (++s == S) {
             s = 0;
             ph ^= 1u;
           }
         }
         if (!ok) break;
-        mma_commit(accf0 + 8 * b);
+        commit(accf0 + 8 * b);
         if (++b == 2) {
           b = 0;
           aph ^= 1u;
@@ -363,40 +407,50 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const __grid_constan
       }
       if (any) {
         // All MMAs issued by this thread are complete once `drain` fires.
-        mma_commit(drain);
+        commit(drain);
         const uint64_t t0 = now_ns();
         while (!mbar_test(drain, 0) && now_ns() - t0 < kWaitNs) __nanosleep(100);
       }
     }
     __syncwarp();
   } else {
-    const int q = warp & 3;             // TMEM lane quarter: rows 32 q ..
-    const int half = (warp - 2) >> 2;   // half of the tile's columns
+    const int q = warp & 3;            // TMEM lane quarter: rows 32 q ..
+    const int part = (warp - 2) >> 2;  // this warp's group of columns
+    constexpr int kParts = L::kEpilogueWarps / 4;
     const uint32_t lane_off = static_cast<uint32_t>(32 * q) << 16;
-    uint8_t* stage = out_stage + (warp - 2) * kStageOut;
+    uint8_t* stage = out_stage + (warp - 2) * L::kOutWarp;
+    const uint32_t acce_leader = G == 2 ? map_rank(acce0, 0) : acce0;
+    auto release = [&](int b) {  // this warp has read accumulator b
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (G == 2) mbar_arrive_cluster(acce_leader + 8 * b);
+        else mbar_arrive(acce0 + 8 * b);
+      }
+    };
     int b = 0;
     uint32_t aph = 0;
-    constexpr int kChunks = BN / 2 / 16;  // 16-column pieces of a warp's half (kForward, kGates)
+    constexpr int GC = BN / kParts;  // columns of g and u per warp: 32, or 16 at 64 accumulator columns
+    constexpr int kChunks = GC / 16;
+    constexpr int GP = GC / 8;       // 16-byte pieces of them
     float bias_sum[kChunks];
     if (KIND == kGates) {
 #pragma unroll
       for (int c = 0; c < kChunks; ++c) bias_sum[c] = 0.0f;
     }
     for (int32_t mb = w.mb; mb < w.m_tiles; mb += w.step) {
-      const int64_t row0 = static_cast<int64_t>(mb) * kBM + 32 * q;
+      const int64_t row0 = static_cast<int64_t>(w.row(mb)) + 32 * q;
       const bool row_ok = row0 + lane < p.m;
-      // kGates: the first piece of dh, on its way while the products run.
-      constexpr int CW = BN / 2 < 32 ? BN / 2 : 32;  // columns staged at a time
-      constexpr int GP = CW / 8;
-      uint4 dh_next[GP];
+      const int32_t gcol0 = w.nb * BN + part * GC;
+      // kGates: this warp's piece of dh, on its way while the products run.
+      uint4 dh[GP];
       if (KIND == kGates) {
 #pragma unroll
         for (int k = 0; k < GP; ++k) {
           const int i = lane + 32 * k, r = i / GP, j = i % GP;
-          const int32_t col = w.nb * BN + half * (BN / 2) + j * 8;
-          dh_next[k] = row0 + r < p.m && col < p.n
-                           ? __ldg(reinterpret_cast<const uint4*>(p.dh + (row0 + r) * p.n + col))
-                           : make_uint4(0, 0, 0, 0);
+          dh[k] = row0 + r < p.m && gcol0 + j * 8 < p.n
+                      ? __ldg(reinterpret_cast<const uint4*>(p.dh + (row0 + r) * p.n + gcol0 + j * 8))
+                      : make_uint4(0, 0, 0, 0);
         }
       }
       bool ready = true;
@@ -407,10 +461,9 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const __grid_constan
       const uint32_t acc = tmem_base + lane_off + static_cast<uint32_t>(b * NACC);
 
       if (KIND == kForward) {
-        constexpr int P = BN / 16;  // 16-byte pieces per row of a warp's half
-#pragma unroll 1
+#pragma unroll
         for (int c = 0; c < kChunks; ++c) {
-          const int lc = half * (BN / 2) + c * 16;
+          const int lc = part * GC + c * 16;
           uint32_t gr[16], ur[16];
           tmem_ld_2x16(acc + lc, acc + BN + lc, gr, ur);
           float g[16], u[16];
@@ -428,130 +481,96 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const __grid_constan
           }
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            *reinterpret_cast<uint4*>(stage + piece_at<P>(lane, c * 2 + j)) =
+            *reinterpret_cast<uint4*>(stage + piece_at<GP>(lane, c * 2 + j)) =
                 make_uint4(pack_bf16(g[8 * j], g[8 * j + 1]), pack_bf16(g[8 * j + 2], g[8 * j + 3]),
                            pack_bf16(g[8 * j + 4], g[8 * j + 5]), pack_bf16(g[8 * j + 6], g[8 * j + 7]));
           }
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(acce0 + 8 * b);
-        const int32_t col0 = w.nb * BN + half * (BN / 2);
-        store_bf16<P>(stage, p.out, p.n, row0, p.m, col0, p.n - col0);
+        release(b);
+        store_bf16<GP>(stage, p.out, p.n, row0, p.m, gcol0, p.n - gcol0);
         __syncwarp();
       } else if (KIND == kGates) {
-        uint8_t* stage2 = stage + kStageOut / 2;  // dg goes where dh was, du here
-        constexpr int kSub = CW / 16;
+        uint8_t* stage2 = stage + L::kOutWarp / 2;  // dg goes where dh was, du here
 #pragma unroll
-        for (int cc = 0; cc < BN / 2 / CW; ++cc) {
-#pragma unroll
-          for (int k = 0; k < GP; ++k) {
-            const int i = lane + 32 * k;
-            *reinterpret_cast<uint4*>(stage + piece_at<GP>(i / GP, i % GP)) = dh_next[k];
-          }
-          if (cc + 1 < BN / 2 / CW) {
-#pragma unroll
-            for (int k = 0; k < GP; ++k) {
-              const int i = lane + 32 * k, r = i / GP, j = i % GP;
-              const int32_t col = w.nb * BN + half * (BN / 2) + (cc + 1) * CW + j * 8;
-              dh_next[k] = row0 + r < p.m && col < p.n
-                               ? __ldg(reinterpret_cast<const uint4*>(p.dh + (row0 + r) * p.n + col))
-                               : make_uint4(0, 0, 0, 0);
-            }
-          }
-          __syncwarp();
-#pragma unroll
-          for (int c = 0; c < kSub; ++c) {
-            const int lc = half * (BN / 2) + cc * CW + c * 16;
-            uint32_t gr[16], ur[16];
-            tmem_ld_2x16(acc + lc, acc + BN + lc, gr, ur);
-            float g[16], u[16], d[16];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              float f[8];
-              Vec16<__nv_bfloat16>::unpack(*reinterpret_cast<const uint4*>(stage + piece_at<GP>(lane, c * 2 + j)), f);
-#pragma unroll
-              for (int i = 0; i < 8; ++i) d[8 * j + i] = f[i];
-            }
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              g[j] = __uint_as_float(gr[j]) + biases[lc + j];
-              u[j] = __uint_as_float(ur[j]) + biases[BN + lc + j];
-            }
-            switch (p.act) {
-              case DGFX_ACT_RELU: gate_backward<DGFX_ACT_RELU>(g, u, d); break;
-              case DGFX_ACT_SILU: gate_backward<DGFX_ACT_SILU>(g, u, d); break;
-              case DGFX_ACT_GELU: gate_backward<DGFX_ACT_GELU>(g, u, d); break;
-              case DGFX_ACT_SIGMOID: gate_backward<DGFX_ACT_SIGMOID>(g, u, d); break;
-              default: gate_backward<DGFX_ACT_NONE>(g, u, d); break;
-            }
-            float v[32];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              v[j] = row_ok ? g[j] : 0.0f;
-              v[16 + j] = row_ok ? u[j] : 0.0f;
-            }
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              *reinterpret_cast<uint4*>(stage + piece_at<GP>(lane, c * 2 + j)) =
-                  make_uint4(pack_bf16(g[8 * j], g[8 * j + 1]), pack_bf16(g[8 * j + 2], g[8 * j + 3]),
-                             pack_bf16(g[8 * j + 4], g[8 * j + 5]), pack_bf16(g[8 * j + 6], g[8 * j + 7]));
-              *reinterpret_cast<uint4*>(stage2 + piece_at<GP>(lane, c * 2 + j)) =
-                  make_uint4(pack_bf16(u[8 * j], u[8 * j + 1]), pack_bf16(u[8 * j + 2], u[8 * j + 3]),
-                             pack_bf16(u[8 * j + 4], u[8 * j + 5]), pack_bf16(u[8 * j + 6], u[8 * j + 7]));
-            }
-            bias_sum[cc * kSub + c] += transpose_sum(v);
-          }
-          if (cc + 1 == BN / 2 / CW) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(acce0 + 8 * b);
-          } else {
-            __syncwarp();
-          }
-          const int32_t col0 = w.nb * BN + half * (BN / 2) + cc * CW;
-          store_bf16<GP>(stage, p.out, 2 * static_cast<int64_t>(p.n), row0, p.m, col0, p.n - col0);
-          store_bf16<GP>(stage2, p.out + p.n, 2 * static_cast<int64_t>(p.n), row0, p.m, col0, p.n - col0);
-          __syncwarp();
+        for (int k = 0; k < GP; ++k) {
+          const int i = lane + 32 * k;
+          *reinterpret_cast<uint4*>(stage + piece_at<GP>(i / GP, i % GP)) = dh[k];
         }
+        __syncwarp();
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+          const int lc = part * GC + c * 16;
+          uint32_t gr[16], ur[16];
+          tmem_ld_2x16(acc + lc, acc + BN + lc, gr, ur);
+          float g[16], u[16], d[16];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float f[8];
+            Vec16<__nv_bfloat16>::unpack(*reinterpret_cast<const uint4*>(stage + piece_at<GP>(lane, c * 2 + j)), f);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) d[8 * j + i] = f[i];
+          }
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            g[j] = __uint_as_float(gr[j]) + biases[lc + j];
+            u[j] = __uint_as_float(ur[j]) + biases[BN + lc + j];
+          }
+          switch (p.act) {
+            case DGFX_ACT_RELU: gate_backward<DGFX_ACT_RELU>(g, u, d); break;
+            case DGFX_ACT_SILU: gate_backward<DGFX_ACT_SILU>(g, u, d); break;
+            case DGFX_ACT_GELU: gate_backward<DGFX_ACT_GELU>(g, u, d); break;
+            case DGFX_ACT_SIGMOID: gate_backward<DGFX_ACT_SIGMOID>(g, u, d); break;
+            default: gate_backward<DGFX_ACT_NONE>(g, u, d); break;
+          }
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            *reinterpret_cast<uint4*>(stage + piece_at<GP>(lane, c * 2 + j)) =
+                make_uint4(pack_bf16(g[8 * j], g[8 * j + 1]), pack_bf16(g[8 * j + 2], g[8 * j + 3]),
+                           pack_bf16(g[8 * j + 4], g[8 * j + 5]), pack_bf16(g[8 * j + 6], g[8 * j + 7]));
+            *reinterpret_cast<uint4*>(stage2 + piece_at<GP>(lane, c * 2 + j)) =
+                make_uint4(pack_bf16(u[8 * j], u[8 * j + 1]), pack_bf16(u[8 * j + 2], u[8 * j + 3]),
+                           pack_bf16(u[8 * j + 4], u[8 * j + 5]), pack_bf16(u[8 * j + 6], u[8 * j + 7]));
+          }
+          float v[32];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            v[j] = row_ok ? g[j] : 0.0f;
+            v[16 + j] = row_ok ? u[j] : 0.0f;
+          }
+          bias_sum[c] += transpose_sum(v);
+        }
+        release(b);
+        store_bf16<GP>(stage, p.out, 2 * static_cast<int64_t>(p.n), row0, p.m, gcol0, p.n - gcol0);
+        store_bf16<GP>(stage2, p.out + p.n, 2 * static_cast<int64_t>(p.n), row0, p.m, gcol0, p.n - gcol0);
+        __syncwarp();
       } else if (KIND == kInput) {
         const int32_t kk = p.k1 + p.k2;
-#pragma unroll 1
-        for (int cc = 0; cc < BN / 64 + (BN < 64 ? 1 : 0); ++cc) {
-          constexpr int W = BN < 64 ? BN : 64;  // columns staged at a time
-          constexpr int P = W / 8;
-          const int lc = half * BN + cc * W;
+        constexpr int C = NACC / kParts;  // columns per warp, 32 staged at a time
 #pragma unroll
-          for (int c = 0; c < W / 32; ++c) {
-            uint32_t v0[16], v1[16];
-            tmem_ld_2x16(acc + lc + c * 32, acc + lc + c * 32 + 16, v0, v1);
+        for (int cc = 0; cc < C / 32; ++cc) {
+          const int lc = part * C + cc * 32;
+          uint32_t v0[16], v1[16];
+          tmem_ld_2x16(acc + lc, acc + lc + 16, v0, v1);
+          if (cc + 1 == C / 32) release(b);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              uint32_t o[4], o2[4];
+          for (int j = 0; j < 2; ++j) {
+            uint32_t o[4], o2[4];
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                o[i] = pack_bf16(__uint_as_float(v0[8 * j + 2 * i]), __uint_as_float(v0[8 * j + 2 * i + 1]));
-                o2[i] = pack_bf16(__uint_as_float(v1[8 * j + 2 * i]), __uint_as_float(v1[8 * j + 2 * i + 1]));
-              }
-              *reinterpret_cast<uint4*>(stage + piece_at<P>(lane, c * 4 + j)) = make_uint4(o[0], o[1], o[2], o[3]);
-              *reinterpret_cast<uint4*>(stage + piece_at<P>(lane, c * 4 + 2 + j)) =
-                  make_uint4(o2[0], o2[1], o2[2], o2[3]);
+            for (int i = 0; i < 4; ++i) {
+              o[i] = pack_bf16(__uint_as_float(v0[8 * j + 2 * i]), __uint_as_float(v0[8 * j + 2 * i + 1]));
+              o2[i] = pack_bf16(__uint_as_float(v1[8 * j + 2 * i]), __uint_as_float(v1[8 * j + 2 * i + 1]));
             }
+            *reinterpret_cast<uint4*>(stage + piece_at<4>(lane, j)) = make_uint4(o[0], o[1], o[2], o[3]);
+            *reinterpret_cast<uint4*>(stage + piece_at<4>(lane, 2 + j)) = make_uint4(o2[0], o2[1], o2[2], o2[3]);
           }
-          if (lc + W == (half + 1) * BN) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(acce0 + 8 * b);
-          } else {
-            __syncwarp();
-          }
+          __syncwarp();
           const int32_t col0 = w.nb * NACC + lc;
 #pragma unroll
-          for (int k = 0; k < P; ++k) {
-            const int i = lane + 32 * k, r = i / P, j = i % P;
+          for (int k = 0; k < 4; ++k) {
+            const int i = lane + 32 * k, r = i / 4, j = i % 4;
             const int32_t col = col0 + j * 8;
             if (row0 + r < p.m && col < kk) {
-              const uint4 v = *reinterpret_cast<const uint4*>(stage + piece_at<P>(r, j));
+              const uint4 v = *reinterpret_cast<const uint4*>(stage + piece_at<4>(r, j));
               if (col < p.k1) {
                 if (p.out != nullptr) *reinterpret_cast<uint4*>(p.out + (row0 + r) * p.k1 + col) = v;
               } else if (p.out2 != nullptr) {
@@ -562,37 +581,37 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const __grid_constan
           __syncwarp();
         }
       } else {
-        const WeightTile t(p, w.nb, NACC);
+        const WeightTile t(p, w.nb, kBM * G, NACC);
         const int64_t kk = p.k1 + p.k2;
-        const int32_t split = static_cast<int32_t>(blockIdx.x) / p.n_tiles;
-        float* out = p.partial + (static_cast<int64_t>(split) * 2 * p.n + static_cast<int64_t>(t.half) * p.n) * kk;
-        const int32_t n_row = t.n0 + 32 * q;
+        float* out = p.partial + static_cast<int64_t>(w.unit / p.n_tiles) * 2 * p.n * kk;
+        const int32_t n_row = t.row0 + w.rank * kBM + 32 * q;
+        constexpr int C = NACC / kParts;  // columns per warp, 16 staged at a time
 #pragma unroll 1
-        for (int cc = 0; cc < BN / 32; ++cc) {
-          const int lc = half * BN + cc * 32;
-          uint32_t v0[16], v1[16];
-          tmem_ld_2x16(acc + lc, acc + lc + 16, v0, v1);
+        for (int cc = 0; cc < C / 32; ++cc) {
+          const int lc = part * C + cc * 32;
+          uint32_t v[2][16];
+          tmem_ld_2x16(acc + lc, acc + lc + 16, v[0], v[1]);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            *reinterpret_cast<uint4*>(stage + piece_at<8>(lane, j)) =
-                make_uint4(v0[4 * j], v0[4 * j + 1], v0[4 * j + 2], v0[4 * j + 3]);
-            *reinterpret_cast<uint4*>(stage + piece_at<8>(lane, 4 + j)) =
-                make_uint4(v1[4 * j], v1[4 * j + 1], v1[4 * j + 2], v1[4 * j + 3]);
-          }
-          __syncwarp();
+          for (int half = 0; half < 2; ++half) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const int i = lane + 32 * k, r = i / 8, j = i % 8;
-            if (n_row + r < p.n && lc + j * 4 < t.kcols) {
-              *reinterpret_cast<uint4*>(out + (n_row + r) * kk + t.kcol0 + lc + j * 4) =
-                  *reinterpret_cast<const uint4*>(stage + piece_at<8>(r, j));
+            for (int j = 0; j < 4; ++j) {
+              *reinterpret_cast<uint4*>(stage + piece_at<4>(lane, j)) =
+                  make_uint4(v[half][4 * j], v[half][4 * j + 1], v[half][4 * j + 2], v[half][4 * j + 3]);
             }
+            __syncwarp();
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int i = lane + 32 * k, r = i / 4, j = i % 4;
+              const int32_t col = lc + half * 16 + j * 4;
+              if (n_row + r < 2 * p.n && col < t.kcols) {
+                *reinterpret_cast<uint4*>(out + (n_row + r) * kk + t.kcol0 + col) =
+                    *reinterpret_cast<const uint4*>(stage + piece_at<4>(r, j));
+              }
+            }
+            __syncwarp();
           }
-          __syncwarp();
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(acce0 + 8 * b);
+        release(b);
       }
       if (++b == 2) {
         b = 0;
@@ -600,11 +619,11 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const __grid_constan
       }
     }
     if (KIND == kGates) {
-      // Lane l of a piece holds the sum of column l of dg (l < 16) or du.
-      const int64_t slot = (static_cast<int64_t>(blockIdx.x) / p.n_tiles) * 4 + q;
+      // Lane l of a chunk holds the sum of column l of dg (l < 16) or du.
+      const int64_t slot = (static_cast<int64_t>(w.unit / p.n_tiles) * G + w.rank) * 4 + q;
 #pragma unroll
       for (int c = 0; c < kChunks; ++c) {
-        const int32_t col = w.nb * BN + half * (BN / 2) + c * 16 + (lane & 15);
+        const int32_t col = w.nb * BN + part * GC + c * 16 + (lane & 15);
         if (col < p.n) p.partial[(slot * 2 + (lane >> 4)) * p.n + col] = bias_sum[c];
       }
     }
@@ -612,11 +631,29 @@ __global__ void __launch_bounds__(kThreads, 1) gated_kernel(const __grid_constan
 
   tc_fence_before();
   __syncthreads();
+  if (G == 2) cluster_sync();  // the peer still reads this CTA's operands and barriers until here
   tc_fence_after();
   if (warp == 1) {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(L::kTmemCols)
-                 : "memory");
+    if (G == 2) {
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(L::kTmemCols)
+                   : "memory");
+    } else {
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(L::kTmemCols)
+                   : "memory");
+    }
   }
+}
+
+template <int KIND, int NACC>
+__global__ void __launch_bounds__(Layout<KIND, NACC>::kThreads, 1)
+    gated_kernel(const __grid_constant__ Maps maps, const Args p) {
+  gated_body<KIND, NACC>(maps, p);
+}
+
+template <int KIND>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Layout<KIND, 256>::kThreads, 1)
+    gated_pair_kernel(const __grid_constant__ Maps maps, const Args p) {
+  gated_body<KIND, 256>(maps, p);
 }
 
 // dW from the splits' fp32 tiles and the bias gradients from the CTAs' sums,
@@ -665,28 +702,35 @@ __global__ void __launch_bounds__(256) gated_finish_kernel(const float* __restri
   }
 }
 
-template <int KIND, int NACC>
-int launch(const Maps& maps, const Args& p, int grid, cudaStream_t stream) {
-  static std::once_flag once[64];
+template <class K>
+int launch(K kernel, size_t smem, int threads, std::once_flag* once, const Maps& maps, const Args& p, int grid,
+           cudaStream_t stream) {
   int dev = 0;
   DGFX_CUDA_TRY(cudaGetDevice(&dev));
   cudaError_t attr_err = cudaSuccess;
   std::call_once(once[dev & 63], [&]() {
-    attr_err = cudaFuncSetAttribute(gated_kernel<KIND, NACC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    static_cast<int>(Layout<NACC>::kBytes));
+    attr_err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   });
   DGFX_CUDA_TRY(attr_err);
-  gated_kernel<KIND, NACC><<<grid, kThreads, Layout<NACC>::kBytes, stream>>>(maps, p);
+  kernel<<<grid, threads, smem, stream>>>(maps, p);
   DGFX_CUDA_TRY(cudaGetLastError());
   return DGFX_OK;
 }
 
+// `units`: CTAs, or pairs of them at 256 accumulator columns.
 template <int KIND>
-int launch_nacc(int nacc, const Maps& maps, const Args& p, int grid, cudaStream_t stream) {
+int launch_nacc(int nacc, const Maps& maps, const Args& p, int units, cudaStream_t stream) {
+  static std::once_flag once[3][64];
   switch (nacc) {
-    case 256: return launch<KIND, 256>(maps, p, grid, stream);
-    case 128: return launch<KIND, 128>(maps, p, grid, stream);
-    default: return launch<KIND, 64>(maps, p, grid, stream);
+    case 256:
+      return launch(gated_pair_kernel<KIND>, Layout<KIND, 256>::kBytes, Layout<KIND, 256>::kThreads, once[0], maps, p,
+                    2 * units, stream);
+    case 128:
+      return launch(gated_kernel<KIND, 128>, Layout<KIND, 128>::kBytes, Layout<KIND, 128>::kThreads, once[1], maps, p,
+                    units, stream);
+    default:
+      return launch(gated_kernel<KIND, 64>, Layout<KIND, 64>::kBytes, Layout<KIND, 64>::kThreads, once[2], maps, p,
+                    units, stream);
   }
 }
 
@@ -694,36 +738,49 @@ constexpr int kSms = 148;
 
 // Accumulator columns: the widest tile that still gives every SM one (a
 // narrow tile reads A more often but spreads a small product over the SMs).
-int pick_nacc(int64_t m_tiles, int64_t cols, int per_col) {
-  for (int nacc = 256; nacc > 64; nacc /= 2) {
-    if (m_tiles * ceil_div(cols * per_col, nacc) >= kSms) return nacc;
-  }
+int pick_nacc(int64_t m, int64_t cols) {
+  if (ceil_div(m, 2 * kBM) * ceil_div(cols, 256) >= kSms / 2) return 256;
+  if (ceil_div(m, kBM) * ceil_div(cols, 128) >= kSms) return 128;
   return 64;
 }
 
+struct Tiles {
+  int nacc, n_tiles, units, units_per_n;  // units: CTAs or pairs; slots: CTAs that share a column block
+  int slots() const { return units_per_n * (nacc == 256 ? 2 : 1); }
+};
+
+// A product with m rows and `cols` accumulator columns, column blocks fixed per unit.
+Tiles plan_rows(int64_t m, int64_t cols) {
+  Tiles t;
+  t.nacc = pick_nacc(m, cols);
+  const int group = t.nacc == 256 ? 2 : 1;
+  t.n_tiles = static_cast<int>(ceil_div(cols, t.nacc));
+  t.units_per_n = static_cast<int>(
+      std::max<int64_t>(1, std::min<int64_t>(ceil_div(m, kBM * group), kSms / group / t.n_tiles)));
+  t.units = t.n_tiles * t.units_per_n;
+  return t;
+}
+
 struct Plan {
-  int64_t m_tiles;
-  int nacc_gate, tiles_gate, ctas_gate;      // kForward, kGates
-  int nacc_input, tiles_input, ctas_input;   // kInput
-  int nacc_weight, tiles_weight, splits, kb_split, cb1;
+  Tiles gate, input, weight;
+  int splits, kb_split, cb1;
 };
 
 Plan make_plan(int64_t m, int64_t k1, int64_t k2, int64_t n) {
   Plan pl{};
-  pl.m_tiles = ceil_div(m, kBM);
-  pl.nacc_gate = pick_nacc(pl.m_tiles, n, 2);
-  pl.tiles_gate = static_cast<int>(ceil_div(2 * n, pl.nacc_gate));
-  pl.ctas_gate = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(pl.m_tiles, kSms / pl.tiles_gate)));
-  pl.nacc_input = pick_nacc(pl.m_tiles, k1 + k2, 1);
-  pl.tiles_input = static_cast<int>(ceil_div(k1 + k2, pl.nacc_input));
-  pl.ctas_input = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(pl.m_tiles, kSms / pl.tiles_input)));
-  const int64_t row_blocks = 2 * ceil_div(n, kBM), kb = ceil_div(m, kBK);
-  pl.nacc_weight = std::max(k1, k2) > 128 ? 256 : (std::max(k1, k2) > 64 ? 128 : 64);
-  pl.cb1 = static_cast<int>(ceil_div(k1, pl.nacc_weight));
-  pl.tiles_weight = static_cast<int>(row_blocks * (pl.cb1 + ceil_div(k2, pl.nacc_weight)));
-  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(kb, kSms / pl.tiles_weight));
-  pl.kb_split = static_cast<int>(ceil_div(std::max<int64_t>(kb, 1), want));
-  pl.splits = static_cast<int>(ceil_div(std::max<int64_t>(kb, 1), pl.kb_split));
+  // Column blocks of the gate product hold half gate, half up columns.
+  pl.gate = plan_rows(m, 2 * n);
+  pl.input = plan_rows(m, k1 + k2);
+  const int64_t widest = std::max(k1, k2), kb = std::max<int64_t>(ceil_div(m, kBK), 1);
+  pl.weight.nacc = widest > 128 && 2 * n >= 256 ? 256 : (widest > 64 ? 128 : 64);
+  const int group = pl.weight.nacc == 256 ? 2 : 1;
+  pl.cb1 = static_cast<int>(ceil_div(k1, pl.weight.nacc));
+  pl.weight.n_tiles = static_cast<int>(ceil_div(2 * n, kBM * group) * (pl.cb1 + ceil_div(k2, pl.weight.nacc)));
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(kb, kSms / group / pl.weight.n_tiles));
+  pl.kb_split = static_cast<int>(ceil_div(kb, want));
+  pl.splits = static_cast<int>(ceil_div(kb, pl.kb_split));
+  pl.weight.units = pl.weight.n_tiles * pl.splits;
+  pl.weight.units_per_n = pl.splits;
   return pl;
 }
 
@@ -739,7 +796,7 @@ Work carve(void* base, size_t cap, const Plan& pl, int64_t m, int64_t kk, int64_
   Work w;
   w.d = arena.take<__nv_bfloat16>(static_cast<size_t>(m) * 2 * n);
   w.tiles = arena.take<float>(static_cast<size_t>(pl.splits) * 2 * n * kk);
-  w.sums = arena.take<float>(static_cast<size_t>(pl.ctas_gate) * 4 * 2 * n);
+  w.sums = arena.take<float>(static_cast<size_t>(pl.gate.slots()) * 4 * 2 * n);
   w.ok = arena.ok();
   w.bytes = arena.used;
   return w;
@@ -796,7 +853,7 @@ extern "C" int dgfx_gated_dense_concat_bf16(const void* d_x1, int64_t k1, const 
   if (err == nullptr) return fail(DGFX_ERR_CUDA, "dgfx_gated_dense_concat_bf16: status word unavailable");
   const Plan pl = make_plan(m, k1, k2, n);
   Maps maps{};
-  DGFX_TRY(gate_maps(&maps, d_x1, k1, d_x2, k2, m, d_w_gate, d_w_up, n, pl.nacc_gate));
+  DGFX_TRY(gate_maps(&maps, d_x1, k1, d_x2, k2, m, d_w_gate, d_w_up, n, pl.gate.nacc));
   Args p{};
   p.m = m;
   p.n = static_cast<int32_t>(n);
@@ -804,14 +861,14 @@ extern "C" int dgfx_gated_dense_concat_bf16(const void* d_x1, int64_t k1, const 
   p.k2 = static_cast<int32_t>(k2);
   p.kb1 = static_cast<int32_t>(ceil_div(k1, kBK));
   p.kb_total = p.kb1 + static_cast<int32_t>(ceil_div(k2, kBK));
-  p.n_tiles = pl.tiles_gate;
-  p.ctas_per_n = pl.ctas_gate;
+  p.n_tiles = pl.gate.n_tiles;
+  p.units_per_n = pl.gate.units_per_n;
   p.act = activation;
   p.b_gate = d_b_gate;
   p.b_up = d_b_up;
   p.out = static_cast<__nv_bfloat16*>(d_h);
   p.err = err;
-  return launch_nacc<kForward>(pl.nacc_gate, maps, p, pl.tiles_gate * pl.ctas_gate, stream);
+  return launch_nacc<kForward>(pl.gate.nacc, maps, p, pl.gate.units, stream);
 }
 
 extern "C" int dgfx_gated_dense_concat_backward_workspace_size(int64_t k1, int64_t k2, int64_t m, int64_t n,
@@ -866,19 +923,19 @@ extern "C" int dgfx_gated_dense_concat_backward_bf16(const void* d_dh, const voi
   p.err = err;
   {  // D = [dg | du] and the bias sums
     Maps maps{};
-    DGFX_TRY(gate_maps(&maps, d_x1, k1, d_x2, k2, m, d_w_gate, d_w_up, n, pl.nacc_gate));
+    DGFX_TRY(gate_maps(&maps, d_x1, k1, d_x2, k2, m, d_w_gate, d_w_up, n, pl.gate.nacc));
     Args a = p;
     a.kb1 = static_cast<int32_t>(ceil_div(k1, kBK));
     a.kb_total = a.kb1 + static_cast<int32_t>(ceil_div(k2, kBK));
-    a.n_tiles = pl.tiles_gate;
-    a.ctas_per_n = pl.ctas_gate;
+    a.n_tiles = pl.gate.n_tiles;
+    a.units_per_n = pl.gate.units_per_n;
     a.act = activation;
     a.b_gate = d_b_gate;
     a.b_up = d_b_up;
     a.dh = static_cast<const __nv_bfloat16*>(d_dh);
     a.out = ws.d;
     a.partial = ws.sums;
-    DGFX_TRY(launch_nacc<kGates>(pl.nacc_gate, maps, a, pl.tiles_gate * pl.ctas_gate, stream));
+    DGFX_TRY(launch_nacc<kGates>(pl.gate.nacc, maps, a, pl.gate.units, stream));
   }
   if (d_dx1 != nullptr || d_dx2 != nullptr) {
     Maps maps{};
@@ -889,11 +946,11 @@ extern "C" int dgfx_gated_dense_concat_backward_bf16(const void* d_dh, const voi
     Args a = p;
     a.kb1 = static_cast<int32_t>(ceil_div(n, kBK));
     a.kb_total = 2 * a.kb1;
-    a.n_tiles = pl.tiles_input;
-    a.ctas_per_n = pl.ctas_input;
+    a.n_tiles = pl.input.n_tiles;
+    a.units_per_n = pl.input.units_per_n;
     a.out = static_cast<__nv_bfloat16*>(d_dx1);
     a.out2 = static_cast<__nv_bfloat16*>(d_dx2);
-    DGFX_TRY(launch_nacc<kInput>(pl.nacc_input, maps, a, pl.tiles_input * pl.ctas_input, stream));
+    DGFX_TRY(launch_nacc<kInput>(pl.input.nacc, maps, a, pl.input.units, stream));
   }
   if (d_dw_gate != nullptr) {
     Maps maps{};
@@ -903,17 +960,17 @@ extern "C" int dgfx_gated_dense_concat_backward_bf16(const void* d_dh, const voi
     Args a = p;
     a.kb_total = static_cast<int32_t>(ceil_div(m, kBK));
     a.kb_split = pl.kb_split;
-    a.n_tiles = pl.tiles_weight;
+    a.n_tiles = pl.weight.n_tiles;
     a.cb1 = pl.cb1;
     a.partial = ws.tiles;
-    DGFX_TRY(launch_nacc<kWeights>(pl.nacc_weight, maps, a, pl.tiles_weight * pl.splits, stream));
+    DGFX_TRY(launch_nacc<kWeights>(pl.weight.nacc, maps, a, pl.weight.units, stream));
   }
   if (d_dw_gate != nullptr || d_db_gate != nullptr || d_db_up != nullptr) {
     const int64_t bias_blocks = d_db_gate != nullptr || d_db_up != nullptr ? ceil_div(2 * n, 32) : 0;
     const int64_t weight_blocks = d_dw_gate != nullptr ? std::min<int64_t>(ceil_div(2 * n * kk / 4, 256), kSms * 8) : 0;
     gated_finish_kernel<<<static_cast<unsigned>(bias_blocks + weight_blocks), 256, 0, stream>>>(
         ws.tiles, pl.splits, n, kk, static_cast<uint2*>(d_dw_gate), static_cast<uint2*>(d_dw_up), ws.sums,
-        pl.ctas_gate * 4, static_cast<int32_t>(bias_blocks), d_db_gate, d_db_up);
+        pl.gate.slots() * 4, static_cast<int32_t>(bias_blocks), d_db_gate, d_db_up);
     DGFX_CUDA_TRY(cudaGetLastError());
   }
   return DGFX_OK;
