@@ -118,37 +118,44 @@ __device__ __forceinline__ uint32_t piece_at(int r, int j) {
 
 // act(g) * u, or the pair (dg, du), for 16 columns of one row.
 template <int ACT>
-__device__ __forceinline__ void gate_forward(float (&g)[16], const float (&u)[16]) {
+__device__ __forceinline__ void gate_forward(float2 (&g)[8], const float2 (&u)[8]) {
 #pragma unroll
-  for (int j = 0; j < 16; ++j) g[j] = act_f<ACT>(g[j]) * u[j];
+  for (int j = 0; j < 8; ++j) g[j] = mul2(act2_f<ACT>(g[j]), u[j]);
 }
 
 template <int ACT>
-__device__ __forceinline__ void gate_backward(float (&g)[16], float (&u)[16], const float (&d)[16]) {
+__device__ __forceinline__ void gate_backward(float2 (&g)[8], float2 (&u)[8], const float2 (&d)[8]) {
 #pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    float v, s;
-    act_both_f<ACT>(g[j], &v, &s);
-    const float uj = u[j];
-    u[j] = d[j] * v;
-    g[j] = d[j] * uj * s;
+  for (int j = 0; j < 8; ++j) {
+    float2 v, s;
+    act2_both_f<ACT>(g[j], &v, &s);
+    g[j] = mul2(mul2(d[j], u[j]), s);
+    u[j] = mul2(d[j], v);
   }
 }
 
-// Sums 32 values over the 32 lanes: lane l returns the total of v[l].
-__device__ __forceinline__ float transpose_sum(float (&v)[32]) {
+// Sums 32 values (16 pairs) over the 32 lanes: lane l returns the total of
+// value l.
+__device__ __forceinline__ float transpose_sum(float2 (&v)[16]) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const bool upper = (lane & o) != 0;
+  for (int o = 8; o > 0; o >>= 1) {
+    const bool upper = (lane & (2 * o)) != 0;
 #pragma unroll
     for (int i = 0; i < o; ++i) {
-      const float send = upper ? v[i] : v[i + o];
-      const float keep = upper ? v[i + o] : v[i];
-      v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+      const float2 send = upper ? v[i] : v[i + o], keep = upper ? v[i + o] : v[i];
+      v[i] = add2(keep, make_float2(__shfl_xor_sync(0xffffffffu, send.x, 2 * o),
+                                    __shfl_xor_sync(0xffffffffu, send.y, 2 * o)));
     }
   }
-  return v[0];
+  const bool odd = (lane & 1) != 0;
+  const float send = odd ? v[0].x : v[0].y, keep = odd ? v[0].y : v[0].x;
+  return keep + __shfl_xor_sync(0xffffffffu, send, 1);
+}
+
+__device__ __forceinline__ uint4 pack8(const float2* f) {
+  return make_uint4(pack_bf16(f[0].x, f[0].y), pack_bf16(f[1].x, f[1].y), pack_bf16(f[2].x, f[2].y),
+                    pack_bf16(f[3].x, f[3].y));
 }
 
 // The tiles of one CTA or pair (`unit`). Kinds with a fixed column block per
@@ -245,16 +252,42 @@ __device__ __forceinline__ void load_stage(const Maps& maps, const Args& p, cons
 // Writes a warp's staged 32 rows x P pieces of bf16 to rows row0.. of `out`
 // ([m, pitch], this block of columns starting at col0, `limit` columns left).
 template <int P>
-__device__ __forceinline__ void store_bf16(const uint8_t* stage, __nv_bfloat16* out, int64_t pitch, int64_t row0,
+__device__ __forceinline__ void store_bf16(const uint8_t* stage, __nv_bfloat16* out, int32_t pitch, int64_t row0,
                                            int64_t m, int32_t col0, int32_t limit) {
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, r0 = lane / P, j = lane % P;
+  __nv_bfloat16* to = out + row0 * pitch + col0 + r0 * pitch + j * 8;
+  if (row0 + 32 <= m && P * 8 <= limit) {
 #pragma unroll
-  for (int k = 0; k < P; ++k) {
-    const int i = lane + 32 * k, r = i / P, j = i % P;
-    if (row0 + r < m && j * 8 < limit) {
-      *reinterpret_cast<uint4*>(out + (row0 + r) * pitch + col0 + j * 8) =
-          *reinterpret_cast<const uint4*>(stage + piece_at<P>(r, j));
+    for (int k = 0; k < P; ++k) {
+      *reinterpret_cast<uint4*>(to + k * (32 / P) * pitch) =
+          *reinterpret_cast<const uint4*>(stage + piece_at<P>(r0 + k * (32 / P), j));
     }
+  } else if (j * 8 < limit) {
+#pragma unroll
+    for (int k = 0; k < P; ++k) {
+      if (row0 + r0 + k * (32 / P) < m) {
+        *reinterpret_cast<uint4*>(to + k * (32 / P) * pitch) =
+            *reinterpret_cast<const uint4*>(stage + piece_at<P>(r0 + k * (32 / P), j));
+      }
+    }
+  }
+}
+
+// g and u of 16 columns from the accumulators, biases added (16-byte reads,
+// the same for every lane).
+__device__ __forceinline__ void load_gates(uint32_t acc_g, uint32_t acc_u, const float* bias_g, const float* bias_u,
+                                           float2 (&g)[8], float2 (&u)[8]) {
+  uint32_t gr[16], ur[16];
+  tmem_ld_2x16(acc_g, acc_u, gr, ur);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float4 bg = reinterpret_cast<const float4*>(bias_g)[j], bu = reinterpret_cast<const float4*>(bias_u)[j];
+    g[2 * j] = add2(make_float2(__uint_as_float(gr[4 * j]), __uint_as_float(gr[4 * j + 1])), make_float2(bg.x, bg.y));
+    g[2 * j + 1] =
+        add2(make_float2(__uint_as_float(gr[4 * j + 2]), __uint_as_float(gr[4 * j + 3])), make_float2(bg.z, bg.w));
+    u[2 * j] = add2(make_float2(__uint_as_float(ur[4 * j]), __uint_as_float(ur[4 * j + 1])), make_float2(bu.x, bu.y));
+    u[2 * j + 1] =
+        add2(make_float2(__uint_as_float(ur[4 * j + 2]), __uint_as_float(ur[4 * j + 3])), make_float2(bu.z, bu.w));
   }
 }
 
@@ -464,14 +497,8 @@ __device__ __forceinline__ void gated_body(const Maps& maps, const Args& p) {
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
           const int lc = part * GC + c * 16;
-          uint32_t gr[16], ur[16];
-          tmem_ld_2x16(acc + lc, acc + BN + lc, gr, ur);
-          float g[16], u[16];
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            g[j] = __uint_as_float(gr[j]) + biases[lc + j];
-            u[j] = __uint_as_float(ur[j]) + biases[BN + lc + j];
-          }
+          float2 g[8], u[8];
+          load_gates(acc + lc, acc + BN + lc, biases + lc, biases + BN + lc, g, u);
           switch (p.act) {
             case DGFX_ACT_RELU: gate_forward<DGFX_ACT_RELU>(g, u); break;
             case DGFX_ACT_SILU: gate_forward<DGFX_ACT_SILU>(g, u); break;
@@ -481,9 +508,7 @@ __device__ __forceinline__ void gated_body(const Maps& maps, const Args& p) {
           }
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            *reinterpret_cast<uint4*>(stage + piece_at<GP>(lane, c * 2 + j)) =
-                make_uint4(pack_bf16(g[8 * j], g[8 * j + 1]), pack_bf16(g[8 * j + 2], g[8 * j + 3]),
-                           pack_bf16(g[8 * j + 4], g[8 * j + 5]), pack_bf16(g[8 * j + 6], g[8 * j + 7]));
+            *reinterpret_cast<uint4*>(stage + piece_at<GP>(lane, c * 2 + j)) = pack8(g + 4 * j);
           }
         }
         release(b);
@@ -500,20 +525,14 @@ __device__ __forceinline__ void gated_body(const Maps& maps, const Args& p) {
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
           const int lc = part * GC + c * 16;
-          uint32_t gr[16], ur[16];
-          tmem_ld_2x16(acc + lc, acc + BN + lc, gr, ur);
-          float g[16], u[16], d[16];
+          float2 g[8], u[8], d[8];
+          load_gates(acc + lc, acc + BN + lc, biases + lc, biases + BN + lc, g, u);
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             float f[8];
             Vec16<__nv_bfloat16>::unpack(*reinterpret_cast<const uint4*>(stage + piece_at<GP>(lane, c * 2 + j)), f);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) d[8 * j + i] = f[i];
-          }
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            g[j] = __uint_as_float(gr[j]) + biases[lc + j];
-            u[j] = __uint_as_float(ur[j]) + biases[BN + lc + j];
+            for (int i = 0; i < 4; ++i) d[4 * j + i] = make_float2(f[2 * i], f[2 * i + 1]);
           }
           switch (p.act) {
             case DGFX_ACT_RELU: gate_backward<DGFX_ACT_RELU>(g, u, d); break;
@@ -524,24 +543,24 @@ __device__ __forceinline__ void gated_body(const Maps& maps, const Args& p) {
           }
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            *reinterpret_cast<uint4*>(stage + piece_at<GP>(lane, c * 2 + j)) =
-                make_uint4(pack_bf16(g[8 * j], g[8 * j + 1]), pack_bf16(g[8 * j + 2], g[8 * j + 3]),
-                           pack_bf16(g[8 * j + 4], g[8 * j + 5]), pack_bf16(g[8 * j + 6], g[8 * j + 7]));
-            *reinterpret_cast<uint4*>(stage2 + piece_at<GP>(lane, c * 2 + j)) =
-                make_uint4(pack_bf16(u[8 * j], u[8 * j + 1]), pack_bf16(u[8 * j + 2], u[8 * j + 3]),
-                           pack_bf16(u[8 * j + 4], u[8 * j + 5]), pack_bf16(u[8 * j + 6], u[8 * j + 7]));
+            *reinterpret_cast<uint4*>(stage + piece_at<GP>(lane, c * 2 + j)) = pack8(g + 4 * j);
+            *reinterpret_cast<uint4*>(stage2 + piece_at<GP>(lane, c * 2 + j)) = pack8(u + 4 * j);
           }
-          float v[32];
+          float2 v[16];
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            v[j] = row_ok ? g[j] : 0.0f;
-            v[16 + j] = row_ok ? u[j] : 0.0f;
+          for (int j = 0; j < 8; ++j) {
+            v[j] = g[j];
+            v[8 + j] = u[j];
+          }
+          if (row0 + 32 > p.m) {  // the last rows: nothing from behind the end
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = row_ok ? v[j] : make_float2(0.0f, 0.0f);
           }
           bias_sum[c] += transpose_sum(v);
         }
         release(b);
-        store_bf16<GP>(stage, p.out, 2 * static_cast<int64_t>(p.n), row0, p.m, gcol0, p.n - gcol0);
-        store_bf16<GP>(stage2, p.out + p.n, 2 * static_cast<int64_t>(p.n), row0, p.m, gcol0, p.n - gcol0);
+        store_bf16<GP>(stage, p.out, 2 * p.n, row0, p.m, gcol0, p.n - gcol0);
+        store_bf16<GP>(stage2, p.out + p.n, 2 * p.n, row0, p.m, gcol0, p.n - gcol0);
         __syncwarp();
       } else if (KIND == kInput) {
         const int32_t kk = p.k1 + p.k2;

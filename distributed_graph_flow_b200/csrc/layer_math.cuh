@@ -25,6 +25,32 @@ __device__ __forceinline__ float rcp_f(float x) {
 // 1 / (1 + e^-z) without overflow at either end: e^-z = inf gives 0.
 __device__ __forceinline__ float sigmoid_f(float z) { return rcp_f(1.0f + exp_f(-z)); }
 
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 z, x, y;\n\t"
+      "mov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\t"
+      "mov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 w, {%6, %7};\n\t"
+      "fma.rn.f32x2 z, x, y, w;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+
 // Activations (DGFX_ACT_*) and their derivatives in fp32. gelu is the exact
 // form z Phi(z) = z (1 + erf(z / sqrt 2)) / 2. relu'(0) = 0. relu compares
 // instead of taking a maximum, so that NaN passes through.
@@ -58,6 +84,40 @@ __device__ __forceinline__ void act_both_f(float z, float* value, float* slope) 
   } else {
     *value = z;
     *slope = 1.0f;
+  }
+}
+
+// The same for two values at once.
+__device__ __forceinline__ float2 sigmoid2(float2 z) {
+  const float2 t = mul2(z, make_float2(-1.4426950408889634f, -1.4426950408889634f));
+  float2 e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
+  e = add2(e, make_float2(1.0f, 1.0f));
+  return make_float2(rcp_f(e.x), rcp_f(e.y));
+}
+
+template <int ACT>
+__device__ __forceinline__ float2 act2_f(float2 z) {
+  if (ACT == DGFX_ACT_SILU) return mul2(z, sigmoid2(z));
+  if (ACT == DGFX_ACT_SIGMOID) return sigmoid2(z);
+  return make_float2(act_f<ACT>(z.x), act_f<ACT>(z.y));
+}
+
+template <int ACT>
+__device__ __forceinline__ void act2_both_f(float2 z, float2* value, float2* slope) {
+  const float2 one = make_float2(1.0f, 1.0f), minus = make_float2(-1.0f, -1.0f);
+  if (ACT == DGFX_ACT_SILU) {
+    const float2 s = sigmoid2(z);
+    *value = mul2(z, s);
+    *slope = mul2(s, fma2(z, fma2(s, minus, one), one));
+  } else if (ACT == DGFX_ACT_SIGMOID) {
+    const float2 s = sigmoid2(z);
+    *value = s;
+    *slope = mul2(s, fma2(s, minus, one));
+  } else {
+    act_both_f<ACT>(z.x, &value->x, &slope->x);
+    act_both_f<ACT>(z.y, &value->y, &slope->y);
   }
 }
 

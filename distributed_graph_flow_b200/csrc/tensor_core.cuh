@@ -145,8 +145,12 @@ __device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
   return r;
 }
 
+// Arrives at a barrier of either CTA. Relaxed: it orders no memory (a release
+// at cluster scope would wait for this thread's stores to global memory);
+// what it announces is the end of tensor-memory reads, ordered by the
+// tcgen05 fence before it.
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 // Loads into this CTA's shared memory, reported to `bar` in either CTA of the pair.
