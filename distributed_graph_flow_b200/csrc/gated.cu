@@ -69,19 +69,23 @@ struct Args {
   unsigned int* err;
 };
 
-// Per CTA. NACC accumulator columns; 256 of them on a pair of CTAs.
-template <int KIND, int NACC>
+// Per CTA. NACC accumulator columns; 256 of them on a pair of CTAs. RES: the
+// weights of a CTA's column block stay in shared memory (up to kResident
+// K-blocks), and only A rows come by the ring.
+constexpr int kResident = 8;
+template <int KIND, int NACC, bool RES>
 struct Layout {
   static constexpr int kGroup = NACC == 256 ? 2 : 1;            // CTAs that share a tile
   static constexpr int kEpilogueWarps = NACC == 256 ? 16 : 8;
   static constexpr int kThreads = 64 + 32 * kEpilogueWarps;
   static constexpr uint32_t kA = kBM * kBK * 2;
   static constexpr uint32_t kB = NACC / kGroup * kBK * 2;
-  static constexpr uint32_t kStage = kA + kB;
-  static constexpr uint32_t kOutWarp = KIND == kGates ? 4096 : 2048;  // staging bytes per epilogue warp
-  static constexpr int kStages = NACC != 256 ? 4 : (KIND == kGates ? 5 : 6);
+  static constexpr uint32_t kStage = RES ? kA : kA + kB;
+  static constexpr uint32_t kHeld = RES ? kResident * kB : 0;
+  static constexpr uint32_t kOutWarp = 2048;  // staging bytes per epilogue warp
+  static constexpr int kStages = RES || NACC != 256 ? 4 : 6;
   static constexpr uint32_t kTmemCols = 2 * NACC;
-  static constexpr size_t kBytes = static_cast<size_t>(kStages) * kStage + kEpilogueWarps * kOutWarp +
+  static constexpr size_t kBytes = static_cast<size_t>(kStages) * kStage + kHeld + kEpilogueWarps * kOutWarp +
                                    NACC * sizeof(float) /* biases */ + 1024 /* align */ + 256 /* barriers */;
   static_assert(kBytes <= 232448, "shared memory of a CTA");
 };
@@ -209,24 +213,24 @@ __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, u
   else tma_load_2d(dst, map, bar, x, y);
 }
 
-template <int KIND, int NACC>
-__device__ __forceinline__ void load_stage(const Maps& maps, const Args& p, const Walk<KIND, Layout<KIND, NACC>::kGroup>& w,
-                                           int32_t mb, int32_t kb, uint32_t a_dst, uint32_t bar) {
-  using L = Layout<KIND, NACC>;
-  constexpr int G = L::kGroup;
-  const uint32_t b_dst = a_dst + L::kA;
+// Operand tiles of one K-block: A to a_dst, B to b_dst (either may be left out).
+template <int KIND, int NACC, bool DO_A, bool DO_B, int G>
+__device__ __forceinline__ void load_stage(const Maps& maps, const Args& p, const Walk<KIND, G>& w, int32_t mb, int32_t kb,
+                                           uint32_t a_dst, uint32_t b_dst, uint32_t bar) {
   if (KIND == kForward || KIND == kGates) {
     constexpr int BN = NACC / 2;
     const bool first = kb < p.kb1;
     const int32_t x = (first ? kb : kb - p.kb1) * kBK;
-    load_box<G>(a_dst, first ? &maps.a1 : &maps.a2, bar, x, w.row(mb));
-    const CUtensorMap* gate = first ? &maps.b1 : &maps.b2;
-    const CUtensorMap* up = first ? &maps.b3 : &maps.b4;
-    if (G == 2) {
-      load_box<G>(b_dst, w.rank == 0 ? gate : up, bar, x, w.nb * BN);
-    } else {
-      load_box<G>(b_dst, gate, bar, x, w.nb * BN);
-      load_box<G>(b_dst + BN * kBK * 2, up, bar, x, w.nb * BN);
+    if (DO_A) load_box<G>(a_dst, first ? &maps.a1 : &maps.a2, bar, x, w.row(mb));
+    if (DO_B) {
+      const CUtensorMap* gate = first ? &maps.b1 : &maps.b2;
+      const CUtensorMap* up = first ? &maps.b3 : &maps.b4;
+      if (G == 2) {
+        load_box<G>(b_dst, w.rank == 0 ? gate : up, bar, x, w.nb * BN);
+      } else {
+        load_box<G>(b_dst, gate, bar, x, w.nb * BN);
+        load_box<G>(b_dst + BN * kBK * 2, up, bar, x, w.nb * BN);
+      }
     }
   } else if (KIND == kInput) {
     const bool first = kb < p.kb1;
@@ -291,23 +295,24 @@ __device__ __forceinline__ void load_gates(uint32_t acc_g, uint32_t acc_u, const
   }
 }
 
-template <int KIND, int NACC>
+template <int KIND, int NACC, bool RES>
 __device__ __forceinline__ void gated_body(const Maps& maps, const Args& p) {
-  using L = Layout<KIND, NACC>;
+  using L = Layout<KIND, NACC, RES>;
   constexpr int G = L::kGroup, BN = NACC / 2, S = L::kStages;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   // 128-byte swizzled tiles need 1024-byte aligned shared addresses (the same
   // offset in both CTAs of a pair).
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  uint8_t* out_stage = smem + S * L::kStage;
+  uint8_t* held = smem + S * L::kStage;
+  uint8_t* out_stage = held + L::kHeld;
   float* biases = reinterpret_cast<float*>(out_stage + L::kEpilogueWarps * L::kOutWarp);
   uint64_t* bars = reinterpret_cast<uint64_t*>(biases + NACC);
-  // bars: full[S], empty[S], acc_full[2], acc_empty[2], drain
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S + 5);
+  // bars: full[S], empty[S], acc_full[2], acc_empty[2], drain, held
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S + 6);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + S);
   const uint32_t accf0 = smem_u32(bars + 2 * S), acce0 = smem_u32(bars + 2 * S + 2);
-  const uint32_t drain = smem_u32(bars + 2 * S + 4);
+  const uint32_t drain = smem_u32(bars + 2 * S + 4), held_bar = smem_u32(bars + 2 * S + 5);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Walk<KIND, G> w(p);
 
@@ -321,6 +326,7 @@ __device__ __forceinline__ void gated_body(const Maps& maps, const Args& p) {
       mbar_init(acce0 + 8 * b, G * L::kEpilogueWarps);
     }
     mbar_init(drain, 1);
+    mbar_init(held_bar, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -359,6 +365,13 @@ __device__ __forceinline__ void gated_body(const Maps& maps, const Args& p) {
       uint32_t ph = 0;
       uint32_t issued = 0;  // stages with a load issued in the current ring pass
       bool ok = true;
+      if (RES) {  // the weights of this column block, once
+        if (w.rank == 0) mbar_arrive_expect_tx(held_bar, G * L::kB * static_cast<uint32_t>(w.kb_end));
+        const uint32_t report = G == 2 ? map_rank(held_bar, 0) : held_bar;
+        for (int32_t kb = 0; kb < w.kb_end; ++kb) {
+          load_stage<KIND, NACC, false, true, G>(maps, p, w, 0, kb, 0u, smem_u32(held + kb * L::kB), report);
+        }
+      }
       for (int32_t mb = w.mb; mb < w.m_tiles && ok; mb += w.step) {
         for (int32_t kb = w.kb_begin; kb < w.kb_end; ++kb) {
           if (!mbar_wait(empty0 + 8 * s, ph ^ 1u, abort_flag, p.err)) {
@@ -366,7 +379,8 @@ __device__ __forceinline__ void gated_body(const Maps& maps, const Args& p) {
             break;
           }
           if (w.rank == 0) mbar_arrive_expect_tx(full0 + 8 * s, G * L::kStage);
-          load_stage<KIND, NACC>(maps, p, w, mb, kb, smem_u32(smem + s * L::kStage), report0 + 8 * s);
+          const uint32_t a_dst = smem_u32(smem + s * L::kStage);
+          load_stage<KIND, NACC, true, !RES, G>(maps, p, w, mb, kb, a_dst, a_dst + L::kA, report0 + 8 * s);
           issued |= 1u << s;
           if (++s == S) {
             s = 0;
@@ -386,6 +400,10 @@ __device__ __forceinline__ void gated_body(const Maps& maps, const Args& p) {
             while (!mbar_test(full0 + 8 * j, ph) && now_ns() - t0 < kWaitNs) __nanosleep(100);
           }
         }
+        if (RES && w.rank == 0) {
+          const uint64_t t0 = now_ns();
+          while (!mbar_test(held_bar, 0) && now_ns() - t0 < kWaitNs) __nanosleep(100);
+        }
       }
     }
     __syncwarp();
@@ -403,7 +421,7 @@ __device__ __forceinline__ void gated_body(const Maps& maps, const Args& p) {
       uint32_t ph = 0;
       int b = 0;
       uint32_t aph = 0;
-      bool ok = true;
+      bool ok = !RES || mbar_wait(held_bar, 0, abort_flag, p.err);
       bool any = false;
       for (int32_t mb = w.mb; mb < w.m_tiles && ok; mb += w.step) {
         if (!mbar_wait(acce0 + 8 * b, aph ^ 1u, abort_flag, p.err)) break;
@@ -417,7 +435,8 @@ __device__ __forceinline__ void gated_body(const Maps& maps, const Args& p) {
           tc_fence_after();
           const uint32_t a_addr = smem_u32(smem + s * L::kStage);
           const uint64_t adesc = kAMn ? smem_desc_sw128_mn(a_addr) : smem_desc_sw128(a_addr);
-          const uint64_t bdesc = kBMn ? smem_desc_sw128_mn(a_addr + L::kA) : smem_desc_sw128(a_addr + L::kA);
+          const uint32_t b_addr = RES ? smem_u32(held) + static_cast<uint32_t>(kb) * L::kB : a_addr + L::kA;
+          const uint64_t bdesc = kBMn ? smem_desc_sw128_mn(b_addr) : smem_desc_sw128(b_addr);
 #pragma unroll
           for (int k = 0; k < kBK / 16; ++k) {
             const uint32_t accumulate = (kb != w.kb_begin || k != 0) ? 1u : 0u;
@@ -515,7 +534,7 @@ __device__ __forceinline__ void gated_body(const Maps& maps, const Args& p) {
         store_bf16<GP>(stage, p.out, p.n, row0, p.m, gcol0, p.n - gcol0);
         __syncwarp();
       } else if (KIND == kGates) {
-        uint8_t* stage2 = stage + L::kOutWarp / 2;  // dg goes where dh was, du here
+        uint4 du[GP];  // dg goes where dh was, du after it
 #pragma unroll
         for (int k = 0; k < GP; ++k) {
           const int i = lane + 32 * k;
@@ -544,7 +563,7 @@ __device__ __forceinline__ void gated_body(const Maps& maps, const Args& p) {
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             *reinterpret_cast<uint4*>(stage + piece_at<GP>(lane, c * 2 + j)) = pack8(g + 4 * j);
-            *reinterpret_cast<uint4*>(stage2 + piece_at<GP>(lane, c * 2 + j)) = pack8(u + 4 * j);
+            du[c * 2 + j] = pack8(u + 4 * j);
           }
           float2 v[16];
 #pragma unroll
@@ -560,7 +579,11 @@ __device__ __forceinline__ void gated_body(const Maps& maps, const Args& p) {
         }
         release(b);
         store_bf16<GP>(stage, p.out, 2 * p.n, row0, p.m, gcol0, p.n - gcol0);
-        store_bf16<GP>(stage2, p.out + p.n, 2 * p.n, row0, p.m, gcol0, p.n - gcol0);
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < GP; ++j) *reinterpret_cast<uint4*>(stage + piece_at<GP>(lane, j)) = du[j];
+        __syncwarp();
+        store_bf16<GP>(stage, p.out + p.n, 2 * p.n, row0, p.m, gcol0, p.n - gcol0);
         __syncwarp();
       } else if (KIND == kInput) {
         const int32_t kk = p.k1 + p.k2;
@@ -664,15 +687,15 @@ __device__ __forceinline__ void gated_body(const Maps& maps, const Args& p) {
 }
 
 template <int KIND, int NACC>
-__global__ void __launch_bounds__(Layout<KIND, NACC>::kThreads, 1)
+__global__ void __launch_bounds__(Layout<KIND, NACC, false>::kThreads, 1)
     gated_kernel(const __grid_constant__ Maps maps, const Args p) {
-  gated_body<KIND, NACC>(maps, p);
+  gated_body<KIND, NACC, false>(maps, p);
 }
 
-template <int KIND>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Layout<KIND, 256>::kThreads, 1)
+template <int KIND, bool RES>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Layout<KIND, 256, RES>::kThreads, 1)
     gated_pair_kernel(const __grid_constant__ Maps maps, const Args p) {
-  gated_body<KIND, 256>(maps, p);
+  gated_body<KIND, 256, RES>(maps, p);
 }
 
 // dW from the splits' fp32 tiles and the bias gradients from the CTAs' sums,
@@ -736,21 +759,30 @@ int launch(K kernel, size_t smem, int threads, std::once_flag* once, const Maps&
   return DGFX_OK;
 }
 
+template <int KIND, int NACC>
+int launch_single(const Maps& maps, const Args& p, int units, cudaStream_t stream) {
+  static std::once_flag once[64];
+  using L = Layout<KIND, NACC, false>;
+  return launch(gated_kernel<KIND, NACC>, L::kBytes, L::kThreads, once, maps, p, units, stream);
+}
+
+template <int KIND, bool RES>
+int launch_pairs(const Maps& maps, const Args& p, int units, cudaStream_t stream) {
+  static std::once_flag once[64];
+  using L = Layout<KIND, 256, RES>;
+  return launch(gated_pair_kernel<KIND, RES>, L::kBytes, L::kThreads, once, maps, p, 2 * units, stream);
+}
+
 // `units`: CTAs, or pairs of them at 256 accumulator columns.
 template <int KIND>
 int launch_nacc(int nacc, const Maps& maps, const Args& p, int units, cudaStream_t stream) {
-  static std::once_flag once[3][64];
-  switch (nacc) {
-    case 256:
-      return launch(gated_pair_kernel<KIND>, Layout<KIND, 256>::kBytes, Layout<KIND, 256>::kThreads, once[0], maps, p,
-                    2 * units, stream);
-    case 128:
-      return launch(gated_kernel<KIND, 128>, Layout<KIND, 128>::kBytes, Layout<KIND, 128>::kThreads, once[1], maps, p,
-                    units, stream);
-    default:
-      return launch(gated_kernel<KIND, 64>, Layout<KIND, 64>::kBytes, Layout<KIND, 64>::kThreads, once[2], maps, p,
-                    units, stream);
+  constexpr bool kHolds = KIND == kForward || KIND == kGates;
+  if (nacc == 256) {
+    if (kHolds && p.kb_total <= kResident) return launch_pairs<KIND, kHolds>(maps, p, units, stream);
+    return launch_pairs<KIND, false>(maps, p, units, stream);
   }
+  if (nacc == 128) return launch_single<KIND, 128>(maps, p, units, stream);
+  return launch_single<KIND, 64>(maps, p, units, stream);
 }
 
 constexpr int kSms = 148;

@@ -52,14 +52,26 @@ __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
   return ok != 0;
 }
 
+// The same, but the thread may sleep for a while (a hardware limit) before it
+// is told no: a waiting warp takes no issue slots.
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
 // Waits for the phase of `parity` to complete; false on timeout (latched in
 // *err) or when another role already aborted (the abort word is then set).
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, unsigned int* err) {
-  if (mbar_test(bar, parity)) return true;
+  if (mbar_try(bar, parity)) return true;
   const uint64_t t0 = now_ns();
   for (uint32_t i = 1;; ++i) {
-    if (mbar_test(bar, parity)) return true;
-    if ((i & 255u) == 0) {
+    if (mbar_try(bar, parity)) return true;
+    if ((i & 15u) == 0) {
       if (*abort_flag) return false;
       if (now_ns() - t0 > kWaitNs) {
         *abort_flag = 1;
@@ -67,7 +79,6 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
         return false;
       }
     }
-    if (i > 32) __nanosleep(20);
   }
 }
 
