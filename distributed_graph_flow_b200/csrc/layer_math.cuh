@@ -51,14 +51,34 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   return r;
 }
 
-// Activations (DGFX_ACT_*) and their derivatives in fp32. gelu is the exact
-// form z Phi(z) = z (1 + erf(z / sqrt 2)) / 2. relu'(0) = 0. relu compares
+// Phi(z), the normal distribution function, and e^(-z^2 / 2): with x = |z| /
+// sqrt 2, erfc(x) = P(1 / (1 + p x)) e^(-x^2) (Abramowitz and Stegun, Handbook
+// of Mathematical Functions, 7.1.26, absolute error below 1.5e-7), and
+// Phi(z) = erfc(x) / 2 below zero, one minus that above: no subtraction in
+// the lower tail, and the exponential is the derivative's too.
+__device__ __forceinline__ float normal_cdf_f(float z, float* bell) {
+  const float t = rcp_f(fmaf(fabsf(z), 0.23164189f, 1.0f));
+  float poly = fmaf(t, 0.5307027145f, -0.7265760135f);
+  poly = fmaf(poly, t, 0.7107068705f);
+  poly = fmaf(poly, t, -0.142248368f);
+  poly = fmaf(poly, t, 0.127414796f);
+  const float e = exp_f(-0.5f * z * z);
+  const float tail = poly * t * e;
+  *bell = e;
+  return z < 0.0f ? tail : 1.0f - tail;
+}
+
+// Activations (DGFX_ACT_*) and their derivatives in fp32. gelu is the form
+// z Phi(z) = z (1 + erf(z / sqrt 2)) / 2. relu'(0) = 0. relu compares
 // instead of taking a maximum, so that NaN passes through.
 template <int ACT>
 __device__ __forceinline__ float act_f(float z) {
   if (ACT == DGFX_ACT_RELU) return z < 0.0f ? 0.0f : z;
   if (ACT == DGFX_ACT_SILU) return z * sigmoid_f(z);
-  if (ACT == DGFX_ACT_GELU) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+  if (ACT == DGFX_ACT_GELU) {
+    float bell;
+    return z * normal_cdf_f(z, &bell);
+  }
   if (ACT == DGFX_ACT_SIGMOID) return sigmoid_f(z);
   return z;
 }
@@ -74,9 +94,10 @@ __device__ __forceinline__ void act_both_f(float z, float* value, float* slope) 
     *value = z * s;
     *slope = s * (1.0f + z * (1.0f - s));
   } else if (ACT == DGFX_ACT_GELU) {
-    const float cdf = 0.5f + 0.5f * erff(z * 0.70710678118654752f);
+    float bell;
+    const float cdf = normal_cdf_f(z, &bell);
     *value = z * cdf;
-    *slope = cdf + z * 0.39894228040143268f * exp_f(-0.5f * z * z);
+    *slope = fmaf(z * 0.39894228040143268f, bell, cdf);
   } else if (ACT == DGFX_ACT_SIGMOID) {
     const float s = sigmoid_f(z);
     *value = s;

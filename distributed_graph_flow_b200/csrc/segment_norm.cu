@@ -76,6 +76,34 @@ struct Params {
   float eps;
 };
 
+// A thread's four channels as two pairs.
+struct Pairs {
+  float2 v[2];
+  __device__ Pairs() {}
+  __device__ explicit Pairs(const float (&f)[kCh]) {
+    v[0] = make_float2(f[0], f[1]);
+    v[1] = make_float2(f[2], f[3]);
+  }
+  __device__ void to(float (&f)[kCh]) const {
+    f[0] = v[0].x;
+    f[1] = v[0].y;
+    f[2] = v[1].x;
+    f[3] = v[1].y;
+  }
+};
+
+__device__ __forceinline__ Pairs negated(const float (&f)[kCh]) {
+  const float n[kCh] = {-f[0], -f[1], -f[2], -f[3]};
+  return Pairs(n);
+}
+
+template <class T>
+__device__ __forceinline__ Pairs unpack_pairs(const typename Quad<T>::raw& r) {
+  float f[kCh];
+  Quad<T>::unpack(r, f);
+  return Pairs(f);
+}
+
 struct Place {
   int rl, col, per_pass;
   bool on;
@@ -342,19 +370,25 @@ __device__ __forceinline__ RowStats row_stats(const Params& p, const Share& sh) 
   RowStats s = {};
   if (sh.mine == 0) return s;
   float x0[kCh];
+  Pairs minus;
+  Pairs sum(s.mean), sq(s.m2);
   bool first = true;
   each_row<T>(sh, p.x, [&](const typename Q::raw& v) {
-    float f[kCh];
-    Q::unpack(v, f);
-#pragma unroll
-    for (int c = 0; c < kCh; ++c) {
-      if (first) x0[c] = f[c];
-      const float d = f[c] - x0[c];
-      s.mean[c] += d;
-      s.m2[c] += d * d;
+    const Pairs f = unpack_pairs<T>(v);
+    if (first) {
+      f.to(x0);
+      minus = negated(x0);
+      first = false;
     }
-    first = false;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const float2 d = add2(f.v[c], minus.v[c]);
+      sum.v[c] = add2(sum.v[c], d);
+      sq.v[c] = fma2(d, d, sq.v[c]);
+    }
   });
+  sum.to(s.mean);
+  sq.to(s.m2);
   s.have = static_cast<float>(sh.mine);
   const float inv = 1.0f / s.have;
 #pragma unroll
@@ -376,13 +410,15 @@ __device__ __forceinline__ void apply_rows(const Params& p, const Share& sh, con
   float scale[kCh];
 #pragma unroll
   for (int c = 0; c < kCh; ++c) scale[c] = rs[c] * af.w[c];
+  const Pairs minus = negated(mu), sc(scale), shift(af.b);
   typename Q::raw* y = static_cast<typename Q::raw*>(p.y) + sh.first;
   each_row<T>(sh, p.x, [&](const typename Q::raw& v) {
-    float f[kCh];
-    Q::unpack(v, f);
+    Pairs f = unpack_pairs<T>(v);
 #pragma unroll
-    for (int c = 0; c < kCh; ++c) f[c] = act_f<ACT>(fmaf(f[c] - mu[c], scale[c], af.b[c]));
-    *y = Q::pack(f);
+    for (int c = 0; c < 2; ++c) f.v[c] = act2_f<ACT>(fma2(add2(f.v[c], minus.v[c]), sc.v[c], shift.v[c]));
+    float o[kCh];
+    f.to(o);
+    *y = Q::pack(o);
     y += sh.pitch;
   });
 }
@@ -569,16 +605,16 @@ __global__ void __maxnreg__(64) norm_tile_apply_kernel(Params p) {
 // ---------------------------------------------------------------------------
 // Backward
 // ---------------------------------------------------------------------------
-// xhat and dz. dz and w dz are rounded before any sum or subtraction, the same
-// values in the sums and in dx: a segment of one value then cancels to zero
-// exactly.
+// xhat and dz of a pair. dz and w dz are rounded before any sum or
+// subtraction, the same values in the sums and in dx: a segment of one value
+// then cancels to zero exactly.
 template <int ACT>
-__device__ __forceinline__ void grad_terms(float x, float dy, float mu, float rs, float w, float b, float* xhat,
-                                           float* dz) {
-  *xhat = (x - mu) * rs;
-  float v, slope;
-  act_both_f<ACT>(*xhat * w + b, &v, &slope);
-  *dz = __fmul_rn(dy, slope);
+__device__ __forceinline__ void grad_terms(float2 x, float2 dy, float2 minus_mu, float2 rs, float2 w, float2 b,
+                                           float2* xhat, float2* dz) {
+  *xhat = mul2(add2(x, minus_mu), rs);
+  float2 v, slope;
+  act2_both_f<ACT>(fma2(*xhat, w, b), &v, &slope);
+  *dz = mul2(dy, slope);
 }
 
 // This block's sums for dw and db over its threads, in order, to its slot.
@@ -611,18 +647,20 @@ __device__ __forceinline__ void grad_sums(const Params& p, const Share& sh, cons
                                           const Affine& af, float (&acc)[2][kCh], float (&dwb)[2][kCh]) {
   using Q = Quad<T>;
   float dw[kCh] = {}, db[kCh] = {};  // these rows', so that long sums stay pairwise
+  Pairs sw(dw), sb(db);
+  const Pairs minus = negated(mu), r(rs), w(af.w), b(af.b);
   each_row<T>(sh, p.x, p.dy, [&](const typename Q::raw& v, const typename Q::raw& d) {
-    float f[kCh], g[kCh];
-    Q::unpack(v, f);
-    Q::unpack(d, g);
+    const Pairs f = unpack_pairs<T>(v), g = unpack_pairs<T>(d);
 #pragma unroll
-    for (int c = 0; c < kCh; ++c) {
-      float xh, dz;
-      grad_terms<ACT>(f[c], g[c], mu[c], rs[c], af.w[c], af.b[c], &xh, &dz);
-      dw[c] += dz * xh;
-      db[c] += dz;
+    for (int c = 0; c < 2; ++c) {
+      float2 xh, dz;
+      grad_terms<ACT>(f.v[c], g.v[c], minus.v[c], r.v[c], w.v[c], b.v[c], &xh, &dz);
+      sw.v[c] = fma2(dz, xh, sw.v[c]);
+      sb.v[c] = add2(sb.v[c], dz);
     }
   });
+  sw.to(dw);
+  sb.to(db);
 #pragma unroll
   for (int c = 0; c < kCh; ++c) {
     dwb[0][c] += dw[c];
@@ -638,17 +676,19 @@ __device__ __forceinline__ void grad_rows(const Params& p, const Share& sh, cons
                                           const Affine& af, const float (&s1)[kCh], const float (&s2)[kCh]) {
   using Q = Quad<T>;
   typename Q::raw* dx = static_cast<typename Q::raw*>(p.y) + sh.first;
+  const Pairs minus = negated(mu), r(rs), w(af.w), b(af.b), m1 = negated(s1), m2 = negated(s2);
   each_row<T>(sh, p.x, p.dy, [&](const typename Q::raw& v, const typename Q::raw& d) {
-    float f[kCh], g[kCh];
-    Q::unpack(v, f);
-    Q::unpack(d, g);
+    Pairs f = unpack_pairs<T>(v);
+    const Pairs g = unpack_pairs<T>(d);
 #pragma unroll
-    for (int c = 0; c < kCh; ++c) {
-      float xh, dz;
-      grad_terms<ACT>(f[c], g[c], mu[c], rs[c], af.w[c], af.b[c], &xh, &dz);
-      f[c] = rs[c] * (__fmul_rn(dz, af.w[c]) - s1[c] - xh * s2[c]);
+    for (int c = 0; c < 2; ++c) {
+      float2 xh, dz;
+      grad_terms<ACT>(f.v[c], g.v[c], minus.v[c], r.v[c], w.v[c], b.v[c], &xh, &dz);
+      f.v[c] = mul2(r.v[c], fma2(xh, m2.v[c], add2(mul2(dz, w.v[c]), m1.v[c])));
     }
-    *dx = Q::pack(f);
+    float o[kCh];
+    f.to(o);
+    *dx = Q::pack(o);
     dx += sh.pitch;
   });
 }
