@@ -800,23 +800,23 @@ __global__ void __maxnreg__(80) norm_tile_grad_apply_kernel(Params p) {
   }
 }
 
-// dw and db from the blocks' sums: 32 channels per block, every eighth slot
-// per warp, then the warps' sums in order.
-__global__ void __launch_bounds__(256) norm_params_kernel(const float* __restrict__ partial, int slots, int channels,
+// dw and db from the blocks' sums: 32 channels per block, every 32nd slot per
+// warp, then the warps' sums in order.
+__global__ void __launch_bounds__(1024) norm_params_kernel(const float* __restrict__ partial, int slots, int channels,
                                                           float* __restrict__ dw, float* __restrict__ db) {
-  __shared__ float part[8][32];
+  __shared__ float part[32][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int i = static_cast<int>(blockIdx.x) * 32 + lane;
   float s = 0.0f;
   if (i < 2 * channels) {
 #pragma unroll 8
-    for (int k = warp; k < slots; k += 8) s += __ldg(partial + static_cast<int64_t>(k) * 2 * channels + i);
+    for (int k = warp; k < slots; k += 32) s += __ldg(partial + static_cast<int64_t>(k) * 2 * channels + i);
   }
   part[warp][lane] = s;
   __syncthreads();
   if (warp != 0 || i >= 2 * channels) return;
   s = 0.0f;
-  for (int k = 0; k < 8; ++k) s += part[k][lane];
+  for (int k = 0; k < 32; ++k) s += part[k][lane];
   float* out = i < channels ? dw : db;
   if (out != nullptr) out[i < channels ? i : i - channels] = s;
 }
@@ -870,7 +870,7 @@ int make_plan(const char* who, int64_t rows, int64_t channels, int64_t groups, i
   if (nseg == 0) pl->grid = kSms;
   pl->tile_threads = pl->quads > 256 ? 512 : 256;
   pl->tile_grid = kSms * (backward ? 3 : 4) / (pl->tile_threads / 256);
-  pl->tile_rows = std::max<int64_t>(2 * step_rows(team), ceil_div(rows, kSms * 8));
+  pl->tile_rows = std::max<int64_t>(2 * step_rows(team), ceil_div(rows, 2 * pl->tile_grid));  // two per block
   pl->max_long = rows / (pl->loop_rows + 1) + 1;
   pl->max_tiles = ceil_div(rows, pl->tile_rows) + pl->max_long;
   return DGFX_OK;
@@ -1069,7 +1069,7 @@ extern "C" int dgfx_segment_group_norm_backward(const void* d_dy, const void* d_
   else run<__nv_bfloat16>(activation, true, pl, p, stream);
   DGFX_CUDA_TRY(cudaGetLastError());
   if (d_dweight != nullptr || d_dbias != nullptr) {
-    norm_params_kernel<<<static_cast<unsigned>(ceil_div(2 * channels, 32)), 256, 0, stream>>>(
+    norm_params_kernel<<<static_cast<unsigned>(ceil_div(2 * channels, 32)), 1024, 0, stream>>>(
         w.partial, pl.grid + (pl.longs ? pl.tile_grid : 0), static_cast<int>(channels), d_dweight, d_dbias);
     DGFX_CUDA_TRY(cudaGetLastError());
   }
