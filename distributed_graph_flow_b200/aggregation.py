@@ -182,6 +182,20 @@ def sage_mean_linear_relu(rowptr, col, x, weight, bias=None, agg=None, workspace
     return dense_concat(x[:n_rows], agg, weight, bias, relu=True, out=out, stream=stream)
 
 
+def sage_mean_gated(rowptr, col, x, w_gate, w_up, b_gate=None, b_up=None, activation: str = "silu", agg=None,
+                    workspace=None, out=None, stream=None):
+    """GraphSAGE-mean layer with a gated update: agg = mean over in-neighbours
+    of x (as ``sage_mean_linear_relu``), then act(concat[x, agg] @ w_gate.T +
+    b_gate) * (concat[x, agg] @ w_up.T + b_up) (``gated_dense_concat``). x bf16
+    [N, F], w_gate and w_up bf16 [N_out, 2F]."""
+    torch = _native.require_cuda()
+    n_rows = int(rowptr.numel()) - 1
+    if agg is None:
+        agg = torch.empty((n_rows, int(x.shape[1])), dtype=torch.bfloat16, device=x.device)
+    csr_spmm(rowptr, col, x, normalize=True, out=agg, workspace=workspace, stream=stream)
+    return gated_dense_concat(x[:n_rows], agg, w_gate, w_up, b_gate, b_up, activation, out=out, stream=stream)
+
+
 # ---------------------------------------------------------------------------
 # Propagation matrices of the reference's sparse GNN layers, CSR transpose,
 # segment-sum gradient, mean aggregation over a sampled batch.

@@ -18,6 +18,12 @@ reference's layers need gradients:
   d data[i] = dY[ids[i]] (/ max(count, 1) for the mean), a row gather.
   The two gradients are operators of their own (``dgfx::csr_spmm_grad_x``,
   ``dgfx::segment_sum_grad``), so backward graphs trace with fake tensors.
+* ``dgfx::gated_dense_concat(x1, x2, w_gate, w_up, b_gate, b_up, activation)``,
+  ``dgfx::segment_group_norm(x, offsets, groups, weight, bias, eps,
+  activation)`` and ``dgfx::gated_scan(x, gate, offsets, initial,
+  keep_states)`` — the layer operators around the aggregation, with their
+  gradients (operators too: ``*_grad``). ``gated_scan``, ``segment_group_norm``
+  and ``sage_mean_gated`` below are the calls a model makes.
 * ``dgfx::segment_softmax(logits, messages, segment_ids, num_segments)`` and
   ``dgfx::sage_mean_linear_relu(rowptr, col, x, weight, bias)`` — forward
   (inference) operators with fake implementations.
@@ -28,7 +34,7 @@ must be CUDA tensors.
 
 from __future__ import annotations
 
-from typing import Optional
+from typing import List, Optional, Tuple
 
 import torch
 
@@ -174,3 +180,196 @@ def gin_propagate(x: torch.Tensor, matrix) -> torch.Tensor:
     from aggregation.gin_matrix (differentiable in x)."""
     rowptr, col, val = matrix
     return torch.ops.dgfx.csr_spmm(rowptr, col, val, x, False, -1)
+
+
+# ---------------------------------------------------------------------------
+# gated_dense_concat
+# ---------------------------------------------------------------------------
+def _like_or_none(t: Optional[torch.Tensor], like: torch.Tensor) -> torch.Tensor:
+    """An operator's outputs are tensors: an empty one stands for None."""
+    return like.new_empty(0) if t is None else t
+
+
+@torch.library.custom_op(f"{_LIB}::gated_dense_concat", mutates_args=())
+def gated_dense_concat(x1: torch.Tensor, x2: Optional[torch.Tensor], w_gate: torch.Tensor, w_up: torch.Tensor,
+                       b_gate: Optional[torch.Tensor], b_up: Optional[torch.Tensor],
+                       activation: str = "silu") -> torch.Tensor:
+    return aggregation.gated_dense_concat(x1.contiguous(), None if x2 is None else x2.contiguous(), w_gate.contiguous(),
+                                          w_up.contiguous(), b_gate, b_up, activation)
+
+
+@gated_dense_concat.register_fake
+def _gated_dense_concat_fake(x1, x2, w_gate, w_up, b_gate, b_up, activation="silu"):
+    return x1.new_empty((x1.shape[0], w_gate.shape[0]))
+
+
+@torch.library.custom_op(f"{_LIB}::gated_dense_concat_grad", mutates_args=())
+def gated_dense_concat_grad(grad: torch.Tensor, x1: torch.Tensor, x2: Optional[torch.Tensor], w_gate: torch.Tensor,
+                            w_up: torch.Tensor, b_gate: Optional[torch.Tensor], b_up: Optional[torch.Tensor],
+                            activation: str, need_input: bool, need_weight: bool) -> List[torch.Tensor]:
+    """[dx1, dx2, dw_gate, dw_up, db_gate, db_up], empty where there is none."""
+    grads = aggregation.gated_dense_concat_backward(
+        grad.contiguous(), x1.contiguous(), None if x2 is None else x2.contiguous(), w_gate.contiguous(),
+        w_up.contiguous(), b_gate, b_up, activation, need_input, need_weight)
+    return [_like_or_none(g, grad) for g in grads]
+
+
+@gated_dense_concat_grad.register_fake
+def _gated_dense_concat_grad_fake(grad, x1, x2, w_gate, w_up, b_gate, b_up, activation, need_input, need_weight):
+    def like(t, wanted=True):
+        return torch.empty(t.shape, dtype=t.dtype, device=t.device) if t is not None and wanted else grad.new_empty(0)
+
+    return [like(x1, need_input), like(x2, need_input), like(w_gate, need_weight), like(w_up, need_weight),
+            like(b_gate), like(b_up)]
+
+
+def _gated_dense_concat_setup(ctx, inputs, output):
+    ctx.save_for_backward(*inputs[:6])
+    ctx.activation = inputs[6]
+
+
+def _gated_dense_concat_backward(ctx, grad):
+    x1, x2, w_gate, w_up, b_gate, b_up = ctx.saved_tensors
+    need = ctx.needs_input_grad
+    grads = torch.ops.dgfx.gated_dense_concat_grad(grad, x1, x2, w_gate, w_up, b_gate, b_up, ctx.activation,
+                                                   need[0] or need[1], need[2] or need[3])
+    return (*(g if n else None for g, n in zip(grads, need)), None)
+
+
+gated_dense_concat.register_autograd(_gated_dense_concat_backward, setup_context=_gated_dense_concat_setup)
+
+
+def sage_mean_gated(rowptr, col, x, w_gate, w_up, b_gate=None, b_up=None, activation: str = "silu") -> torch.Tensor:
+    """GraphSAGE-mean layer with a gated update (aggregation.sage_mean_gated),
+    differentiable in x, the weights and the biases."""
+    agg = torch.ops.dgfx.csr_spmm(rowptr, col, None, x, True, -1)
+    return torch.ops.dgfx.gated_dense_concat(x[: rowptr.shape[0] - 1], agg, w_gate, w_up, b_gate, b_up, activation)
+
+
+# ---------------------------------------------------------------------------
+# segment_group_norm
+# ---------------------------------------------------------------------------
+@torch.library.custom_op(f"{_LIB}::segment_group_norm", mutates_args=())
+def _segment_group_norm(x: torch.Tensor, offsets: torch.Tensor, groups: int, weight: Optional[torch.Tensor],
+                        bias: Optional[torch.Tensor], eps: float,
+                        activation: str) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return aggregation.segment_group_norm(x.contiguous(), offsets.contiguous(), groups, weight, bias, eps, activation)
+
+
+@_segment_group_norm.register_fake
+def _segment_group_norm_fake(x, offsets, groups, weight, bias, eps, activation):
+    stats = (offsets.shape[0] - 1, groups)
+    return (x.new_empty(x.shape), x.new_empty(stats, dtype=torch.float32), x.new_empty(stats, dtype=torch.float32))
+
+
+@torch.library.custom_op(f"{_LIB}::segment_group_norm_grad", mutates_args=())
+def _segment_group_norm_grad(grad: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor, mean: torch.Tensor,
+                             rstd: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor],
+                             activation: str) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(dx, dweight, dbias), empty where there is no weight or bias."""
+    dx, dw, db = aggregation.segment_group_norm_backward(grad.contiguous(), x.contiguous(), offsets.contiguous(), mean,
+                                                         rstd, weight, bias, activation)
+    return dx, _like_or_none(dw, mean), _like_or_none(db, mean)
+
+
+@_segment_group_norm_grad.register_fake
+def _segment_group_norm_grad_fake(grad, x, offsets, mean, rstd, weight, bias, activation):
+    return (x.new_empty(x.shape), mean.new_empty(0) if weight is None else weight.new_empty(weight.shape),
+            mean.new_empty(0) if bias is None else bias.new_empty(bias.shape))
+
+
+def _segment_group_norm_setup(ctx, inputs, output):
+    x, offsets, groups, weight, bias, eps, activation = inputs
+    _, mean, rstd = output
+    ctx.mark_non_differentiable(mean, rstd)
+    ctx.save_for_backward(x, offsets, mean, rstd, weight, bias)
+    ctx.activation = activation
+
+
+def _segment_group_norm_backward(ctx, grad, grad_mean, grad_rstd):
+    x, offsets, mean, rstd, weight, bias = ctx.saved_tensors
+    dx, dw, db = torch.ops.dgfx.segment_group_norm_grad(grad.to(x.dtype), x, offsets, mean, rstd, weight, bias,
+                                                        ctx.activation)
+    need = ctx.needs_input_grad
+    return dx if need[0] else None, None, None, dw if need[3] else None, db if need[4] else None, None, None
+
+
+_segment_group_norm.register_autograd(_segment_group_norm_backward, setup_context=_segment_group_norm_setup)
+
+
+def segment_group_norm(x, offsets, groups: int, weight=None, bias=None, eps: float = 1e-5,
+                       activation: str = "none") -> torch.Tensor:
+    """Group norm with an activation over the segments of a merged batch
+    (aggregation.segment_group_norm), differentiable in x, weight and bias."""
+    return torch.ops.dgfx.segment_group_norm(x, offsets, groups, weight, bias, eps, activation)[0]
+
+
+# ---------------------------------------------------------------------------
+# gated_scan
+# ---------------------------------------------------------------------------
+def _scan_states(x):
+    """Values that the backward pass of a scan over x keeps: one state per
+    channel before every 8th row, every 4th in float32."""
+    block = 4 if x.dtype == torch.float32 else 8
+    return (x.shape[0] + block - 1) // block * x.shape[1]
+
+
+@torch.library.custom_op(f"{_LIB}::gated_scan", mutates_args=())
+def _gated_scan(x: torch.Tensor, gate: torch.Tensor, offsets: torch.Tensor, initial: Optional[torch.Tensor],
+                keep_states: bool) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(h, final, states for the backward pass: empty unless keep_states)."""
+    out = aggregation.gated_scan(x.contiguous(), gate.contiguous(), offsets.contiguous(),
+                                 None if initial is None else initial.contiguous(), return_saved=keep_states)
+    return out if keep_states else (*out, out[1].new_empty(0))
+
+
+@_gated_scan.register_fake
+def _gated_scan_fake(x, gate, offsets, initial, keep_states):
+    return (x.new_empty(x.shape), x.new_empty((offsets.shape[0] - 1, x.shape[1]), dtype=torch.float32),
+            x.new_empty(_scan_states(x) if keep_states else 0, dtype=torch.float32))
+
+
+@torch.library.custom_op(f"{_LIB}::gated_scan_grad", mutates_args=())
+def _gated_scan_grad(grad: Optional[torch.Tensor], grad_final: Optional[torch.Tensor], x: torch.Tensor,
+                     gate: torch.Tensor, offsets: torch.Tensor, saved: torch.Tensor,
+                     initial: Optional[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(dx, dgate, dinitial), the last empty without initial."""
+    dx, dgate, dinitial = aggregation.gated_scan_backward(
+        None if grad is None else grad.contiguous(), x.contiguous(), gate.contiguous(), offsets.contiguous(), saved,
+        None if initial is None else initial.contiguous(), None if grad_final is None else grad_final.contiguous())
+    return dx, dgate, _like_or_none(dinitial, saved)
+
+
+@_gated_scan_grad.register_fake
+def _gated_scan_grad_fake(grad, grad_final, x, gate, offsets, saved, initial):
+    return (x.new_empty(x.shape), gate.new_empty(gate.shape),
+            saved.new_empty(0) if initial is None else initial.new_empty(initial.shape))
+
+
+def _gated_scan_setup(ctx, inputs, output):
+    x, gate, offsets, initial, keep_states = inputs
+    if not keep_states:
+        raise RuntimeError("dgfx::gated_scan: gradients need keep_states=True")
+    ctx.mark_non_differentiable(output[2])
+    ctx.set_materialize_grads(False)
+    ctx.save_for_backward(x, gate, offsets, output[2], initial)
+
+
+def _gated_scan_backward(ctx, grad, grad_final, grad_saved):
+    x, gate, offsets, saved, initial = ctx.saved_tensors
+    need = ctx.needs_input_grad
+    if grad is None and grad_final is None:
+        return None, None, None, None, None
+    dx, dgate, dinitial = torch.ops.dgfx.gated_scan_grad(grad, grad_final, x, gate, offsets, saved, initial)
+    return dx if need[0] else None, dgate if need[1] else None, None, dinitial if need[3] else None, None
+
+
+_gated_scan.register_autograd(_gated_scan_backward, setup_context=_gated_scan_setup)
+
+
+def gated_scan(x, gate, offsets, initial=None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Gated linear recurrence over ragged windows (aggregation.gated_scan):
+    (h, final), differentiable in x, gate and initial. The states that the
+    backward pass needs are only kept where a gradient can be asked for."""
+    keep = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, gate, initial))
+    return torch.ops.dgfx.gated_scan(x, gate, offsets, initial, keep)[:2]
