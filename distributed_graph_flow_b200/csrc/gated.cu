@@ -787,9 +787,12 @@ int launch_nacc(int nacc, const Maps& maps, const Args& p, int units, cudaStream
 
 constexpr int kSms = 148;
 
-// Accumulator columns: the widest tile that still gives every SM one (a
-// narrow tile reads A more often but spreads a small product over the SMs).
+// Accumulator columns: no wider than the product needs, and the widest tile
+// that still gives every SM one (a narrow tile reads A more often but spreads
+// a small product over the SMs).
 int pick_nacc(int64_t m, int64_t cols) {
+  if (cols <= 64) return 64;
+  if (cols <= 128) return ceil_div(m, kBM) >= kSms ? 128 : 64;
   if (ceil_div(m, 2 * kBM) * ceil_div(cols, 256) >= kSms / 2) return 256;
   if (ceil_div(m, kBM) * ceil_div(cols, 128) >= kSms) return 128;
   return 64;

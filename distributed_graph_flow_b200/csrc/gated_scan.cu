@@ -192,6 +192,65 @@ __device__ __forceinline__ typename Pair<T>::raw* column(void* base, const Param
   return static_cast<typename Pair<T>::raw*>(base) + r0 * p.pairs + pair;
 }
 
+// The first segment behind `seg` whose end lies past `row` (nseg if none),
+// and the last one before `seg` that begins above it (-1 if none): the
+// neighbours with rows. Mostly the very next one; a run of segments without
+// rows is crossed by doubling steps, then halving.
+__device__ __forceinline__ int64_t next_segment(const Params& p, int64_t seg, int64_t row) {
+  int64_t lo = seg + 1;  // segments before lo end at or before row
+  if (lo >= p.nseg || __ldg(p.off + lo + 1) > row) return lo < p.nseg ? lo : p.nseg;
+  int64_t step = 1, hi = lo + 1;  // every segment before hi does
+  for (;;) {
+    const int64_t probe = hi - 1 + step;
+    if (probe >= p.nseg) break;
+    if (__ldg(p.off + probe + 1) > row) {
+      int64_t a = hi, b = probe;  // the first past lies in [a, b]
+      while (a < b) {
+        const int64_t mid = (a + b) >> 1;
+        if (__ldg(p.off + mid + 1) > row) b = mid;
+        else a = mid + 1;
+      }
+      return a;
+    }
+    hi = probe + 1;
+    step *= 2;
+  }
+  int64_t a = hi, b = p.nseg;
+  while (a < b) {
+    const int64_t mid = (a + b) >> 1;
+    if (__ldg(p.off + mid + 1) > row) b = mid;
+    else a = mid + 1;
+  }
+  return a;
+}
+__device__ __forceinline__ int64_t previous_segment(const Params& p, int64_t seg) {
+  const int64_t row = __ldg(p.off + seg);
+  if (seg == 0 || __ldg(p.off + seg - 1) < row) return seg - 1;
+  int64_t step = 1, lo = seg - 1;  // segments from lo to seg begin at or past row
+  for (;;) {
+    const int64_t probe = lo - step;
+    if (probe < 0) break;
+    if (__ldg(p.off + probe) < row) {
+      int64_t a = probe, b = lo;  // a begins above row, b does not
+      while (b - a > 1) {
+        const int64_t mid = (a + b) >> 1;
+        if (__ldg(p.off + mid) < row) a = mid;
+        else b = mid;
+      }
+      return a;
+    }
+    lo = probe;
+    step *= 2;
+  }
+  int64_t a = -1, b = lo;
+  while (b - a > 1) {
+    const int64_t mid = (a + b) >> 1;
+    if (__ldg(p.off + mid) < row) a = mid;
+    else b = mid;
+  }
+  return a;
+}
+
 // ---------------------------------------------------------------------------
 // Edge kernel: a warp per segment
 // ---------------------------------------------------------------------------
@@ -453,13 +512,14 @@ __global__ void __launch_bounds__(kThreads, 4) scan_apply_kernel(Params p) {
             if (hp != nullptr) hp[i * p.pairs] = P::pack(st);
             if (r + 1 == limit) {  // this row is the segment's last: on to the next one with rows
               if (inside && p.final != nullptr) store2(p.final, seg, p.channels, at.ch, st);
-              int64_t end = r0 + r + 1;
-              do {
-                ++seg;
-                if (seg < p.nseg) end = __ldg(p.off + seg + 1);
-              } while (seg < p.nseg && end <= r0 + r + 1);
+              seg = next_segment(p, seg, r0 + r + 1);
               inside = seg < p.nseg;
-              limit = inside ? until(end < hi ? end : hi) : p.chunk_rows + 1;
+              if (inside) {
+                const int64_t end = __ldg(p.off + seg + 1);
+                limit = until(end < hi ? end : hi);
+              } else {
+                limit = p.chunk_rows + 1;
+              }
               st = inside && p.initial != nullptr ? load2(p.initial, seg, p.channels, at.ch) : make_float2(0.0f, 0.0f);
             }
           }
@@ -553,18 +613,15 @@ __global__ void __launch_bounds__(kThreads, 2) scan_apply_up_kernel(Params p) {
         int b = begin;
         while (low >= 0 && b >= b0) {
           if (b < b0 + B) starts |= 1u << (b - b0);
-          do {
-            --low;
-          } while (low >= 0 && __ldg(p.off + low) >= __ldg(p.off + low + 1));
+          low = previous_segment(p, low);
           b = low >= 0 ? rel(__ldg(p.off + low)) : -1;
         }
         float2 a[B], keep[B], q[B];
 #pragma unroll
         for (int i = 0; i < B; ++i) {
           if ((starts >> i) & 1u) {
-            do {
-              ++low;
-            } while (__ldg(p.off + low) >= __ldg(p.off + low + 1));
+            low = next_segment(p, low, r0 + b0 + i);
+            low = low < p.nseg ? low : p.nseg - 1;  // only where offsets do not ascend
             st = p.initial != nullptr ? load2(p.initial, low, p.channels, at.ch) : make_float2(0.0f, 0.0f);
           }
           const Row<T> row(g[i], x[i]);
@@ -590,9 +647,7 @@ __global__ void __launch_bounds__(kThreads, 2) scan_apply_up_kernel(Params p) {
             dgp[i * p.pairs] = inside ? P::pack(dg) : P::zero();
             if ((starts >> i) & 1u) {  // this row is the segment's first: on to the one before
               if (p.dinitial != nullptr) store2(p.dinitial, seg, p.channels, at.ch, e);
-              do {
-                --seg;
-              } while (seg >= 0 && __ldg(p.off + seg) >= __ldg(p.off + seg + 1));
+              seg = previous_segment(p, seg);
               end = seg >= 0 ? r : -1;
               begin = seg >= 0 ? rel(__ldg(p.off + seg)) : -1;
             }

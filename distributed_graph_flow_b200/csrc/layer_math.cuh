@@ -118,8 +118,29 @@ __device__ __forceinline__ float2 sigmoid2(float2 z) {
   return make_float2(rcp_f(e.x), rcp_f(e.y));
 }
 
+__device__ __forceinline__ float2 normal_cdf2(float2 z, float2* bell) {
+  auto both = [](float v) { return make_float2(v, v); };
+  const float2 a = fma2(make_float2(fabsf(z.x), fabsf(z.y)), both(0.23164189f), both(1.0f));
+  const float2 t = make_float2(rcp_f(a.x), rcp_f(a.y));
+  float2 poly = fma2(t, both(0.5307027145f), both(-0.7265760135f));
+  poly = fma2(poly, t, both(0.7107068705f));
+  poly = fma2(poly, t, both(-0.142248368f));
+  poly = fma2(poly, t, both(0.127414796f));
+  const float2 x = mul2(mul2(z, both(-0.5f * 1.4426950408889634f)), z);
+  float2 e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(x.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(x.y));
+  const float2 tail = mul2(mul2(poly, t), e), rest = fma2(tail, both(-1.0f), both(1.0f));
+  *bell = e;
+  return make_float2(z.x < 0.0f ? tail.x : rest.x, z.y < 0.0f ? tail.y : rest.y);
+}
+
 template <int ACT>
 __device__ __forceinline__ float2 act2_f(float2 z) {
+  if (ACT == DGFX_ACT_GELU) {
+    float2 bell;
+    return mul2(z, normal_cdf2(z, &bell));
+  }
   if (ACT == DGFX_ACT_SILU) return mul2(z, sigmoid2(z));
   if (ACT == DGFX_ACT_SIGMOID) return sigmoid2(z);
   return make_float2(act_f<ACT>(z.x), act_f<ACT>(z.y));
@@ -136,6 +157,11 @@ __device__ __forceinline__ void act2_both_f(float2 z, float2* value, float2* slo
     const float2 s = sigmoid2(z);
     *value = s;
     *slope = mul2(s, fma2(s, minus, one));
+  } else if (ACT == DGFX_ACT_GELU) {
+    float2 bell;
+    const float2 cdf = normal_cdf2(z, &bell);
+    *value = mul2(z, cdf);
+    *slope = fma2(mul2(z, make_float2(0.39894228040143268f, 0.39894228040143268f)), bell, cdf);
   } else {
     act_both_f<ACT>(z.x, &value->x, &slope->x);
     act_both_f<ACT>(z.y, &value->y, &slope->y);

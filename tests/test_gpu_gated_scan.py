@@ -87,6 +87,9 @@ LENGTHS = {
     "windows": [30, 1, 200, 7, 0, 64, 129, 128, 127],
     "long": [2500],
     "two_long": [1300, 0, 1100],
+    "runs_of_empties": [0] * 700 + [3] + [0] * 300 + [1, 0, 2] + [0] * 1000 + [40] + [0] * 513,
+    "empty_but_the_first": [20] + [0] * 900,
+    "empty_but_the_last": [0] * 900 + [20],
 }
 
 
