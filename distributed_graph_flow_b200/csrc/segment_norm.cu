@@ -116,6 +116,10 @@ struct Place {
 };
 
 __device__ __forceinline__ void team_sync(int id, int threads) {
+  if (threads == 32) {
+    __syncwarp();
+    return;
+  }
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
@@ -313,45 +317,65 @@ __device__ __forceinline__ void few_rows(const typename Quad<T>::raw* x, const t
   }
 }
 
-// The same for a share's rows in order, kAhead loads at a time.
-template <class T, class F>
+// The same for a share's rows in order, kAhead loads at a time. WIDE: full
+// batches without checks, then the rest; otherwise one checked batch of half as
+// many, over and over: a short segment has few full batches, and its warps,
+// each somewhere else in the code, live off the instruction cache.
+template <class T, bool WIDE, class F>
 __device__ __forceinline__ void each_row(const Share& sh, const void* base, F f) {
-  constexpr int B = kAhead<T>;
+  constexpr int B = WIDE ? kAhead<T> : kAhead<T> / 2;
   using raw = typename Quad<T>::raw;
   const raw* x = static_cast<const raw*>(base) + sh.first;
   int left = sh.mine;
-  for (; left >= B; left -= B) {
-    raw v[B];
+  if (WIDE) {
+    for (; left >= B; left -= B) {
+      raw v[B];
 #pragma unroll
-    for (int i = 0; i < B; ++i) v[i] = __ldg(x + i * sh.pitch);
-    x += B * sh.pitch;
+      for (int i = 0; i < B; ++i) v[i] = __ldg(x + i * sh.pitch);
+      x += B * sh.pitch;
 #pragma unroll
-    for (int i = 0; i < B; ++i) f(v[i]);
+      for (int i = 0; i < B; ++i) f(v[i]);
+    }
+    if (left > B / 4) few_rows<T, B - 1>(x, sh.pitch, left, f);
+    else if (left > 0) few_rows<T, B / 4>(x, sh.pitch, left, f);
+  } else {
+#pragma unroll 1
+    for (; left > 0; left -= B) {
+      few_rows<T, B>(x, sh.pitch, left, f);
+      x += B * sh.pitch;
+    }
   }
-  if (left > B / 4) few_rows<T, B - 1>(x, sh.pitch, left, f);
-  else if (left > 0) few_rows<T, B / 4>(x, sh.pitch, left, f);
 }
-template <class T, class F>
+template <class T, bool WIDE, class F>
 __device__ __forceinline__ void each_row(const Share& sh, const void* base, const void* other, F f) {
   constexpr int B = kAhead<T> / 2;
   using raw = typename Quad<T>::raw;
   const raw* x = static_cast<const raw*>(base) + sh.first;
   const raw* d = static_cast<const raw*>(other) + sh.first;
   int left = sh.mine;
-  for (; left >= B; left -= B) {
-    raw v[B], w[B];
+  if (WIDE) {
+    for (; left >= B; left -= B) {
+      raw v[B], w[B];
 #pragma unroll
-    for (int i = 0; i < B; ++i) {
-      v[i] = __ldg(x + i * sh.pitch);
-      w[i] = __ldg(d + i * sh.pitch);
+      for (int i = 0; i < B; ++i) {
+        v[i] = __ldg(x + i * sh.pitch);
+        w[i] = __ldg(d + i * sh.pitch);
+      }
+      x += B * sh.pitch;
+      d += B * sh.pitch;
+#pragma unroll
+      for (int i = 0; i < B; ++i) f(v[i], w[i]);
     }
-    x += B * sh.pitch;
-    d += B * sh.pitch;
-#pragma unroll
-    for (int i = 0; i < B; ++i) f(v[i], w[i]);
+    if (left > B / 4) few_rows<T, B - 1>(x, d, sh.pitch, left, f);
+    else if (left > 0) few_rows<T, B / 4>(x, d, sh.pitch, left, f);
+  } else {
+#pragma unroll 1
+    for (; left > 0; left -= B) {
+      few_rows<T, B>(x, d, sh.pitch, left, f);
+      x += B * sh.pitch;
+      d += B * sh.pitch;
+    }
   }
-  if (left > B / 4) few_rows<T, B - 1>(x, d, sh.pitch, left, f);
-  else if (left > 0) few_rows<T, B / 4>(x, d, sh.pitch, left, f);
 }
 
 // Mean and centred squares of this thread's channels over its share. The
@@ -364,7 +388,7 @@ struct RowStats {
   float mean[kCh], m2[kCh], have;
 };
 
-template <class T>
+template <class T, bool WIDE>
 __device__ __forceinline__ RowStats row_stats(const Params& p, const Share& sh) {
   using Q = Quad<T>;
   RowStats s = {};
@@ -373,7 +397,7 @@ __device__ __forceinline__ RowStats row_stats(const Params& p, const Share& sh) 
   Pairs minus;
   Pairs sum(s.mean), sq(s.m2);
   bool first = true;
-  each_row<T>(sh, p.x, [&](const typename Q::raw& v) {
+  each_row<T, WIDE>(sh, p.x, [&](const typename Q::raw& v) {
     const Pairs f = unpack_pairs<T>(v);
     if (first) {
       f.to(x0);
@@ -402,7 +426,7 @@ __device__ __forceinline__ RowStats row_stats(const Params& p, const Share& sh) 
 }
 
 // y of a share's rows from their statistics.
-template <class T, int ACT>
+template <class T, int ACT, bool WIDE>
 __device__ __forceinline__ void apply_rows(const Params& p, const Share& sh, const Affine& af, const float (&mu)[kCh],
                                            const float (&rs)[kCh]) {
   using Q = Quad<T>;
@@ -412,7 +436,7 @@ __device__ __forceinline__ void apply_rows(const Params& p, const Share& sh, con
   for (int c = 0; c < kCh; ++c) scale[c] = rs[c] * af.w[c];
   const Pairs minus = negated(mu), sc(scale), shift(af.b);
   typename Q::raw* y = static_cast<typename Q::raw*>(p.y) + sh.first;
-  each_row<T>(sh, p.x, [&](const typename Q::raw& v) {
+  each_row<T, WIDE>(sh, p.x, [&](const typename Q::raw& v) {
     Pairs f = unpack_pairs<T>(v);
 #pragma unroll
     for (int c = 0; c < 2; ++c) f.v[c] = act2_f<ACT>(fma2(add2(f.v[c], minus.v[c]), sc.v[c], shift.v[c]));
@@ -449,7 +473,7 @@ __global__ void __maxnreg__(64) norm_forward_kernel(Params p) {
     const float inv = n > 0 ? 1.0f / (static_cast<float>(n) * static_cast<float>(cg)) : 0.0f;
     float mu[kCh], rs[kCh], acc[1][kCh] = {};
     const Share sh(p, at, begin, end);
-    const RowStats rst = row_stats<T>(p, sh);
+    const RowStats rst = row_stats<T, false>(p, sh);
 #pragma unroll
     for (int c = 0; c < kCh; ++c) acc[0][c] = rst.have * rst.mean[c];
     group_sums<1>(p, acc, at, t, p.team, bar, red, gsum);
@@ -463,7 +487,7 @@ __global__ void __maxnreg__(64) norm_forward_kernel(Params p) {
     group_sums<1>(p, acc, at, t, p.team, bar, red, gsum);
     each_group(p, at, g0, [&](int c, int g) { rs[c] = at.on ? rsqrtf(gsum[g] * inv + p.eps) : 0.0f; });
     for (int g = t; g < p.groups; g += p.team) p.rstd[s * p.groups + g] = rsqrtf(gsum[g] * inv + p.eps);
-    apply_rows<T, ACT>(p, sh, af, mu, rs);
+    apply_rows<T, ACT, false>(p, sh, af, mu, rs);
   }
   zero_outside<T>(p, lo, hi);
   if (p.long_counter != nullptr) list_longs(p, lo, hi, smem);
@@ -544,7 +568,7 @@ __global__ void __maxnreg__(64) norm_tile_stats_kernel(Params p) {
   const int cg = p.channels / p.groups;
   for (int tile = blockIdx.x; tile < all.tiles; tile += gridDim.x) {
     const Tile tl(p, all, tile);
-    const RowStats rst = row_stats<T>(p, Share(p, at, tl.begin, tl.end));
+    const RowStats rst = row_stats<T, true>(p, Share(p, at, tl.begin, tl.end));
     const float n_tile = static_cast<float>(tl.end - tl.begin) * static_cast<float>(cg);
     float acc[1][kCh];
 #pragma unroll
@@ -598,7 +622,7 @@ __global__ void __maxnreg__(64) norm_tile_apply_kernel(Params p) {
       mu[c] = __ldg(p.mean + tl.seg * p.groups + g);
       rs[c] = __ldg(p.rstd + tl.seg * p.groups + g);
     });
-    apply_rows<T, ACT>(p, Share(p, at, tl.begin, tl.end), af, mu, rs);
+    apply_rows<T, ACT, true>(p, Share(p, at, tl.begin, tl.end), af, mu, rs);
   }
 }
 
@@ -642,14 +666,14 @@ __device__ __forceinline__ void write_partial(const Params& p, const float (&dwb
 
 // A share's sums for dw and db (added to dwb), and from them its part of the
 // group sums: sum w dz xhat and sum w dz are w times those, channel by channel.
-template <class T, int ACT>
+template <class T, int ACT, bool WIDE>
 __device__ __forceinline__ void grad_sums(const Params& p, const Share& sh, const float (&mu)[kCh], const float (&rs)[kCh],
                                           const Affine& af, float (&acc)[2][kCh], float (&dwb)[2][kCh]) {
   using Q = Quad<T>;
   float dw[kCh] = {}, db[kCh] = {};  // these rows', so that long sums stay pairwise
   Pairs sw(dw), sb(db);
   const Pairs minus = negated(mu), r(rs), w(af.w), b(af.b);
-  each_row<T>(sh, p.x, p.dy, [&](const typename Q::raw& v, const typename Q::raw& d) {
+  each_row<T, WIDE>(sh, p.x, p.dy, [&](const typename Q::raw& v, const typename Q::raw& d) {
     const Pairs f = unpack_pairs<T>(v), g = unpack_pairs<T>(d);
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
@@ -671,13 +695,13 @@ __device__ __forceinline__ void grad_sums(const Params& p, const Share& sh, cons
 }
 
 // dx of a share's rows from their group's sums (divided by n).
-template <class T, int ACT>
+template <class T, int ACT, bool WIDE>
 __device__ __forceinline__ void grad_rows(const Params& p, const Share& sh, const float (&mu)[kCh], const float (&rs)[kCh],
                                           const Affine& af, const float (&s1)[kCh], const float (&s2)[kCh]) {
   using Q = Quad<T>;
   typename Q::raw* dx = static_cast<typename Q::raw*>(p.y) + sh.first;
   const Pairs minus = negated(mu), r(rs), w(af.w), b(af.b), m1 = negated(s1), m2 = negated(s2);
-  each_row<T>(sh, p.x, p.dy, [&](const typename Q::raw& v, const typename Q::raw& d) {
+  each_row<T, WIDE>(sh, p.x, p.dy, [&](const typename Q::raw& v, const typename Q::raw& d) {
     Pairs f = unpack_pairs<T>(v);
     const Pairs g = unpack_pairs<T>(d);
 #pragma unroll
@@ -722,7 +746,7 @@ __global__ void __maxnreg__(80) norm_backward_kernel(Params p) {
       rs[c] = at.on ? __ldg(p.rstd + s * p.groups + g) : 0.0f;
     });
     const Share sh(p, at, begin, end);
-    grad_sums<T, ACT>(p, sh, mu, rs, af, acc, dwb);
+    grad_sums<T, ACT, false>(p, sh, mu, rs, af, acc, dwb);
     group_sums<2>(p, acc, at, t, p.team, bar, red, gsum);
     if (sh.mine > 0) {
       float s1[kCh], s2[kCh];
@@ -730,7 +754,7 @@ __global__ void __maxnreg__(80) norm_backward_kernel(Params p) {
         s1[c] = gsum[g] * inv;
         s2[c] = gsum[p.groups + g] * inv;
       });
-      grad_rows<T, ACT>(p, sh, mu, rs, af, s1, s2);
+      grad_rows<T, ACT, false>(p, sh, mu, rs, af, s1, s2);
     }
   }
   zero_outside<T>(p, lo, hi);
@@ -761,7 +785,7 @@ __global__ void __maxnreg__(80) norm_tile_grad_kernel(Params p) {
       mu[c] = at.on ? __ldg(p.mean + tl.seg * p.groups + g) : 0.0f;
       rs[c] = at.on ? __ldg(p.rstd + tl.seg * p.groups + g) : 0.0f;
     });
-    grad_sums<T, ACT>(p, Share(p, at, tl.begin, tl.end), mu, rs, af, acc, dwb);
+    grad_sums<T, ACT, true>(p, Share(p, at, tl.begin, tl.end), mu, rs, af, acc, dwb);
     group_sums<2>(p, acc, at, threadIdx.x, threads, 1, red, gsum);
     for (int g = threadIdx.x; g < p.groups; g += threads) {
       p.tile_sums[static_cast<int64_t>(tile) * p.groups + g] = make_float2(gsum[g], gsum[p.groups + g]);
@@ -796,7 +820,7 @@ __global__ void __maxnreg__(80) norm_tile_grad_apply_kernel(Params p) {
       s1[c] = s.x;
       s2[c] = s.y;
     });
-    grad_rows<T, ACT>(p, Share(p, at, tl.begin, tl.end), mu, rs, af, s1, s2);
+    grad_rows<T, ACT, true>(p, Share(p, at, tl.begin, tl.end), mu, rs, af, s1, s2);
   }
 }
 
