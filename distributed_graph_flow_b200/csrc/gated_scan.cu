@@ -141,16 +141,18 @@ struct Effect {
     v.x = (n.x < 0.0f || v.x < 0.0f) ? -1.0f : v.x * n.x;
     v.z = (n.z < 0.0f || v.z < 0.0f) ? -1.0f : v.z * n.z;
   }
-  // Items `from`, from + dir, .. (n of them) of a table, in that order.
+  // Items `from`, from + dir, .. (n of them) of a table, in that order, N
+  // loads at a time.
+  template <int N>
   __device__ void then_items(const float4* __restrict__ table, int64_t from, int dir, int64_t n, int64_t pitch) {
-    for (int64_t i = 0; i < n; i += 4) {
-      float4 t[4];
+    for (int64_t i = 0; i < n; i += N) {
+      float4 t[N];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < N; ++k) {
         if (i + k < n) t[k] = __ldg(table + (from + dir * (i + k)) * pitch);
       }
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < N; ++k) {
         if (i + k < n) then(t[k]);
       }
     }
@@ -196,18 +198,18 @@ __device__ __forceinline__ typename Pair<T>::raw* column(void* base, const Param
 // and the last one before `seg` that begins above it (-1 if none): the
 // neighbours with rows. Mostly the very next one; a run of segments without
 // rows is crossed by doubling steps, then halving.
-__device__ __forceinline__ int64_t next_segment(const Params& p, int64_t seg, int64_t row) {
+__device__ __forceinline__ int64_t next_segment(const int64_t* __restrict__ off, int64_t nseg, int64_t seg, int64_t row) {
   int64_t lo = seg + 1;  // segments before lo end at or before row
-  if (lo >= p.nseg || __ldg(p.off + lo + 1) > row) return lo < p.nseg ? lo : p.nseg;
+  if (lo >= nseg || __ldg(off + lo + 1) > row) return lo < nseg ? lo : nseg;
   int64_t step = 1, hi = lo + 1;  // every segment before hi does
   for (;;) {
     const int64_t probe = hi - 1 + step;
-    if (probe >= p.nseg) break;
-    if (__ldg(p.off + probe + 1) > row) {
+    if (probe >= nseg) break;
+    if (__ldg(off + probe + 1) > row) {
       int64_t a = hi, b = probe;  // the first past lies in [a, b]
       while (a < b) {
         const int64_t mid = (a + b) >> 1;
-        if (__ldg(p.off + mid + 1) > row) b = mid;
+        if (__ldg(off + mid + 1) > row) b = mid;
         else a = mid + 1;
       }
       return a;
@@ -215,26 +217,26 @@ __device__ __forceinline__ int64_t next_segment(const Params& p, int64_t seg, in
     hi = probe + 1;
     step *= 2;
   }
-  int64_t a = hi, b = p.nseg;
+  int64_t a = hi, b = nseg;
   while (a < b) {
     const int64_t mid = (a + b) >> 1;
-    if (__ldg(p.off + mid + 1) > row) b = mid;
+    if (__ldg(off + mid + 1) > row) b = mid;
     else a = mid + 1;
   }
   return a;
 }
-__device__ __forceinline__ int64_t previous_segment(const Params& p, int64_t seg) {
-  const int64_t row = __ldg(p.off + seg);
-  if (seg == 0 || __ldg(p.off + seg - 1) < row) return seg - 1;
+__device__ __forceinline__ int64_t previous_segment(const int64_t* __restrict__ off, int64_t seg) {
+  const int64_t row = __ldg(off + seg);
+  if (seg == 0 || __ldg(off + seg - 1) < row) return seg - 1;
   int64_t step = 1, lo = seg - 1;  // segments from lo to seg begin at or past row
   for (;;) {
     const int64_t probe = lo - step;
     if (probe < 0) break;
-    if (__ldg(p.off + probe) < row) {
+    if (__ldg(off + probe) < row) {
       int64_t a = probe, b = lo;  // a begins above row, b does not
       while (b - a > 1) {
         const int64_t mid = (a + b) >> 1;
-        if (__ldg(p.off + mid) < row) a = mid;
+        if (__ldg(off + mid) < row) a = mid;
         else b = mid;
       }
       return a;
@@ -245,7 +247,7 @@ __device__ __forceinline__ int64_t previous_segment(const Params& p, int64_t seg
   int64_t a = -1, b = lo;
   while (b - a > 1) {
     const int64_t mid = (a + b) >> 1;
-    if (__ldg(p.off + mid) < row) a = mid;
+    if (__ldg(off + mid) < row) a = mid;
     else b = mid;
   }
   return a;
@@ -407,7 +409,7 @@ __global__ void __launch_bounds__(kThreads) scan_level_kernel(const float4* __re
   if (g >= outs) return;
   const int64_t first = g * kLevel, last = first + kLevel < count ? first + kLevel : count;
   Effect f;
-  f.then_items(items + pair, up ? last - 1 : first, up ? -1 : 1, last - first, pairs);
+  f.then_items<16>(items + pair, up ? last - 1 : first, up ? -1 : 1, last - first, pairs);
   out[g * pairs + pair] = f.v;
 }
 
@@ -417,17 +419,17 @@ __device__ __forceinline__ float2 entering(const Params& p, int64_t j, int64_t o
   Effect f;
   const int64_t g = j / kLevel, s = g / kLevel, go = o / kLevel, so = go / kLevel;
   if (up) {
-    if (so > s) f.then_items(p.super_ah + pair, so, -1, so - s, p.pairs);
+    if (so > s) f.then_items<4>(p.super_ah + pair, so, -1, so - s, p.pairs);
     const int64_t g_hi = so > s ? (s + 1) * kLevel - 1 : go;
-    if (go > g) f.then_items(p.group_ah + pair, g_hi, -1, g_hi - g, p.pairs);
+    if (go > g) f.then_items<4>(p.group_ah + pair, g_hi, -1, g_hi - g, p.pairs);
     const int64_t c_hi = go > g ? (g + 1) * kLevel - 1 : o;
-    f.then_items(p.chunk_ah + pair, c_hi, -1, c_hi - j, p.pairs);
+    f.then_items<4>(p.chunk_ah + pair, c_hi, -1, c_hi - j, p.pairs);
   } else {
-    if (so < s) f.then_items(p.super_ah + pair, so, 1, s - so, p.pairs);
+    if (so < s) f.then_items<4>(p.super_ah + pair, so, 1, s - so, p.pairs);
     const int64_t g_lo = so < s ? s * kLevel : go;
-    if (go < g) f.then_items(p.group_ah + pair, g_lo, 1, g - g_lo, p.pairs);
+    if (go < g) f.then_items<4>(p.group_ah + pair, g_lo, 1, g - g_lo, p.pairs);
     const int64_t c_lo = go < g ? g * kLevel : o;
-    f.then_items(p.chunk_ah + pair, c_lo, 1, j - c_lo, p.pairs);
+    f.then_items<4>(p.chunk_ah + pair, c_lo, 1, j - c_lo, p.pairs);
   }
   return make_float2(f.v.y, f.v.w);
 }
@@ -512,7 +514,7 @@ __global__ void __launch_bounds__(kThreads, 4) scan_apply_kernel(Params p) {
             if (hp != nullptr) hp[i * p.pairs] = P::pack(st);
             if (r + 1 == limit) {  // this row is the segment's last: on to the next one with rows
               if (inside && p.final != nullptr) store2(p.final, seg, p.channels, at.ch, st);
-              seg = next_segment(p, seg, r0 + r + 1);
+              seg = next_segment(p.off, p.nseg, seg, r0 + r + 1);
               inside = seg < p.nseg;
               if (inside) {
                 const int64_t end = __ldg(p.off + seg + 1);
@@ -613,14 +615,14 @@ __global__ void __launch_bounds__(kThreads, 2) scan_apply_up_kernel(Params p) {
         int b = begin;
         while (low >= 0 && b >= b0) {
           if (b < b0 + B) starts |= 1u << (b - b0);
-          low = previous_segment(p, low);
+          low = previous_segment(p.off, low);
           b = low >= 0 ? rel(__ldg(p.off + low)) : -1;
         }
         float2 a[B], keep[B], q[B];
 #pragma unroll
         for (int i = 0; i < B; ++i) {
           if ((starts >> i) & 1u) {
-            low = next_segment(p, low, r0 + b0 + i);
+            low = next_segment(p.off, p.nseg, low, r0 + b0 + i);
             low = low < p.nseg ? low : p.nseg - 1;  // only where offsets do not ascend
             st = p.initial != nullptr ? load2(p.initial, low, p.channels, at.ch) : make_float2(0.0f, 0.0f);
           }
@@ -647,7 +649,7 @@ __global__ void __launch_bounds__(kThreads, 2) scan_apply_up_kernel(Params p) {
             dgp[i * p.pairs] = inside ? P::pack(dg) : P::zero();
             if ((starts >> i) & 1u) {  // this row is the segment's first: on to the one before
               if (p.dinitial != nullptr) store2(p.dinitial, seg, p.channels, at.ch, e);
-              seg = previous_segment(p, seg);
+              seg = previous_segment(p.off, seg);
               end = seg >= 0 ? r : -1;
               begin = seg >= 0 ? rel(__ldg(p.off + seg)) : -1;
             }
