@@ -52,6 +52,8 @@ namespace dgfx {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kApplyThreads = 128;
+constexpr int kAhead = 1;  // blocks of rows on their way in the apply kernels
 constexpr int kCh = 4;     // channels per thread of the single step
 // Rows loaded at a time (32 bytes of each input); rows between saved states.
 template <class T>
@@ -171,7 +173,7 @@ struct Spot {
   int64_t j;
   int pair, ch;
   __device__ explicit Spot(const Params& p) {
-    const int64_t t = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+    const int64_t t = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
     if (t <= 0x7fffffff) {
       const uint32_t q = static_cast<uint32_t>(t) / static_cast<uint32_t>(p.pairs);
       j = q;
@@ -437,14 +439,54 @@ __device__ __forceinline__ float2 entering(const Params& p, int64_t j, int64_t o
 // ---------------------------------------------------------------------------
 // Apply kernels
 // ---------------------------------------------------------------------------
-// Both walk a chunk in blocks of kBlock rows, the next block's loads in
-// flight. A block that lies inside of one segment, with neither edge of it,
+// Both walk a chunk in blocks of kBlock rows, the loads of the next kAhead
+// blocks in flight on their way to shared memory, where each thread has slots
+// of its own: they cost no registers (held in registers instead, 80 bytes
+// spilled and a long series took 91 rather than 80 us). One block ahead is
+// enough: two and three measured 57 and 62 us at 600,011 rows of 64 channels,
+// one 55. A block that lies inside of one segment, with neither edge of it,
 // takes the plain path; any other is walked with its checks per row.
+// A thread waits for its own copies only.
+template <class T, int INPUTS>
+struct Slots {
+  static constexpr int B = kBlock<T>;
+  using raw = typename Pair<T>::raw;
+  raw v[kAhead + 1][INPUTS][B][kApplyThreads];
+
+  // Starts on rows of one input, `pitch` apart, into a stage; `left` of them
+  // are there, the others read as zeros.
+  __device__ __forceinline__ void start(int stage, int input, const raw* from, int pitch, int left) {
+    raw* to = &v[stage][input][0][threadIdx.x];
+    if (left >= B) {
+#pragma unroll
+      for (int i = 0; i < B; ++i) copy(to + i * kApplyThreads, from + i * pitch);
+    } else {
+#pragma unroll
+      for (int i = 0; i < B; ++i) {
+        if (i < left) copy(to + i * kApplyThreads, from + i * pitch);
+        else to[i * kApplyThreads] = Pair<T>::zero();
+      }
+    }
+  }
+  __device__ static __forceinline__ void copy(raw* to, const raw* from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(
+                     static_cast<uint32_t>(__cvta_generic_to_shared(to))),
+                 "l"(from), "n"(sizeof(raw))
+                 : "memory");
+  }
+  // Closes the block that was started last; waits for the one kAhead blocks
+  // before it.
+  __device__ static __forceinline__ void close() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+  __device__ static __forceinline__ void wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory"); }
+  __device__ __forceinline__ raw get(int stage, int input, int i) const { return v[stage][input][i][threadIdx.x]; }
+};
+
 template <class T>
-__global__ void __launch_bounds__(kThreads, 4) scan_apply_kernel(Params p) {
+__global__ void __launch_bounds__(kApplyThreads, 8) scan_apply_kernel(Params p) {
   constexpr int B = kBlock<T>;
   using P = Pair<T>;
   using raw = typename P::raw;
+  __shared__ Slots<T, 2> slots;
   const Spot at(p);
   if (at.j < p.chunks) {
     const int64_t r0 = at.j << p.chunk_shift;
@@ -452,25 +494,18 @@ __global__ void __launch_bounds__(kThreads, 4) scan_apply_kernel(Params p) {
     const raw* gp = column<T>(p.gate, p, r0, at.pair);
     const raw* xp = column<T>(p.x, p, r0, at.pair);
     raw* hp = p.h != nullptr ? column<T>(p.h, p, r0, at.pair) : nullptr;
-    auto fetch = [&](int left, raw(&g)[B], raw(&x)[B]) {  // the next block, `left` rows from the end
-      if (left >= B) {
-#pragma unroll
-        for (int i = 0; i < B; ++i) {
-          g[i] = __ldg(gp + i * p.pairs);
-          x[i] = __ldg(xp + i * p.pairs);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < B; ++i) {
-          g[i] = i < left ? __ldg(gp + i * p.pairs) : P::zero();
-          x[i] = i < left ? __ldg(xp + i * p.pairs) : P::zero();
-        }
+    auto start = [&](int stage, int left) {  // the next block, `left` rows from the end
+      if (left > 0) {
+        slots.start(stage, 0, gp, p.pairs, left);
+        slots.start(stage, 1, xp, p.pairs, left);
+        gp += B * p.pairs;
+        xp += B * p.pairs;
       }
-      gp += B * p.pairs;
-      xp += B * p.pairs;
+      slots.close();
     };
-    raw g[B], x[B];
-    fetch(n, g, x);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) start(k, n - k * B);
+    int stage = 0;
     // The current segment, the row (from r0) where it ends, and whether there
     // is one: rows before the first and behind the last have none.
     int64_t seg = clamp64(__ldg(p.edge_seg + at.j), -1, p.nseg);
@@ -490,8 +525,8 @@ __global__ void __launch_bounds__(kThreads, 4) scan_apply_kernel(Params p) {
     if (limit == 0) limit = p.chunk_rows + 1;  // only where offsets do not ascend
     float* save = p.save != nullptr ? p.save + r0 / B * p.channels + at.ch : nullptr;
     for (int b0 = 0; b0 < n; b0 += B) {
-      raw gn[B], xn[B];
-      fetch(n - b0 - B, gn, xn);
+      start(stage == 0 ? kAhead : stage - 1, n - b0 - kAhead * B);
+      slots.wait();
       if (save != nullptr) {
         *reinterpret_cast<float2*>(save) = st;
         save += p.channels;
@@ -499,7 +534,7 @@ __global__ void __launch_bounds__(kThreads, 4) scan_apply_kernel(Params p) {
       if (inside && b0 + B < limit && b0 + B <= n) {
 #pragma unroll
         for (int i = 0; i < B; ++i) {
-          const Row<T> row(g[i], x[i]);
+          const Row<T> row(slots.get(stage, 0, i), slots.get(stage, 1, i));
           row.step(st);
           if (hp != nullptr) hp[i * p.pairs] = P::pack(st);
         }
@@ -508,7 +543,7 @@ __global__ void __launch_bounds__(kThreads, 4) scan_apply_kernel(Params p) {
         for (int i = 0; i < B; ++i) {
           const int r = b0 + i;
           if (r < n) {
-            const Row<T> row(g[i], x[i]);
+            const Row<T> row(slots.get(stage, 0, i), slots.get(stage, 1, i));
             row.step(st);
             if (!inside) st = make_float2(0.0f, 0.0f);
             if (hp != nullptr) hp[i * p.pairs] = P::pack(st);
@@ -528,20 +563,17 @@ __global__ void __launch_bounds__(kThreads, 4) scan_apply_kernel(Params p) {
         }
       }
       if (hp != nullptr) hp += B * p.pairs;
-#pragma unroll
-      for (int i = 0; i < B; ++i) {
-        g[i] = gn[i];
-        x[i] = xn[i];
-      }
+      stage = stage == kAhead ? 0 : stage + 1;
     }
   }
 }
 
 template <class T>
-__global__ void __launch_bounds__(kThreads, 2) scan_apply_up_kernel(Params p) {
+__global__ void __launch_bounds__(kApplyThreads, 4) scan_apply_up_kernel(Params p) {
   constexpr int B = kBlock<T>;
   using P = Pair<T>;
   using raw = typename P::raw;
+  __shared__ Slots<T, 3> slots;
   const Spot at(p);
   if (at.j < p.chunks) {
     const int64_t r0 = at.j << p.chunk_shift;
@@ -555,19 +587,21 @@ __global__ void __launch_bounds__(kThreads, 2) scan_apply_up_kernel(Params p) {
     const raw* dp = p.grad != nullptr ? column<T>(p.grad, p, r0 + b0, at.pair) : nullptr;
     raw* dxp = column<T>(p.dx, p, r0 + b0, at.pair);
     raw* dgp = column<T>(p.dgate, p, r0 + b0, at.pair);
-    auto fetch = [&](int left, raw(&g)[B], raw(&x)[B], raw(&d)[B]) {  // a block, `left` rows from the end
-#pragma unroll
-      for (int i = 0; i < B; ++i) {
-        g[i] = i < left ? __ldg(gp + i * p.pairs) : P::zero();
-        x[i] = i < left ? __ldg(xp + i * p.pairs) : P::zero();
-        d[i] = i < left && dp != nullptr ? __ldg(dp + i * p.pairs) : P::zero();
+    auto start = [&](int stage, int left) {  // the next block up, `left` rows from the end (none: no such block)
+      if (left > 0) {
+        slots.start(stage, 0, gp, p.pairs, left);
+        slots.start(stage, 1, xp, p.pairs, left);
+        if (dp != nullptr) slots.start(stage, 2, dp, p.pairs, left);
+        gp -= B * p.pairs;
+        xp -= B * p.pairs;
+        if (dp != nullptr) dp -= B * p.pairs;
       }
-      gp -= B * p.pairs;
-      xp -= B * p.pairs;
-      if (dp != nullptr) dp -= B * p.pairs;
+      slots.close();
     };
-    raw g[B], x[B], d[B];
-    fetch(n - b0, g, x, d);
+    start(0, n - b0);
+#pragma unroll
+    for (int k = 1; k < kAhead; ++k) start(k, b0 >= k * B ? B : 0);
+    int stage = 0;
     const float* saved = p.saved + (r0 + b0) / B * p.channels + at.ch;
     float2 before = __ldg(reinterpret_cast<const float2*>(saved));
     // The segment of the current row (with rows; -1 when none is left), its
@@ -581,10 +615,10 @@ __global__ void __launch_bounds__(kThreads, 2) scan_apply_up_kernel(Params p) {
       if (end64 > r0 + n) e = entering(p, at.j, (end64 - 1) >> p.chunk_shift, at.pair, true);
     }
     for (; b0 >= 0; b0 -= B) {
-      raw gn[B], xn[B], dn[B];
+      start(stage == 0 ? kAhead : stage - 1, b0 >= kAhead * B ? B : 0);
+      slots.wait();
       float2 before_next = make_float2(0.0f, 0.0f);
       if (b0 > 0) {
-        fetch(B, gn, xn, dn);
         saved -= p.channels;
         before_next = __ldg(reinterpret_cast<const float2*>(saved));
       }
@@ -593,7 +627,7 @@ __global__ void __launch_bounds__(kThreads, 2) scan_apply_up_kernel(Params p) {
         float2 a[B], keep[B], q[B];  // q = (h_{t-1} - x_t) a_t (1 - a_t), forward
 #pragma unroll
         for (int i = 0; i < B; ++i) {
-          const Row<T> row(g[i], x[i]);
+          const Row<T> row(slots.get(stage, 0, i), slots.get(stage, 1, i));
           a[i] = row.a;
           keep[i] = row.keep;
           q[i] = make_float2((st.x - row.x.x) * (row.a.x * row.keep.x), (st.y - row.x.y) * (row.a.y * row.keep.y));
@@ -601,7 +635,7 @@ __global__ void __launch_bounds__(kThreads, 2) scan_apply_up_kernel(Params p) {
         }
 #pragma unroll
         for (int i = B - 1; i >= 0; --i) {
-          const float2 dv = P::unpack(d[i]);
+          const float2 dv = P::unpack(dp != nullptr ? slots.get(stage, 2, i) : P::zero());
           const float2 delta = make_float2(dv.x + e.x, dv.y + e.y);
           e = make_float2(a[i].x * delta.x, a[i].y * delta.y);
           dxp[i * p.pairs] = P::pack(make_float2(keep[i].x * delta.x, keep[i].y * delta.y));
@@ -626,7 +660,7 @@ __global__ void __launch_bounds__(kThreads, 2) scan_apply_up_kernel(Params p) {
             low = low < p.nseg ? low : p.nseg - 1;  // only where offsets do not ascend
             st = p.initial != nullptr ? load2(p.initial, low, p.channels, at.ch) : make_float2(0.0f, 0.0f);
           }
-          const Row<T> row(g[i], x[i]);
+          const Row<T> row(slots.get(stage, 0, i), slots.get(stage, 1, i));
           a[i] = row.a;
           keep[i] = row.keep;
           q[i] = make_float2((st.x - row.x.x) * (row.a.x * row.keep.x), (st.y - row.x.y) * (row.a.y * row.keep.y));
@@ -640,7 +674,7 @@ __global__ void __launch_bounds__(kThreads, 2) scan_apply_up_kernel(Params p) {
             if (r + 1 == end) {
               e = p.grad_final != nullptr ? load2(p.grad_final, seg, p.channels, at.ch) : make_float2(0.0f, 0.0f);
             }
-            const float2 dv = P::unpack(d[i]);
+            const float2 dv = P::unpack(dp != nullptr ? slots.get(stage, 2, i) : P::zero());
             const float2 delta = make_float2(dv.x + e.x, dv.y + e.y);
             const float2 dx = make_float2(keep[i].x * delta.x, keep[i].y * delta.y);
             const float2 dg = make_float2(q[i].x * delta.x, q[i].y * delta.y);
@@ -658,12 +692,7 @@ __global__ void __launch_bounds__(kThreads, 2) scan_apply_up_kernel(Params p) {
       }
       dxp -= B * p.pairs;
       dgp -= B * p.pairs;
-#pragma unroll
-      for (int i = 0; i < B; ++i) {
-        g[i] = gn[i];
-        x[i] = xn[i];
-        d[i] = dn[i];
-      }
+      stage = stage == kAhead ? 0 : stage + 1;
       before = before_next;
     }
   }
@@ -738,7 +767,9 @@ size_t carve(void* base, size_t cap, int64_t rows, int64_t channels, Params* p, 
   return arena.used;
 }
 
-unsigned grid_of(int64_t items) { return static_cast<unsigned>(std::max<int64_t>(1, ceil_div(items, kThreads))); }
+unsigned grid_of(int64_t items, int threads = kThreads) {
+  return static_cast<unsigned>(std::max<int64_t>(1, ceil_div(items, threads)));
+}
 
 template <class T>
 int launch(const Params& p, bool up, cudaStream_t stream) {
@@ -761,8 +792,9 @@ int launch(const Params& p, bool up, cudaStream_t stream) {
     }
   }
   if (p.chunks > 0) {
-    if (up) scan_apply_up_kernel<T><<<grid, kThreads, 0, stream>>>(p);
-    else scan_apply_kernel<T><<<grid, kThreads, 0, stream>>>(p);
+    const unsigned blocks = grid_of(p.chunks * p.pairs, kApplyThreads);
+    if (up) scan_apply_up_kernel<T><<<blocks, kApplyThreads, 0, stream>>>(p);
+    else scan_apply_kernel<T><<<blocks, kApplyThreads, 0, stream>>>(p);
   }
   DGFX_CUDA_TRY(cudaGetLastError());
   return DGFX_OK;
