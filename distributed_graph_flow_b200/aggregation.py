@@ -389,6 +389,15 @@ def _layer_offsets(who: str, offsets) -> int:
     return offsets.numel() - 1
 
 
+def _layer_apart(who: str, name: str, out, **inputs) -> None:
+    """Refuses an output that shares memory with an input: other blocks of the
+    kernel may still read what one has overwritten."""
+    begin, end = out.data_ptr(), out.data_ptr() + out.numel() * out.element_size()
+    for other, t in inputs.items():
+        if t is not None and t.data_ptr() < end and begin < t.data_ptr() + t.numel() * t.element_size():
+            raise ValueError(f"{who}: {name} must not overlap {other}")
+
+
 class _LayerGuard:
     """Device and stream of a call that does not run where the caller stands:
     the operands' device becomes the current one and ``stream`` the current
@@ -477,14 +486,15 @@ def gated_dense_concat(x1, x2, w_gate, w_up, b_gate=None, b_up=None, activation:
 
     x1 [M, K1], x2 [M, K2] or None, w_gate and w_up [N, K1 + K2] (torch Linear
     layout) bfloat16, biases float32 [N] or None; K1, K2 and N multiples of 8;
-    contiguous. activation: silu, gelu (erf form), relu, sigmoid or none. fp32
-    accumulation, one rounding to bfloat16. ``dense_check`` reports pipeline
+    contiguous; out must not overlap them. activation: silu, gelu (erf form),
+    relu, sigmoid or none. fp32 accumulation, one rounding to bfloat16. ``dense_check`` reports pipeline
     timeouts of this call too."""
     who = "gated_dense_concat"
     m, k1, k2, n = _gated_operands(who, x1, x2, w_gate, w_up, b_gate, b_up)
     act = _activation_code(who, activation)
     if out is not None:
         _layer_operand(who, "out", out, (m, n), torch.bfloat16)
+        _layer_apart(who, "out", out, x1=x1, x2=x2, w_gate=w_gate, w_up=w_up, b_gate=b_gate, b_up=b_up)
     _workspace_bytes("dgfx_gated_dense_concat_backward_workspace_size", k1, k2, m, n)  # refuses sizes before devices
     guard = _layer_guard(who, stream, x1, x2, w_gate, w_up, b_gate, b_up, out)
     if guard is not None:
@@ -691,6 +701,8 @@ def gated_scan_step(x, gate, state, out_state=None, stream=None):
     _layer_operand(who, "state", state, (n, channels), torch.float32)
     if out_state is not None:
         _layer_operand(who, "out_state", out_state, (n, channels), torch.float32)
+        in_place = out_state.data_ptr() == state.data_ptr()
+        _layer_apart(who, "out_state", out_state, x=x, gate=gate, state=None if in_place else state)
     guard = _layer_guard(who, stream, x, gate, state, out_state)
     if guard is not None:
         with guard:

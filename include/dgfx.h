@@ -352,7 +352,7 @@ int dgfx_dense_check(dgfx_stream stream);
  * d_w_gate, d_w_up bf16 [n, k1 + k2] (torch Linear layout), biases fp32 [n] or
  * NULL, act a DGFX_ACT_*; fp32 accumulation, both projections and the gate
  * in one kernel, one rounding to bf16. k1 >= 8; k1, k2 and n multiples of 8;
- * operands contiguous and 16-byte aligned.
+ * operands contiguous and 16-byte aligned; outputs must not overlap inputs.
  * Backward from d_dh (bf16 [m, n]): d_dx1, d_dx2 (bf16, each may be NULL),
  * d_dw_gate and d_dw_up (bf16, both or neither), d_db_gate, d_db_up (fp32,
  * each may be NULL). The projections are computed again; the gradients of

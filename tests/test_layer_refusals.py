@@ -69,6 +69,22 @@ def test_refused(call, match):
         call()
 
 
+def test_overlapping_outputs():
+    """An output over an input would be read by other blocks after it is
+    written; the step's state in place is each thread's own."""
+    buf = torch.zeros((12, 16), dtype=BF)
+    for name, kw in (("x1", {"x1": buf[:8]}), ("x2", {"x2": buf[4:]}), ("w_gate", {"w_gate": _x(24, 32, BF)[:16]})):
+        out = buf[2:10] if name != "w_gate" else kw["w_gate"].view(-1)[128:256].view(8, 16)
+        with pytest.raises(ValueError, match=f"out must not overlap {name}"):
+            _gated(out=out, **kw)
+    state = torch.zeros(9, 16)
+    with pytest.raises(ValueError, match="out_state must not overlap state"):
+        aggregation.gated_scan_step(_x(), _x(), state[:8], out_state=state[1:])
+    x = _x()
+    with pytest.raises(ValueError, match="out_state must not overlap x"):
+        aggregation.gated_scan_step(x, _x(), state[:8], out_state=x)
+
+
 def test_rows_too_wide():
     with pytest.raises(RuntimeError, match="at most 4096 bytes"):
         aggregation.segment_group_norm(_x(c=1028), OFF, 4)
