@@ -1,6 +1,6 @@
 // Device helpers shared by the layer operators (gated dense, segment group
-// norm, gated scan): activations with their derivatives, 16-byte vectors of
-// fp32 / bf16 as fp32 values, and the ragged-segment lookup.
+// norm, gated scan): activations with their derivatives, two values at a time,
+// and 16-byte vectors of fp32 / bf16 as fp32 values.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -21,9 +21,6 @@ __device__ __forceinline__ float rcp_f(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-
-// 1 / (1 + e^-z) without overflow at either end: e^-z = inf gives 0.
-__device__ __forceinline__ float sigmoid_f(float z) { return rcp_f(1.0f + exp_f(-z)); }
 
 // Two fp32 operations in one instruction.
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
@@ -51,64 +48,7 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   return r;
 }
 
-// Phi(z), the normal distribution function, and e^(-z^2 / 2): with x = |z| /
-// sqrt 2, erfc(x) = P(1 / (1 + p x)) e^(-x^2) (Abramowitz and Stegun, Handbook
-// of Mathematical Functions, 7.1.26, absolute error below 1.5e-7), and
-// Phi(z) = erfc(x) / 2 below zero, one minus that above: no subtraction in
-// the lower tail, and the exponential is the derivative's too.
-__device__ __forceinline__ float normal_cdf_f(float z, float* bell) {
-  const float t = rcp_f(fmaf(fabsf(z), 0.23164189f, 1.0f));
-  float poly = fmaf(t, 0.5307027145f, -0.7265760135f);
-  poly = fmaf(poly, t, 0.7107068705f);
-  poly = fmaf(poly, t, -0.142248368f);
-  poly = fmaf(poly, t, 0.127414796f);
-  const float e = exp_f(-0.5f * z * z);
-  const float tail = poly * t * e;
-  *bell = e;
-  return z < 0.0f ? tail : 1.0f - tail;
-}
-
-// Activations (DGFX_ACT_*) and their derivatives in fp32. gelu is the form
-// z Phi(z) = z (1 + erf(z / sqrt 2)) / 2. relu'(0) = 0. relu compares
-// instead of taking a maximum, so that NaN passes through.
-template <int ACT>
-__device__ __forceinline__ float act_f(float z) {
-  if (ACT == DGFX_ACT_RELU) return z < 0.0f ? 0.0f : z;
-  if (ACT == DGFX_ACT_SILU) return z * sigmoid_f(z);
-  if (ACT == DGFX_ACT_GELU) {
-    float bell;
-    return z * normal_cdf_f(z, &bell);
-  }
-  if (ACT == DGFX_ACT_SIGMOID) return sigmoid_f(z);
-  return z;
-}
-
-// act(z) and act'(z) together (they share the exponential).
-template <int ACT>
-__device__ __forceinline__ void act_both_f(float z, float* value, float* slope) {
-  if (ACT == DGFX_ACT_RELU) {
-    *value = z < 0.0f ? 0.0f : z;
-    *slope = z > 0.0f ? 1.0f : 0.0f;
-  } else if (ACT == DGFX_ACT_SILU) {
-    const float s = sigmoid_f(z);
-    *value = z * s;
-    *slope = s * (1.0f + z * (1.0f - s));
-  } else if (ACT == DGFX_ACT_GELU) {
-    float bell;
-    const float cdf = normal_cdf_f(z, &bell);
-    *value = z * cdf;
-    *slope = fmaf(z * 0.39894228040143268f, bell, cdf);
-  } else if (ACT == DGFX_ACT_SIGMOID) {
-    const float s = sigmoid_f(z);
-    *value = s;
-    *slope = s * (1.0f - s);
-  } else {
-    *value = z;
-    *slope = 1.0f;
-  }
-}
-
-// The same for two values at once.
+// 1 / (1 + e^-z) without overflow at either end: e^-z = inf gives 0.
 __device__ __forceinline__ float2 sigmoid2(float2 z) {
   const float2 t = mul2(z, make_float2(-1.4426950408889634f, -1.4426950408889634f));
   float2 e;
@@ -118,6 +58,11 @@ __device__ __forceinline__ float2 sigmoid2(float2 z) {
   return make_float2(rcp_f(e.x), rcp_f(e.y));
 }
 
+// Phi(z), the normal distribution function, and e^(-z^2 / 2): with x = |z| /
+// sqrt 2, erfc(x) = P(1 / (1 + p x)) e^(-x^2) (Abramowitz and Stegun, Handbook
+// of Mathematical Functions, 7.1.26, absolute error below 1.5e-7), and
+// Phi(z) = erfc(x) / 2 below zero, one minus that above: no subtraction in
+// the lower tail, and the exponential is the derivative's too.
 __device__ __forceinline__ float2 normal_cdf2(float2 z, float2* bell) {
   auto both = [](float v) { return make_float2(v, v); };
   const float2 a = fma2(make_float2(fabsf(z.x), fabsf(z.y)), both(0.23164189f), both(1.0f));
@@ -135,6 +80,9 @@ __device__ __forceinline__ float2 normal_cdf2(float2 z, float2* bell) {
   return make_float2(z.x < 0.0f ? tail.x : rest.x, z.y < 0.0f ? tail.y : rest.y);
 }
 
+// Activations (DGFX_ACT_*) of two values in fp32. gelu is the form z Phi(z) =
+// z (1 + erf(z / sqrt 2)) / 2. relu compares instead of taking a maximum, so
+// that NaN passes through.
 template <int ACT>
 __device__ __forceinline__ float2 act2_f(float2 z) {
   if (ACT == DGFX_ACT_GELU) {
@@ -143,9 +91,11 @@ __device__ __forceinline__ float2 act2_f(float2 z) {
   }
   if (ACT == DGFX_ACT_SILU) return mul2(z, sigmoid2(z));
   if (ACT == DGFX_ACT_SIGMOID) return sigmoid2(z);
-  return make_float2(act_f<ACT>(z.x), act_f<ACT>(z.y));
+  if (ACT == DGFX_ACT_RELU) return make_float2(z.x < 0.0f ? 0.0f : z.x, z.y < 0.0f ? 0.0f : z.y);
+  return z;
 }
 
+// act(z) and act'(z) together (they share the exponential). relu'(0) = 0.
 template <int ACT>
 __device__ __forceinline__ void act2_both_f(float2 z, float2* value, float2* slope) {
   const float2 one = make_float2(1.0f, 1.0f), minus = make_float2(-1.0f, -1.0f);
@@ -162,9 +112,12 @@ __device__ __forceinline__ void act2_both_f(float2 z, float2* value, float2* slo
     const float2 cdf = normal_cdf2(z, &bell);
     *value = mul2(z, cdf);
     *slope = fma2(mul2(z, make_float2(0.39894228040143268f, 0.39894228040143268f)), bell, cdf);
+  } else if (ACT == DGFX_ACT_RELU) {
+    *value = act2_f<ACT>(z);
+    *slope = make_float2(z.x > 0.0f ? 1.0f : 0.0f, z.y > 0.0f ? 1.0f : 0.0f);
   } else {
-    act_both_f<ACT>(z.x, &value->x, &slope->x);
-    act_both_f<ACT>(z.y, &value->y, &slope->y);
+    *value = z;
+    *slope = one;
   }
 }
 
@@ -231,26 +184,6 @@ struct Quad<__nv_bfloat16> {
   }
   __device__ static __forceinline__ raw zero() { return make_uint2(0, 0); }
 };
-
-// First segment whose end lies past `row` (nseg if none): every lane of the
-// warp probes one of 32 evenly spaced ends per round, so the search takes
-// ceil(log32) dependent loads. Call from a full warp; all lanes get it.
-__device__ __forceinline__ int64_t warp_first_segment(const int64_t* __restrict__ off, int64_t nseg, int64_t row) {
-  const int lane = threadIdx.x & 31;
-  int64_t lo = 0, hi = nseg;  // the answer lies in [lo, hi]
-  while (hi > lo) {
-    const int64_t step = (hi - lo + 31) >> 5;
-    const int64_t p = lo + step * (lane + 1) - 1;  // last index of this lane's part
-    const bool past = p >= hi || off[p + 1] > row;
-    const unsigned m = __ballot_sync(0xffffffffu, past);
-    const int k = m == 0u ? 32 : __ffs(static_cast<int>(m)) - 1;
-    const int64_t nlo = lo + step * k;
-    const int64_t nhi = lo + step * (k + 1) - 1;
-    lo = nlo < hi ? nlo : hi;
-    hi = nhi < hi ? nhi : hi;
-  }
-  return lo;
-}
 
 __host__ __device__ __forceinline__ int64_t clamp64(int64_t v, int64_t lo, int64_t hi) {
   return v < lo ? lo : (v > hi ? hi : v);

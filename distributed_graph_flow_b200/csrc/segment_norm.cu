@@ -149,7 +149,7 @@ __device__ __forceinline__ void group_sums(const Params& p, const float (&acc)[K
   const int lanes = 1 << shift;
   const int each = values / p.groups;
   const int sub = t & (lanes - 1);
-    for (int i = 0; i < (K * p.groups) << shift; i += threads) {
+  for (int i = 0; i < (K * p.groups) << shift; i += threads) {
     const int g = (t + i) >> shift;  // k * groups + group
     float s = 0.0f;
     if (g < K * p.groups) {
@@ -159,16 +159,6 @@ __device__ __forceinline__ void group_sums(const Params& p, const float (&acc)[K
     if (g < K * p.groups && sub == 0) gsum[g] = s;
   }
   team_sync(bar, threads);
-}
-
-template <class T>
-__device__ __forceinline__ typename Quad<T>::raw load_quad(const Params& p, const void* base, int64_t row, int col) {
-  return __ldg(static_cast<const typename Quad<T>::raw*>(base) + row * p.quads + col);
-}
-
-template <class T>
-__device__ __forceinline__ void store_quad(const Params& p, int64_t row, int col, const float (&f)[kCh]) {
-  static_cast<typename Quad<T>::raw*>(p.y)[row * p.quads + col] = Quad<T>::pack(f);
 }
 
 // The affine parameters of this thread's channels.
@@ -256,7 +246,8 @@ struct LongList {
   __device__ explicit LongList(const Params& p) {
     const unsigned long long c = *p.long_counter;
     const int64_t t = static_cast<int64_t>(c & 0xffffffffull);
-    count = static_cast<int>(c >> 32);
+    const int64_t n = static_cast<int64_t>(c >> 32);
+    count = static_cast<int>(n < p.max_long ? n : p.max_long);
     tiles = static_cast<int>(t < p.max_tiles ? t : p.max_tiles);
   }
 };
@@ -479,7 +470,7 @@ __global__ void __maxnreg__(64) norm_forward_kernel(Params p) {
     group_sums<1>(p, acc, at, t, p.team, bar, red, gsum);
     each_group(p, at, g0, [&](int c, int g) {
       mu[c] = at.on ? gsum[g] * inv : 0.0f;
-      const float d = rst.mean[c] - mu[c];
+      const float d = rst.have > 0.0f ? rst.mean[c] - mu[c] : 0.0f;
       acc[0][c] = rst.m2[c] + rst.have * d * d;
     });
     for (int g = t; g < p.groups; g += p.team) p.mean[s * p.groups + g] = gsum[g] * inv;
@@ -575,7 +566,7 @@ __global__ void __maxnreg__(64) norm_tile_stats_kernel(Params p) {
     for (int c = 0; c < kCh; ++c) acc[0][c] = rst.have * rst.mean[c];
     group_sums<1>(p, acc, at, threadIdx.x, threads, 1, red, gsum);
     each_group(p, at, g0, [&](int c, int g) {
-      const float d = at.on ? rst.mean[c] - gsum[g] / n_tile : 0.0f;
+      const float d = rst.have > 0.0f ? rst.mean[c] - gsum[g] / n_tile : 0.0f;
       acc[0][c] = rst.m2[c] + rst.have * d * d;
     });
     for (int g = threadIdx.x; g < p.groups; g += threads) {

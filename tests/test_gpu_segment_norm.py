@@ -170,6 +170,15 @@ def test_large_mean_keeps_its_variance(cuda):
     _check(x, off, 4, None, None, torch.randn((500, 16), generator=g), "none")
 
 
+@pytest.mark.parametrize("rows", [3, 700])
+def test_values_whose_square_overflows(cuda, rows):
+    """A mean of 1e20 with a spread of 1e17: squares of the distances stay
+    finite, and threads without rows add nothing (not 0 times infinity)."""
+    g = torch.Generator().manual_seed(9)
+    x = torch.randn((rows, 16), generator=g) * 1e17 + 1e20
+    _check(x, _offsets([rows]), 4, None, None, torch.randn((rows, 16), generator=g), "none")
+
+
 def test_bad_offsets_stay_in_bounds(cuda):
     """Offsets past the rows (or descending) are clamped, never followed."""
     from distributed_graph_flow_b200 import aggregation
