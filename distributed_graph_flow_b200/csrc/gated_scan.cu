@@ -146,12 +146,12 @@ struct Effect {
   // Items `from`, from + dir, .. (n of them) of a table, in that order, N
   // loads at a time.
   template <int N>
-  __device__ void then_items(const float4* __restrict__ table, int64_t from, int dir, int64_t n, int64_t pitch) {
+  __device__ void then_items(const float4* table, int64_t from, int dir, int64_t n, int64_t pitch) {
     for (int64_t i = 0; i < n; i += N) {
       float4 t[N];
 #pragma unroll
       for (int k = 0; k < N; ++k) {
-        if (i + k < n) t[k] = __ldg(table + (from + dir * (i + k)) * pitch);
+        if (i + k < n) t[k] = table[(from + dir * (i + k)) * pitch];
       }
 #pragma unroll
       for (int k = 0; k < N; ++k) {
@@ -264,6 +264,7 @@ __device__ __forceinline__ int64_t previous_segment(const int64_t* __restrict__ 
 // rows get their state or gradient of it: out[s] = in[s] (0 without `in`).
 __global__ void __launch_bounds__(kThreads) scan_edge_kernel(Params p, int up, const float* __restrict__ in,
                                                              float* __restrict__ out) {
+  let_next_start();
   const int64_t threads = static_cast<int64_t>(gridDim.x) * kThreads;
   const int64_t t = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
   const int lane = threadIdx.x & 31;
@@ -345,11 +346,13 @@ __device__ __forceinline__ void walk(const typename Pair<T>::raw* gate, const ty
 // crosses its lower edge, the first row of chunk j + 1.
 template <class T>
 __global__ void __launch_bounds__(kThreads, 4) scan_chunk_kernel(Params p) {
+  let_next_start();
+  after_previous();
   const Spot at(p);
   if (at.j + 1 >= p.chunks) return;
   const int64_t first = at.j << p.chunk_shift, edge = first + p.chunk_rows;
   // Clamped here and below: offsets that do not ascend leave anything.
-  const int64_t seg = clamp64(__ldg(p.edge_seg + at.j + 1), -1, p.nseg);
+  const int64_t seg = clamp64(p.edge_seg[at.j + 1], -1, p.nseg);
   Effect f;
   f.v = make_float4(-1.0f, 0.0f, -1.0f, 0.0f);
   if (seg >= 0 && seg < p.nseg) {
@@ -375,12 +378,14 @@ __global__ void __launch_bounds__(kThreads, 4) scan_chunk_kernel(Params p) {
 // upper edge.
 template <class T>
 __global__ void __launch_bounds__(kThreads, 4) scan_chunk_up_kernel(Params p) {
+  let_next_start();
+  after_previous();
   const Spot at(p);
   if (at.j >= p.chunks || at.j == 0) return;
   const int64_t edge = at.j << p.chunk_shift;
   const int64_t stop = edge + p.chunk_rows < p.rows ? edge + p.chunk_rows : p.rows;
   // The segment of the last row above the edge, if it goes on below it.
-  const int64_t seg = clamp64(__ldg(p.edge_seg + at.j - 1), -1, p.nseg - 1);
+  const int64_t seg = clamp64(p.edge_seg[at.j - 1], -1, p.nseg - 1);
   Effect f;
   f.v = make_float4(-1.0f, 0.0f, -1.0f, 0.0f);
   if (seg >= 0 && __ldg(p.off + seg + 1) > edge) {
@@ -403,8 +408,10 @@ __global__ void __launch_bounds__(kThreads, 4) scan_chunk_up_kernel(Params p) {
 
 // Effects of groups of kLevel items of the level below, in the order of the
 // pass (`up`: from the last to the first).
-__global__ void __launch_bounds__(kThreads) scan_level_kernel(const float4* __restrict__ items, int64_t count, int pairs,
+__global__ void __launch_bounds__(kThreads) scan_level_kernel(const float4* items, int64_t count, int pairs,
                                                               int up, float4* __restrict__ out, int64_t outs) {
+  let_next_start();
+  after_previous();
   const int64_t t = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
   const int64_t g = t / pairs;
   const int pair = static_cast<int>(t - g * pairs);
@@ -483,6 +490,7 @@ struct Slots {
 
 template <class T>
 __global__ void __launch_bounds__(kApplyThreads, 8) scan_apply_kernel(Params p) {
+  after_previous();
   constexpr int B = kBlock<T>;
   using P = Pair<T>;
   using raw = typename P::raw;
@@ -508,7 +516,7 @@ __global__ void __launch_bounds__(kApplyThreads, 8) scan_apply_kernel(Params p) 
     int stage = 0;
     // The current segment, the row (from r0) where it ends, and whether there
     // is one: rows before the first and behind the last have none.
-    int64_t seg = clamp64(__ldg(p.edge_seg + at.j), -1, p.nseg);
+    int64_t seg = clamp64(p.edge_seg[at.j], -1, p.nseg);
     const int64_t hi = clamp64(__ldg(p.off + p.nseg), 0, p.rows);
     auto until = [&](int64_t row) { return static_cast<int>(clamp64(row - r0, 0, p.chunk_rows + 1)); };
     bool inside = seg >= 0 && seg < p.nseg;
@@ -570,6 +578,7 @@ __global__ void __launch_bounds__(kApplyThreads, 8) scan_apply_kernel(Params p) 
 
 template <class T>
 __global__ void __launch_bounds__(kApplyThreads, 4) scan_apply_up_kernel(Params p) {
+  after_previous();
   constexpr int B = kBlock<T>;
   using P = Pair<T>;
   using raw = typename P::raw;
@@ -606,7 +615,7 @@ __global__ void __launch_bounds__(kApplyThreads, 4) scan_apply_up_kernel(Params 
     float2 before = __ldg(reinterpret_cast<const float2*>(saved));
     // The segment of the current row (with rows; -1 when none is left), its
     // first row and the row behind its last, from r0.
-    int64_t seg = clamp64(__ldg(p.edge_seg + at.j), -1, p.nseg - 1);
+    int64_t seg = clamp64(p.edge_seg[at.j], -1, p.nseg - 1);
     int begin = seg >= 0 ? rel(__ldg(p.off + seg)) : -1;
     int end = seg >= 0 ? rel(__ldg(p.off + seg + 1)) : -1;
     float2 e = make_float2(0.0f, 0.0f);
@@ -777,24 +786,24 @@ int launch(const Params& p, bool up, cudaStream_t stream) {
   const unsigned edges = grid_of(std::max(p.chunks, std::min<int64_t>(p.nseg * 32, kSms * 2048)));
   scan_edge_kernel<<<edges, kThreads, 0, stream>>>(p, up, up ? p.grad_final : p.initial, up ? p.dinitial : p.final);
   if (p.chunks > 1) {
-    if (up) scan_chunk_up_kernel<T><<<grid, kThreads, 0, stream>>>(p);
-    else scan_chunk_kernel<T><<<grid, kThreads, 0, stream>>>(p);
+    if (up) launch_after(scan_chunk_up_kernel<T>, grid, kThreads, 0, stream, p);
+    else launch_after(scan_chunk_kernel<T>, grid, kThreads, 0, stream, p);
     // The forward pass has no edge behind the last chunk, the backward pass
     // none above the first: those effects are not written, and no level that
     // a chunk composes holds them.
     if (p.groups > 1) {
-      scan_level_kernel<<<grid_of(p.groups * p.pairs), kThreads, 0, stream>>>(p.chunk_ah, p.chunks, p.pairs, up,
+      launch_after(scan_level_kernel, grid_of(p.groups * p.pairs), kThreads, 0, stream, p.chunk_ah, p.chunks, p.pairs, up,
                                                                              p.group_ah, p.groups);
     }
     if (p.supers > 1) {
-      scan_level_kernel<<<grid_of(p.supers * p.pairs), kThreads, 0, stream>>>(p.group_ah, p.groups, p.pairs, up,
+      launch_after(scan_level_kernel, grid_of(p.supers * p.pairs), kThreads, 0, stream, p.group_ah, p.groups, p.pairs, up,
                                                                              p.super_ah, p.supers);
     }
   }
   if (p.chunks > 0) {
     const unsigned blocks = grid_of(p.chunks * p.pairs, kApplyThreads);
-    if (up) scan_apply_up_kernel<T><<<blocks, kApplyThreads, 0, stream>>>(p);
-    else scan_apply_kernel<T><<<blocks, kApplyThreads, 0, stream>>>(p);
+    if (up) launch_after(scan_apply_up_kernel<T>, blocks, kApplyThreads, 0, stream, p);
+    else launch_after(scan_apply_kernel<T>, blocks, kApplyThreads, 0, stream, p);
   }
   DGFX_CUDA_TRY(cudaGetLastError());
   return DGFX_OK;

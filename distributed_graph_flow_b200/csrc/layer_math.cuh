@@ -185,6 +185,31 @@ struct Quad<__nv_bfloat16> {
   __device__ static __forceinline__ raw zero() { return make_uint2(0, 0); }
 };
 
+// Chains of kernels, each of which needs the one before it: a kernel launched
+// by launch_after may be brought onto the SMs while its predecessor still
+// runs, and waits in after_previous (its first statement) until all of that
+// one's blocks have ended and their writes are visible. The predecessor allows
+// it by let_next_start. What the chain itself has written is read by plain
+// loads, which the compiler keeps behind the wait. The first kernel of a chain is
+// launched as usual.
+__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <class... P, class... A>
+void launch_after(void (*kernel)(P...), unsigned grid, unsigned block, size_t smem, cudaStream_t stream, A... args) {
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(grid);
+  config.blockDim = dim3(block);
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  cudaLaunchKernelEx(&config, kernel, static_cast<P>(args)...);  // its error stays for cudaGetLastError
+}
+
 __host__ __device__ __forceinline__ int64_t clamp64(int64_t v, int64_t lo, int64_t hi) {
   return v < lo ? lo : (v > hi ? hi : v);
 }

@@ -260,7 +260,7 @@ __device__ __forceinline__ int find_long(const int32_t* base, int count, int til
   while (hi - lo > 1) {
     const int step = (hi - lo + 31) >> 5;
     const int q = lo + step * lane;
-    const bool le = q < hi && __ldg(base + q) <= tile;
+    const bool le = q < hi && base[q] <= tile;
     const int k = 31 - __clz(static_cast<int>(__ballot_sync(0xffffffffu, le)));
     hi = min(hi, lo + step * (k + 1));
     lo = lo + step * k;
@@ -443,6 +443,7 @@ __device__ __forceinline__ void apply_rows(const Params& p, const Share& sh, con
 // ---------------------------------------------------------------------------
 template <class T, int ACT>
 __global__ void __maxnreg__(64) norm_forward_kernel(Params p) {
+  let_next_start();
   extern __shared__ float smem[];
   const int in_block = threadIdx.x / p.team, t = threadIdx.x - in_block * p.team, bar = 1 + in_block;
   const Place at(p, t, p.team);
@@ -490,10 +491,10 @@ struct Tile {
   int64_t seg, begin, end, rows_of_seg;  // rows [begin, end)
   __device__ Tile(const Params& p, const LongList& all, int tile) {
     entry = find_long(p.long_base, all.count, tile);
-    first = __ldg(p.long_base + entry);
-    count_tiles = (entry + 1 < all.count ? __ldg(p.long_base + entry + 1) : all.tiles) - first;
-    seg = __ldg(p.long_seg + entry);
-    const longlong2 span = __ldg(p.long_span + entry);
+    first = p.long_base[entry];
+    count_tiles = (entry + 1 < all.count ? p.long_base[entry + 1] : all.tiles) - first;
+    seg = p.long_seg[entry];
+    const longlong2 span = p.long_span[entry];
     const int64_t b = span.x, e = b + span.y;
     rows_of_seg = span.y;
     begin = b + static_cast<int64_t>(tile - first) * p.tile_rows;
@@ -548,6 +549,8 @@ __device__ __forceinline__ void merge_tiles(const Params& p, const Tile& tl, F t
 
 template <class T>
 __global__ void __maxnreg__(64) norm_tile_stats_kernel(Params p) {
+  let_next_start();
+  after_previous();
   extern __shared__ float smem[];
   __shared__ int flag;
   float* red = smem;
@@ -601,6 +604,7 @@ __global__ void __maxnreg__(64) norm_tile_stats_kernel(Params p) {
 
 template <class T, int ACT>
 __global__ void __maxnreg__(64) norm_tile_apply_kernel(Params p) {
+  after_previous();
   const Place at(p, threadIdx.x, blockDim.x);
   const int g0 = at.col * kCh / (p.channels / p.groups);
   const Affine af(p, at);
@@ -610,8 +614,8 @@ __global__ void __maxnreg__(64) norm_tile_apply_kernel(Params p) {
     if (!at.on) continue;
     float mu[kCh], rs[kCh];
     each_group(p, at, g0, [&](int c, int g) {
-      mu[c] = __ldg(p.mean + tl.seg * p.groups + g);
-      rs[c] = __ldg(p.rstd + tl.seg * p.groups + g);
+      mu[c] = p.mean[tl.seg * p.groups + g];
+      rs[c] = p.rstd[tl.seg * p.groups + g];
     });
     apply_rows<T, ACT, true>(p, Share(p, at, tl.begin, tl.end), af, mu, rs);
   }
@@ -710,6 +714,7 @@ __device__ __forceinline__ void grad_rows(const Params& p, const Share& sh, cons
 
 template <class T, int ACT>
 __global__ void __maxnreg__(80) norm_backward_kernel(Params p) {
+  let_next_start();
   extern __shared__ float smem[];
   const int in_block = threadIdx.x / p.team, t = threadIdx.x - in_block * p.team, bar = 1 + in_block;
   const Place at(p, t, p.team);
@@ -758,6 +763,8 @@ __global__ void __maxnreg__(80) norm_backward_kernel(Params p) {
 
 template <class T, int ACT>
 __global__ void __maxnreg__(80) norm_tile_grad_kernel(Params p) {
+  let_next_start();
+  after_previous();
   extern __shared__ float smem[];
   __shared__ int flag;
   float* red = smem;
@@ -796,6 +803,8 @@ __global__ void __maxnreg__(80) norm_tile_grad_kernel(Params p) {
 
 template <class T, int ACT>
 __global__ void __maxnreg__(80) norm_tile_grad_apply_kernel(Params p) {
+  let_next_start();
+  after_previous();
   const Place at(p, threadIdx.x, blockDim.x);
   const int g0 = at.col * kCh / (p.channels / p.groups);
   const Affine af(p, at);
@@ -807,7 +816,7 @@ __global__ void __maxnreg__(80) norm_tile_grad_apply_kernel(Params p) {
     each_group(p, at, g0, [&](int c, int g) {
       mu[c] = __ldg(p.mean + tl.seg * p.groups + g);
       rs[c] = __ldg(p.rstd + tl.seg * p.groups + g);
-      const float2 s = __ldg(p.seg_sums + static_cast<int64_t>(tl.entry) * p.groups + g);
+      const float2 s = p.seg_sums[static_cast<int64_t>(tl.entry) * p.groups + g];
       s1[c] = s.x;
       s2[c] = s.y;
     });
@@ -817,15 +826,16 @@ __global__ void __maxnreg__(80) norm_tile_grad_apply_kernel(Params p) {
 
 // dw and db from the blocks' sums: 32 channels per block, every 32nd slot per
 // warp, then the warps' sums in order.
-__global__ void __launch_bounds__(1024) norm_params_kernel(const float* __restrict__ partial, int slots, int channels,
+__global__ void __launch_bounds__(1024) norm_params_kernel(const float* partial, int slots, int channels,
                                                           float* __restrict__ dw, float* __restrict__ db) {
+  after_previous();
   __shared__ float part[32][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int i = static_cast<int>(blockIdx.x) * 32 + lane;
   float s = 0.0f;
   if (i < 2 * channels) {
 #pragma unroll 8
-    for (int k = warp; k < slots; k += 32) s += __ldg(partial + static_cast<int64_t>(k) * 2 * channels + i);
+    for (int k = warp; k < slots; k += 32) s += partial[static_cast<int64_t>(k) * 2 * channels + i];
   }
   part[warp][lane] = s;
   __syncthreads();
@@ -957,8 +967,8 @@ void launch_forward(const Plan& pl, const Params& p, cudaStream_t stream) {
   norm_forward_kernel<T, ACT><<<pl.grid, pl.threads, smem, stream>>>(p);
   if (pl.longs) {
     const size_t tsmem = (static_cast<size_t>(pl.tile_threads) * pl.split + p.groups) * sizeof(float);
-    norm_tile_stats_kernel<T><<<pl.tile_grid, pl.tile_threads, tsmem, stream>>>(p);
-    norm_tile_apply_kernel<T, ACT><<<pl.tile_grid, pl.tile_threads, 0, stream>>>(p);
+    launch_after(norm_tile_stats_kernel<T>, pl.tile_grid, pl.tile_threads, tsmem, stream, p);
+    launch_after(norm_tile_apply_kernel<T, ACT>, pl.tile_grid, pl.tile_threads, 0, stream, p);
   }
 }
 
@@ -970,8 +980,8 @@ void launch_backward(const Plan& pl, const Params& p, cudaStream_t stream) {
   if (pl.longs) {
     const size_t tsums = 2 * (static_cast<size_t>(pl.tile_threads) * pl.split + p.groups) * sizeof(float);
     const size_t tsmem = std::max(tsums, static_cast<size_t>(pl.tile_threads) * 2 * kCh * sizeof(float));
-    norm_tile_grad_kernel<T, ACT><<<pl.tile_grid, pl.tile_threads, tsmem, stream>>>(p);
-    norm_tile_grad_apply_kernel<T, ACT><<<pl.tile_grid, pl.tile_threads, 0, stream>>>(p);
+    launch_after(norm_tile_grad_kernel<T, ACT>, pl.tile_grid, pl.tile_threads, tsmem, stream, p);
+    launch_after(norm_tile_grad_apply_kernel<T, ACT>, pl.tile_grid, pl.tile_threads, 0, stream, p);
   }
 }
 
@@ -1084,8 +1094,8 @@ extern "C" int dgfx_segment_group_norm_backward(const void* d_dy, const void* d_
   else run<__nv_bfloat16>(activation, true, pl, p, stream);
   DGFX_CUDA_TRY(cudaGetLastError());
   if (d_dweight != nullptr || d_dbias != nullptr) {
-    norm_params_kernel<<<static_cast<unsigned>(ceil_div(2 * channels, 32)), 1024, 0, stream>>>(
-        w.partial, pl.grid + (pl.longs ? pl.tile_grid : 0), static_cast<int>(channels), d_dweight, d_dbias);
+    launch_after(norm_params_kernel, static_cast<unsigned>(ceil_div(2 * channels, 32)), 1024, 0, stream, w.partial,
+                 pl.grid + (pl.longs ? pl.tile_grid : 0), channels, d_dweight, d_dbias);
     DGFX_CUDA_TRY(cudaGetLastError());
   }
   return DGFX_OK;
