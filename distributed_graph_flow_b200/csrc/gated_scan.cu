@@ -128,6 +128,8 @@ struct Params {
   float4* chunk_ah;    // (A, H, A, H) of two channels: [chunks, pairs]
   float4* group_ah;    // [groups, pairs]
   float4* super_ah;    // [supergroups, pairs]
+  int32_t* first_seg;  // at a segment's first row: its number (other rows are not written) [rows]
+  int32_t* last_seg;   // backward: the same at its last row
   int32_t* edge_seg;   // per chunk: where its first (backward: last) row stands among the segments [chunks]
   int64_t rows, nseg, chunks, groups, supers;
   int32_t channels, pairs, chunk_rows, chunk_shift;  // chunk_rows = 1 << chunk_shift
@@ -196,72 +198,17 @@ __device__ __forceinline__ typename Pair<T>::raw* column(void* base, const Param
   return static_cast<typename Pair<T>::raw*>(base) + r0 * p.pairs + pair;
 }
 
-// The first segment behind `seg` whose end lies past `row` (nseg if none),
-// and the last one before `seg` that begins above it (-1 if none): the
-// neighbours with rows. Mostly the very next one; a run of segments without
-// rows is crossed by doubling steps, then halving.
-__device__ __forceinline__ int64_t next_segment(const int64_t* __restrict__ off, int64_t nseg, int64_t seg, int64_t row) {
-  int64_t lo = seg + 1;  // segments before lo end at or before row
-  if (lo >= nseg || __ldg(off + lo + 1) > row) return lo < nseg ? lo : nseg;
-  int64_t step = 1, hi = lo + 1;  // every segment before hi does
-  for (;;) {
-    const int64_t probe = hi - 1 + step;
-    if (probe >= nseg) break;
-    if (__ldg(off + probe + 1) > row) {
-      int64_t a = hi, b = probe;  // the first past lies in [a, b]
-      while (a < b) {
-        const int64_t mid = (a + b) >> 1;
-        if (__ldg(off + mid + 1) > row) b = mid;
-        else a = mid + 1;
-      }
-      return a;
-    }
-    hi = probe + 1;
-    step *= 2;
-  }
-  int64_t a = hi, b = nseg;
-  while (a < b) {
-    const int64_t mid = (a + b) >> 1;
-    if (__ldg(off + mid + 1) > row) b = mid;
-    else a = mid + 1;
-  }
-  return a;
-}
-__device__ __forceinline__ int64_t previous_segment(const int64_t* __restrict__ off, int64_t seg) {
-  const int64_t row = __ldg(off + seg);
-  if (seg == 0 || __ldg(off + seg - 1) < row) return seg - 1;
-  int64_t step = 1, lo = seg - 1;  // segments from lo to seg begin at or past row
-  for (;;) {
-    const int64_t probe = lo - step;
-    if (probe < 0) break;
-    if (__ldg(off + probe) < row) {
-      int64_t a = probe, b = lo;  // a begins above row, b does not
-      while (b - a > 1) {
-        const int64_t mid = (a + b) >> 1;
-        if (__ldg(off + mid) < row) a = mid;
-        else b = mid;
-      }
-      return a;
-    }
-    lo = probe;
-    step *= 2;
-  }
-  int64_t a = -1, b = lo;
-  while (b - a > 1) {
-    const int64_t mid = (a + b) >> 1;
-    if (__ldg(off + mid) < row) a = mid;
-    else b = mid;
-  }
-  return a;
-}
-
 // ---------------------------------------------------------------------------
 // Edge kernel: a warp per segment
 // ---------------------------------------------------------------------------
 // Forward, edge_seg[j] = the segment of chunk j's first row: -1 before the
 // first segment, nseg behind the last. Backward, the last segment with rows
-// that begins at or before chunk j's last row, -1 if there is none. Segments without
-// rows get their state or gradient of it: out[s] = in[s] (0 without `in`).
+// that begins at or before chunk j's last row, -1 if there is none. Every
+// segment with rows leaves its number at its first row (backward: and at its
+// last), so that a walk steps from one to the next by one load, however many
+// segments without rows lie between them (searching the offsets there took
+// 106 us at 2269 windows of 124 rows). Segments without rows get their state or
+// gradient of it: out[s] = in[s] (0 without `in`).
 __global__ void __launch_bounds__(kThreads) scan_edge_kernel(Params p, int up, const float* __restrict__ in,
                                                              float* __restrict__ out) {
   let_next_start();
@@ -285,7 +232,13 @@ __global__ void __launch_bounds__(kThreads) scan_edge_kernel(Params p, int up, c
           store2(out, s, p.channels, c, in != nullptr ? load2(in, s, p.channels, c) : make_float2(0.0f, 0.0f));
         }
       }
-    } else if (up) {
+      continue;
+    }
+    if (lane == 0) {
+      p.first_seg[b] = static_cast<int32_t>(s);
+      if (up) p.last_seg[e - 1] = static_cast<int32_t>(s);
+    }
+    if (up) {
       // Chunks whose last row lies in [b, e); of the last segment with rows,
       // also the chunks behind it.
       for (int64_t j = (b >> p.chunk_shift) + lane; j < p.chunks; j += 32) {
@@ -557,7 +510,7 @@ __global__ void __launch_bounds__(kApplyThreads, 8) scan_apply_kernel(Params p) 
             if (hp != nullptr) hp[i * p.pairs] = P::pack(st);
             if (r + 1 == limit) {  // this row is the segment's last: on to the next one with rows
               if (inside && p.final != nullptr) store2(p.final, seg, p.channels, at.ch, st);
-              seg = next_segment(p.off, p.nseg, seg, r0 + r + 1);
+              seg = r0 + r + 1 < hi ? clamp64(p.first_seg[r0 + r + 1], 0, p.nseg - 1) : p.nseg;
               inside = seg < p.nseg;
               if (inside) {
                 const int64_t end = __ldg(p.off + seg + 1);
@@ -618,6 +571,13 @@ __global__ void __launch_bounds__(kApplyThreads, 4) scan_apply_up_kernel(Params 
     int64_t seg = clamp64(p.edge_seg[at.j], -1, p.nseg - 1);
     int begin = seg >= 0 ? rel(__ldg(p.off + seg)) : -1;
     int end = seg >= 0 ? rel(__ldg(p.off + seg + 1)) : -1;
+    // The segment with rows before the one that begins at row b. (Offsets that
+    // do not ascend may name one that is not above it: the walk ends there.)
+    auto step_back = [&](int b, int64_t* to, int* to_begin) {
+      *to = r0 + b > lo64 && r0 + b <= p.rows ? clamp64(p.last_seg[r0 + b - 1], 0, p.nseg - 1) : -1;
+      *to_begin = *to >= 0 ? rel(__ldg(p.off + *to)) : -1;
+      if (*to_begin >= b) *to = *to_begin = -1;
+    };
     float2 e = make_float2(0.0f, 0.0f);
     if (seg >= 0) {
       const int64_t end64 = clamp64(__ldg(p.off + seg + 1), 0, p.rows);
@@ -651,23 +611,22 @@ __global__ void __launch_bounds__(kApplyThreads, 4) scan_apply_up_kernel(Params 
           dgp[i * p.pairs] = P::pack(make_float2(q[i].x * delta.x, q[i].y * delta.y));
         }
       } else {
-        // Which rows of the block start a segment, and the segment before the
-        // first of them.
+        // Which rows of the block start a segment.
         uint32_t starts = 0;
         int64_t low = seg;
         int b = begin;
         while (low >= 0 && b >= b0) {
           if (b < b0 + B) starts |= 1u << (b - b0);
-          low = previous_segment(p.off, low);
-          b = low >= 0 ? rel(__ldg(p.off + low)) : -1;
+          step_back(b, &low, &b);
         }
         float2 a[B], keep[B], q[B];
 #pragma unroll
         for (int i = 0; i < B; ++i) {
           if ((starts >> i) & 1u) {
-            low = next_segment(p.off, p.nseg, low, r0 + b0 + i);
-            low = low < p.nseg ? low : p.nseg - 1;  // only where offsets do not ascend
-            st = p.initial != nullptr ? load2(p.initial, low, p.channels, at.ch) : make_float2(0.0f, 0.0f);
+            st = make_float2(0.0f, 0.0f);
+            if (p.initial != nullptr) {
+              st = load2(p.initial, clamp64(p.first_seg[r0 + b0 + i], 0, p.nseg - 1), p.channels, at.ch);
+            }
           }
           const Row<T> row(slots.get(stage, 0, i), slots.get(stage, 1, i));
           a[i] = row.a;
@@ -692,9 +651,8 @@ __global__ void __launch_bounds__(kApplyThreads, 4) scan_apply_up_kernel(Params 
             dgp[i * p.pairs] = inside ? P::pack(dg) : P::zero();
             if ((starts >> i) & 1u) {  // this row is the segment's first: on to the one before
               if (p.dinitial != nullptr) store2(p.dinitial, seg, p.channels, at.ch, e);
-              seg = previous_segment(p.off, seg);
+              step_back(r, &seg, &begin);
               end = seg >= 0 ? r : -1;
-              begin = seg >= 0 ? rel(__ldg(p.off + seg)) : -1;
             }
           }
         }
@@ -772,6 +730,8 @@ size_t carve(void* base, size_t cap, int64_t rows, int64_t channels, Params* p, 
   p->group_ah = arena.take<float4>(static_cast<size_t>(p->groups) * p->pairs);
   p->super_ah = arena.take<float4>(static_cast<size_t>(p->supers) * p->pairs);
   p->edge_seg = arena.take<int32_t>(static_cast<size_t>(p->chunks));
+  p->first_seg = arena.take<int32_t>(static_cast<size_t>(rows));
+  p->last_seg = arena.take<int32_t>(static_cast<size_t>(rows));
   *ok = arena.ok();
   return arena.used;
 }
