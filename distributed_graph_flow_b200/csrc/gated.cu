@@ -351,6 +351,10 @@ __device__ __forceinline__ void gated_body(const Maps& maps, const Args& p) {
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
   }
+  // Going backward the kernels form a chain: what is above runs beside the
+  // end of the one before.
+  let_next_start();
+  if (KIND == kInput || KIND == kWeights) after_previous();
   tc_fence_before();
   __syncthreads();
   if (G == 2) cluster_sync();  // the peer's barriers are ready
@@ -702,19 +706,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Layout<KIND, 256, RE
 // both added in order (results do not change from run to run). The first
 // `bias_blocks` blocks take 32 bias columns each (a warp adds every eighth
 // slot, then the warps' sums are added), the others the weights.
-__global__ void __launch_bounds__(256) gated_finish_kernel(const float* __restrict__ tiles, int32_t splits, int64_t n,
+__global__ void __launch_bounds__(256) gated_finish_kernel(const float* tiles, int32_t splits, int64_t n,
                                                            int64_t kk, uint2* __restrict__ dw_gate,
-                                                           uint2* __restrict__ dw_up, const float* __restrict__ sums,
+                                                           uint2* __restrict__ dw_up, const float* sums,
                                                            int32_t slots, int32_t bias_blocks,
                                                            float* __restrict__ db_gate, float* __restrict__ db_up) {
   __shared__ float part[8][32];
+  after_previous();
   if (static_cast<int32_t>(blockIdx.x) < bias_blocks) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t i = static_cast<int64_t>(blockIdx.x) * 32 + lane;
     float s = 0.0f;
     if (i < 2 * n) {
 #pragma unroll 8
-      for (int32_t k = warp; k < slots; k += 8) s += __ldg(sums + static_cast<int64_t>(k) * 2 * n + i);
+      for (int32_t k = warp; k < slots; k += 8) s += sums[static_cast<int64_t>(k) * 2 * n + i];
     }
     part[warp][lane] = s;
     __syncthreads();
@@ -732,7 +737,7 @@ __global__ void __launch_bounds__(256) gated_finish_kernel(const float* __restri
     float4 s = make_float4(0, 0, 0, 0);
 #pragma unroll 4
     for (int32_t k = 0; k < splits; ++k) {
-      const float4 v = __ldg(reinterpret_cast<const float4*>(tiles) + k * quads + i);
+      const float4 v = reinterpret_cast<const float4*>(tiles)[k * quads + i];
       s.x += v.x;
       s.y += v.y;
       s.z += v.z;
@@ -745,7 +750,7 @@ __global__ void __launch_bounds__(256) gated_finish_kernel(const float* __restri
 }
 
 template <class K>
-int launch(K kernel, size_t smem, int threads, std::once_flag* once, const Maps& maps, const Args& p, int grid,
+int launch(K kernel, bool follows, size_t smem, int threads, std::once_flag* once, const Maps& maps, const Args& p, int grid,
            cudaStream_t stream) {
   int dev = 0;
   DGFX_CUDA_TRY(cudaGetDevice(&dev));
@@ -754,7 +759,8 @@ int launch(K kernel, size_t smem, int threads, std::once_flag* once, const Maps&
     attr_err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   });
   DGFX_CUDA_TRY(attr_err);
-  kernel<<<grid, threads, smem, stream>>>(maps, p);
+  if (follows) launch_after(kernel, static_cast<unsigned>(grid), static_cast<unsigned>(threads), smem, stream, maps, p);
+  else kernel<<<grid, threads, smem, stream>>>(maps, p);
   DGFX_CUDA_TRY(cudaGetLastError());
   return DGFX_OK;
 }
@@ -763,14 +769,14 @@ template <int KIND, int NACC>
 int launch_single(const Maps& maps, const Args& p, int units, cudaStream_t stream) {
   static std::once_flag once[64];
   using L = Layout<KIND, NACC, false>;
-  return launch(gated_kernel<KIND, NACC>, L::kBytes, L::kThreads, once, maps, p, units, stream);
+  return launch(gated_kernel<KIND, NACC>, KIND == kInput || KIND == kWeights, L::kBytes, L::kThreads, once, maps, p, units, stream);
 }
 
 template <int KIND, bool RES>
 int launch_pairs(const Maps& maps, const Args& p, int units, cudaStream_t stream) {
   static std::once_flag once[64];
   using L = Layout<KIND, 256, RES>;
-  return launch(gated_pair_kernel<KIND, RES>, L::kBytes, L::kThreads, once, maps, p, 2 * units, stream);
+  return launch(gated_pair_kernel<KIND, RES>, KIND == kInput || KIND == kWeights, L::kBytes, L::kThreads, once, maps, p, 2 * units, stream);
 }
 
 // `units`: CTAs, or pairs of them at 256 accumulator columns.
@@ -1022,9 +1028,9 @@ extern "C" int dgfx_gated_dense_concat_backward_bf16(const void* d_dh, const voi
   if (d_dw_gate != nullptr || d_db_gate != nullptr || d_db_up != nullptr) {
     const int64_t bias_blocks = d_db_gate != nullptr || d_db_up != nullptr ? ceil_div(2 * n, 32) : 0;
     const int64_t weight_blocks = d_dw_gate != nullptr ? std::min<int64_t>(ceil_div(2 * n * kk / 4, 256), kSms * 8) : 0;
-    gated_finish_kernel<<<static_cast<unsigned>(bias_blocks + weight_blocks), 256, 0, stream>>>(
-        ws.tiles, pl.splits, n, kk, static_cast<uint2*>(d_dw_gate), static_cast<uint2*>(d_dw_up), ws.sums,
-        pl.gate.slots() * 4, static_cast<int32_t>(bias_blocks), d_db_gate, d_db_up);
+    launch_after(gated_finish_kernel, static_cast<unsigned>(bias_blocks + weight_blocks), 256, 0, stream, ws.tiles,
+                 pl.splits, n, kk, static_cast<uint2*>(d_dw_gate), static_cast<uint2*>(d_dw_up), ws.sums,
+                 pl.gate.slots() * 4, bias_blocks, d_db_gate, d_db_up);
     DGFX_CUDA_TRY(cudaGetLastError());
   }
   return DGFX_OK;
