@@ -10,6 +10,12 @@ The two forms the reference's GNN layers use:
     24-38); normalize=True is the row-normalised (mean) aggregation.
 Both run in hand-written sm_100a kernels (csrc/aggregate.cu) and accumulate
 in fp32; inputs/outputs are fp32 or bf16.
+
+Around the aggregation, the operators of the layers, with their gradients:
+``dense_concat`` and ``gated_dense_concat`` (the update, csrc/dense.cu and
+csrc/gated.cu), ``segment_group_norm`` (per-graph norm of a merged batch,
+csrc/segment_norm.cu) and ``gated_scan`` (recurrence over ragged windows,
+csrc/gated_scan.cu).
 """
 
 from __future__ import annotations

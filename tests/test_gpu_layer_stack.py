@@ -254,3 +254,26 @@ def test_captured_layer_matches_eager(ops):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(out, exp))
+
+
+def test_tensor_form_of_the_gated_layer(ops):
+    """aggregation.sage_mean_gated (into given buffers, on another stream)
+    against the torch operator, bit for bit."""
+    from distributed_graph_flow_b200 import aggregation
+
+    batch, rowptr, col = _batch()
+    rows = int(rowptr.numel()) - 1
+    g = torch.Generator(device="cuda").manual_seed(4)
+    x = torch.randn((rows, 32), generator=g, device="cuda").to(torch.bfloat16)
+    wg, wu = (0.2 * torch.randn((2, 40, 64), generator=g, device="cuda")).to(torch.bfloat16)
+    bg = torch.randn(40, generator=g, device="cuda")
+    ref = ops.sage_mean_gated(rowptr, col, x, wg.contiguous(), wu.contiguous(), bg, None, "gelu")
+    agg = torch.empty((rows, 32), dtype=torch.bfloat16, device="cuda")
+    out = torch.empty((rows, 40), dtype=torch.bfloat16, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    got = aggregation.sage_mean_gated(rowptr, col, x, wg.contiguous(), wu.contiguous(), bg, None, "gelu", agg=agg, out=out,
+                                      stream=side)
+    torch.cuda.current_stream().wait_stream(side)
+    assert got.data_ptr() == out.data_ptr() and torch.equal(out, ref)
+    aggregation.dense_check()
