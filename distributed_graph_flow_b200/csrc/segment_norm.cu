@@ -13,8 +13,8 @@
 // threads: it reads the segment for the sums and again for the result, the second
 // time from L1. A team is the smallest power of two of threads (32 .. 512,
 // at least a row) that reads the average segment in a few steps, so many
-// small segments share a block. Segments of more than eight steps are listed (in
-// row order) and go through two more kernels: the first reads row tiles and
+// small segments share a block. Segments of more than three to eight steps are
+// listed (in row order) and go through two more kernels: the first reads row tiles and
 // leaves a mean and a centred sum of squares per tile and group, which the
 // block that finishes a segment's last tile merges; the second applies them,
 // tiles in reverse order, so that what the first read last is still in L2.
@@ -875,8 +875,11 @@ int make_plan(const char* who, int64_t rows, int64_t channels, int64_t groups, i
   // kAhead rows per thread, or more than two as long as the teams do not fill
   // the GPU: more threads for the same segment repeat the fixed work of its
   // sums. It takes segments of up to eight steps; longer ones would hold up
-  // their block. Only where 24 steps cover all rows it takes any: two more
-  // launches would cost as much.
+  // their block. Where the teams do not fill the GPU, only of up to three:
+  // row tiles spread over the SMs that are idle (36 segments of 331,464 rows in
+  // all, 16 fp32 channels: 35 us instead of 50; at 300 segments of 250,001 rows,
+  // which fill it, 404 us at six steps, 394 at eight). Only where 24 steps cover all
+  // rows it takes any: two more launches would cost as much.
   const int ahead = (dtype == DGFX_F32 ? kAhead<float> : kAhead<__nv_bfloat16>) / 2;
   const int64_t average = nseg > 0 ? ceil_div(rows, nseg) : 1;
   auto step_rows = [&](int team) { return static_cast<int64_t>(team / pl->quads) * ahead; };
@@ -887,7 +890,8 @@ int make_plan(const char* who, int64_t rows, int64_t channels, int64_t groups, i
   }
   pl->team = team;
   pl->threads = std::max(team, 256);
-  pl->loop_rows = rows <= 24 * step_rows(team) ? rows : 8 * step_rows(team);
+  const int steps = nseg * team < kSms * 768 ? 3 : 8;
+  pl->loop_rows = rows <= 24 * step_rows(team) ? rows : steps * step_rows(team);
   pl->longs = rows > pl->loop_rows;
   const int per_sm = (backward ? 3 : 4) * 256 / pl->threads;
   pl->grid = static_cast<int32_t>(
