@@ -14,10 +14,10 @@
 // time from L1. A team is the smallest power of two of threads (32 .. 512,
 // at least a row) that reads the average segment in a few steps, so many
 // small segments share a block. Segments of more than three to eight steps are
-// listed (in row order) and go through two more kernels: the first reads row tiles and
-// leaves a mean and a centred sum of squares per tile and group, which the
-// block that finishes a segment's last tile merges; the second applies them,
-// tiles in reverse order, so that what the first read last is still in L2.
+// listed (in row order) and go through three more kernels: the first reads row
+// tiles and leaves a mean and a centred sum of squares per tile and group, the
+// second joins a segment's tiles, the third applies them, tiles in reverse
+// order, so that what the first read last is still in L2.
 // When no segment can be that long only the first kernel is launched.
 //
 // Thread t of a team takes the quad (4 channels) t mod Q of every (team / Q)-th
@@ -54,15 +54,14 @@ struct Params {
   float* partial;  // backward: [blocks, 2, C], dw and db of one block
   // Long segments (null if none can be long): how many and how many tiles
   // (count << 32 | tiles), blocks done with the short ones, a slot per
-  // possible first row, the list (number, first tile), finished tiles, per
-  // tile and group two sums.
+  // possible first row, the list (number, first tile), per tile and group two
+  // sums.
   unsigned long long* long_counter;
   unsigned int* blocks_done;
   int32_t* long_slot;
   longlong2* long_span;  // first row, rows
   int32_t* long_seg;
   int32_t* long_base;
-  int32_t* long_done;
   float2* tile_sums;
   float2* seg_sums;  // backward: S1 / n and S2 / n per long segment and group
   int64_t rows, nseg;
@@ -502,57 +501,11 @@ struct Tile {
   }
 };
 
-// True for the whole block when this was the last of the segment's tiles; all
-// tiles' sums are then visible to it.
-__device__ __forceinline__ bool last_tile(const Params& p, const Tile& tile, int* flag) {
-  __threadfence();
-  __syncthreads();
-  if (threadIdx.x == 0) *flag = atomicAdd(p.long_done + tile.entry, 1) == tile.count_tiles - 1;
-  __syncthreads();
-  const bool last = *flag != 0;
-  if (last) __threadfence();
-  return last;
-}
-
-// Adds term(tile's sums, first tile's sums, last tile?) over a segment's
-// tiles, for each group, and hands the total to done(group, total, first
-// tile's sums). The whole block calls; the order of the additions is fixed.
-template <class F, class D>
-__device__ __forceinline__ void merge_tiles(const Params& p, const Tile& tl, F term, D done) {
-  __shared__ float2 part[512];
-  const float2* sums = p.tile_sums + static_cast<int64_t>(tl.first) * p.groups;
-  for (int g0 = 0; g0 < p.groups; g0 += blockDim.x) {
-    const int width = min(p.groups - g0, static_cast<int>(blockDim.x)), lanes = blockDim.x / width;
-    const int lane = threadIdx.x / width, g = g0 + threadIdx.x - lane * width;
-    float2 total = make_float2(0.0f, 0.0f), s0 = total;
-    if (lane < lanes) {
-      s0 = __ldcg(sums + g);
-#pragma unroll 8
-      for (int k = lane; k < tl.count_tiles; k += lanes) {
-        const float2 t = term(__ldcg(sums + static_cast<int64_t>(k) * p.groups + g), s0, k == tl.count_tiles - 1);
-        total.x += t.x;
-        total.y += t.y;
-      }
-    }
-    part[threadIdx.x] = total;
-    __syncthreads();
-    if (lane == 0) {
-      for (int k = 1; k < lanes; ++k) {
-        total.x += part[k * width + threadIdx.x].x;
-        total.y += part[k * width + threadIdx.x].y;
-      }
-      done(g, total, s0);
-    }
-    __syncthreads();
-  }
-}
-
 template <class T>
 __global__ void __maxnreg__(64) norm_tile_stats_kernel(Params p) {
   let_next_start();
   after_previous();
   extern __shared__ float smem[];
-  __shared__ int flag;
   float* red = smem;
   float* gsum = red + blockDim.x * p.split;
   const int threads = blockDim.x;
@@ -579,24 +532,69 @@ __global__ void __maxnreg__(64) norm_tile_stats_kernel(Params p) {
     for (int g = threadIdx.x; g < p.groups; g += threads) {
       p.tile_sums[static_cast<int64_t>(tile) * p.groups + g].y = gsum[g];
     }
-    if (last_tile(p, tl, &flag)) {
-      // Merge the segment's tiles around the first tile's mean m0, as the
-      // threads did their rows.
-      const float n_all = static_cast<float>(tl.rows_of_seg) * static_cast<float>(cg);
-      const float n_full = static_cast<float>(p.tile_rows) * static_cast<float>(cg);
-      const float n_last = static_cast<float>(tl.rows_of_seg - (tl.count_tiles - 1) * p.tile_rows) * static_cast<float>(cg);
-      merge_tiles(
-          p, tl,
-          [&](float2 s, float2 s0, bool last) {
-            const float d = s.x - s0.x, n = last ? n_last : n_full;
-            return make_float2(n * d, s.y + n * d * d);
-          },
-          [&](int g, float2 sum, float2 s0) {
-            const float d = sum.x / n_all;
-            const float m2 = sum.y - sum.x * d;
-            p.mean[tl.seg * p.groups + g] = s0.x + d;
-            p.rstd[tl.seg * p.groups + g] = rsqrtf((m2 < 0.0f ? 0.0f : m2) / n_all + p.eps);
-          });
+  }
+}
+
+// Joins the tiles of every listed segment: up to 32 groups per block and step,
+// the tiles dealt to up to 32 lanes of threads, whose sums are added in order.
+// Forward: means and centred squares, around the first tile's mean as the
+// threads did their rows. BACKWARD: S1 / n and S2 / n. (One block per segment,
+// the one that finished its last tile, took 0.4 ms for 256 groups of a million rows.)
+template <bool BACKWARD>
+__global__ void __launch_bounds__(256) norm_merge_kernel(Params p) {
+  let_next_start();
+  after_previous();
+  __shared__ float2 part[256];
+  constexpr int N = 8;  // loads at a time
+  const LongList all(p);
+  const int width = min(p.groups, 32), lanes = min(256 / width, 32), blocks = (p.groups + width - 1) / width;
+  const int lane = threadIdx.x / width, col = threadIdx.x - lane * width;
+  const int64_t cg = p.channels / p.groups;
+  for (int64_t item = blockIdx.x; item < static_cast<int64_t>(all.count) * blocks; item += gridDim.x) {
+    const int entry = static_cast<int>(item / blocks), g = static_cast<int>(item - static_cast<int64_t>(entry) * blocks) * width + col;
+    const int first = p.long_base[entry], tiles = (entry + 1 < all.count ? p.long_base[entry + 1] : all.tiles) - first;
+    const int64_t rows = p.long_span[entry].y, seg = p.long_seg[entry];
+    if (tiles <= 0) continue;  // only where offsets do not ascend
+    const float2* sums = p.tile_sums + static_cast<int64_t>(first) * p.groups + g;
+    const float n_full = static_cast<float>(p.tile_rows) * static_cast<float>(cg);
+    const float n_last = static_cast<float>(rows - (tiles - 1) * p.tile_rows) * static_cast<float>(cg);
+    const bool on = lane < lanes && g < p.groups;
+    float2 total = make_float2(0.0f, 0.0f), s0 = total;
+    if (on) {
+      if (!BACKWARD) s0 = sums[0];
+      for (int k0 = lane; k0 < tiles; k0 += N * lanes) {
+        float2 v[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          if (k0 + i * lanes < tiles) v[i] = sums[static_cast<int64_t>(k0 + i * lanes) * p.groups];
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int k = k0 + i * lanes;
+          if (k < tiles) {
+            if (BACKWARD) {
+              total = add2(total, v[i]);
+            } else {
+              const float d = v[i].x - s0.x, n = k == tiles - 1 ? n_last : n_full;
+              total.x += n * d;
+              total.y += v[i].y + n * d * d;
+            }
+          }
+        }
+      }
+    }
+    part[threadIdx.x] = total;
+    __syncthreads();
+    if (on && lane == 0) {
+      for (int k = 1; k < lanes; ++k) total = add2(total, part[k * width + col]);
+      const float n_all = static_cast<float>(rows) * static_cast<float>(cg);
+      if (BACKWARD) {
+        p.seg_sums[static_cast<int64_t>(entry) * p.groups + g] = make_float2(total.x / n_all, total.y / n_all);
+      } else {
+        const float d = total.x / n_all, m2 = total.y - total.x * d;
+        p.mean[seg * p.groups + g] = s0.x + d;
+        p.rstd[seg * p.groups + g] = rsqrtf((m2 < 0.0f ? 0.0f : m2) / n_all + p.eps);
+      }
     }
     __syncthreads();
   }
@@ -766,7 +764,6 @@ __global__ void __maxnreg__(80) norm_tile_grad_kernel(Params p) {
   let_next_start();
   after_previous();
   extern __shared__ float smem[];
-  __shared__ int flag;
   float* red = smem;
   float* gsum = red + 2 * blockDim.x * p.split;
   const int threads = blockDim.x;
@@ -788,15 +785,6 @@ __global__ void __maxnreg__(80) norm_tile_grad_kernel(Params p) {
     for (int g = threadIdx.x; g < p.groups; g += threads) {
       p.tile_sums[static_cast<int64_t>(tile) * p.groups + g] = make_float2(gsum[g], gsum[p.groups + g]);
     }
-    if (last_tile(p, tl, &flag)) {
-      const float n_all = static_cast<float>(tl.rows_of_seg) * static_cast<float>(cg);
-      merge_tiles(
-          p, tl, [](float2 s, float2, bool) { return s; },
-          [&](int g, float2 sum, float2) {
-            p.seg_sums[static_cast<int64_t>(tl.entry) * p.groups + g] = make_float2(sum.x / n_all, sum.y / n_all);
-          });
-    }
-    __syncthreads();
   }
   write_partial(p, dwb, at, 1, 0, smem, p.blocks_before + blockIdx.x);
 }
@@ -850,7 +838,7 @@ __global__ void __launch_bounds__(1024) norm_params_kernel(const float* partial,
 // Host side
 // ---------------------------------------------------------------------------
 struct Plan {
-  int32_t quads, team, threads, split, grid, tile_threads, tile_grid;
+  int32_t quads, team, threads, split, grid, tile_threads, tile_grid, merge_grid;
   int64_t loop_rows, tile_rows, max_long, max_tiles;
   bool longs;  // whether a segment can be too long for a team
 };
@@ -901,6 +889,7 @@ int make_plan(const char* who, int64_t rows, int64_t channels, int64_t groups, i
   pl->tile_grid = kSms * (backward ? 3 : 4) / (pl->tile_threads / 256);
   pl->tile_rows = std::max<int64_t>(2 * step_rows(team), ceil_div(rows, 2 * pl->tile_grid));  // two per block
   pl->max_long = rows / (pl->loop_rows + 1) + 1;
+  pl->merge_grid = static_cast<int32_t>(std::min<int64_t>(pl->max_long * ceil_div(groups, 32), kSms * 4));
   pl->max_tiles = ceil_div(rows, pl->tile_rows) + pl->max_long;
   return DGFX_OK;
 }
@@ -909,7 +898,7 @@ struct Work {
   unsigned long long* counter;
   unsigned int* blocks;
   longlong2* span;
-  int32_t *slot, *seg, *base, *done;
+  int32_t *slot, *seg, *base;
   float2 *tile_sums, *seg_sums;
   float* partial;
   size_t clear_bytes, bytes;
@@ -924,7 +913,6 @@ Work carve(void* ws, size_t cap, const Plan& pl, int64_t channels, int64_t group
     w.counter = a.take<unsigned long long>(1);
     w.blocks = a.take<unsigned int>(1);
     w.slot = a.take<int32_t>(static_cast<size_t>(pl.max_long));
-    w.done = a.take<int32_t>(static_cast<size_t>(pl.max_long));
     w.clear_bytes = a.used;
     w.span = a.take<longlong2>(static_cast<size_t>(pl.max_long));
     w.seg = a.take<int32_t>(static_cast<size_t>(pl.max_long));
@@ -958,7 +946,6 @@ Params make_params(const Plan& pl, const Work& w, int64_t rows, int64_t channels
   p.long_span = w.span;
   p.long_seg = w.seg;
   p.long_base = w.base;
-  p.long_done = w.done;
   p.tile_sums = w.tile_sums;
   p.seg_sums = w.seg_sums;
   p.partial = w.partial;
@@ -972,6 +959,7 @@ void launch_forward(const Plan& pl, const Params& p, cudaStream_t stream) {
   if (pl.longs) {
     const size_t tsmem = (static_cast<size_t>(pl.tile_threads) * pl.split + p.groups) * sizeof(float);
     launch_after(norm_tile_stats_kernel<T>, pl.tile_grid, pl.tile_threads, tsmem, stream, p);
+    launch_after(norm_merge_kernel<false>, pl.merge_grid, 256, 0, stream, p);
     launch_after(norm_tile_apply_kernel<T, ACT>, pl.tile_grid, pl.tile_threads, 0, stream, p);
   }
 }
@@ -985,6 +973,7 @@ void launch_backward(const Plan& pl, const Params& p, cudaStream_t stream) {
     const size_t tsums = 2 * (static_cast<size_t>(pl.tile_threads) * pl.split + p.groups) * sizeof(float);
     const size_t tsmem = std::max(tsums, static_cast<size_t>(pl.tile_threads) * 2 * kCh * sizeof(float));
     launch_after(norm_tile_grad_kernel<T, ACT>, pl.tile_grid, pl.tile_threads, tsmem, stream, p);
+    launch_after(norm_merge_kernel<true>, pl.merge_grid, 256, 0, stream, p);
     launch_after(norm_tile_grad_apply_kernel<T, ACT>, pl.tile_grid, pl.tile_threads, 0, stream, p);
   }
 }
