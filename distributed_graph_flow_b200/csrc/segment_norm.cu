@@ -464,7 +464,14 @@ __global__ void __maxnreg__(64) norm_forward_kernel(Params p) {
       continue;
     }
     const int n = static_cast<int>(end - begin);
-    const float inv = n > 0 ? 1.0f / (static_cast<float>(n) * static_cast<float>(cg)) : 0.0f;
+    if (n == 0) {
+      for (int g = t; g < p.groups; g += p.team) {
+        p.mean[s * p.groups + g] = 0.0f;
+        p.rstd[s * p.groups + g] = rsqrtf(p.eps);
+      }
+      continue;
+    }
+    const float inv = 1.0f / (static_cast<float>(n) * static_cast<float>(cg));
     float mu[kCh], rs[kCh], acc[1][kCh] = {};
     const Share sh(p, at, begin, end);
     const RowStats rst = row_stats<T, false>(p, sh);
