@@ -35,6 +35,14 @@
 // Two accumulators: the epilogue of a tile runs beside the products of the next. Every wait is
 // bounded and latched in the status word of dgfx_dense_check; on expiry the roles leave,
 // copies and MMAs are drained and TMEM is freed. No multicast loads.
+//
+// Bound by the tensor cores where there are many rows (K = 512: 4 M N K flop
+// against 2 M (K + N) bytes), at small ones by the chain of one tile. Measured at
+// 500,000 rows, K = 256 + 256, N = 512, silu: forward 385 us by itself (1.36
+// PFLOP/s), 485 us in a loop (1.08), where power holds the clock down; training
+// 2.2 ms in a loop: forward 385, kGates 550 (2 GB of X,
+// dh and D, for which HBM alone takes 310), kInput 412, kWeights 470, finish 5. Tiles of 128 x
+// 256 on single CTAs took 423, 779, 438 and 519. One row: 7 us.
 #include <algorithm>
 
 #include "layer_math.cuh"
@@ -47,6 +55,8 @@ constexpr int kBM = 128;  // rows per CTA
 constexpr int kBK = 64;
 
 enum { kForward = 0, kGates = 1, kInput = 2, kWeights = 3 };
+template <int KIND>
+constexpr bool kFollows = KIND == kInput || KIND == kWeights;  // launched behind another kernel of its call
 
 struct Maps {
   CUtensorMap a1, a2, b1, b2, b3, b4;
@@ -71,7 +81,8 @@ struct Args {
 
 // Per CTA. NACC accumulator columns; 256 of them on a pair of CTAs. RES: the
 // weights of a CTA's column block stay in shared memory (up to kResident
-// K-blocks), and only A rows come by the ring.
+// K-blocks), and only A rows come by the ring (forward 404 us without, 385 with,
+// kGates 600 and 550, at the sizes above).
 constexpr int kResident = 8;
 template <int KIND, int NACC, bool RES>
 struct Layout {
@@ -354,7 +365,7 @@ __device__ __forceinline__ void gated_body(const Maps& maps, const Args& p) {
   // Going backward the kernels form a chain: what is above runs beside the
   // end of the one before.
   let_next_start();
-  if (KIND == kInput || KIND == kWeights) after_previous();
+  if (kFollows<KIND>) after_previous();
   tc_fence_before();
   __syncthreads();
   if (G == 2) cluster_sync();  // the peer's barriers are ready
@@ -769,14 +780,14 @@ template <int KIND, int NACC>
 int launch_single(const Maps& maps, const Args& p, int units, cudaStream_t stream) {
   static std::once_flag once[64];
   using L = Layout<KIND, NACC, false>;
-  return launch(gated_kernel<KIND, NACC>, KIND == kInput || KIND == kWeights, L::kBytes, L::kThreads, once, maps, p, units, stream);
+  return launch(gated_kernel<KIND, NACC>, kFollows<KIND>, L::kBytes, L::kThreads, once, maps, p, units, stream);
 }
 
 template <int KIND, bool RES>
 int launch_pairs(const Maps& maps, const Args& p, int units, cudaStream_t stream) {
   static std::once_flag once[64];
   using L = Layout<KIND, 256, RES>;
-  return launch(gated_pair_kernel<KIND, RES>, KIND == kInput || KIND == kWeights, L::kBytes, L::kThreads, once, maps, p, 2 * units, stream);
+  return launch(gated_pair_kernel<KIND, RES>, kFollows<KIND>, L::kBytes, L::kThreads, once, maps, p, 2 * units, stream);
 }
 
 // `units`: CTAs, or pairs of them at 256 accumulator columns.
@@ -794,8 +805,10 @@ int launch_nacc(int nacc, const Maps& maps, const Args& p, int units, cudaStream
 constexpr int kSms = 148;
 
 // Accumulator columns: no wider than the product needs, and the widest tile
-// that still gives every SM one (a narrow tile reads A more often but spreads
-// a small product over the SMs).
+// that still gives every SM one: a narrow tile reads A more often but spreads
+// a small product over the SMs (K = N = 256, 1000 rows: 4.9 us at 64 columns, 5.7
+// at 128, 8.2 on pairs; 20,000 rows: 17.9, 12.5 and 12.5; 32 outputs of 200,000
+// rows, K = 128: 13.4, 16.9 and 23.9).
 int pick_nacc(int64_t m, int64_t cols) {
   if (cols <= 64) return 64;
   if (cols <= 128) return ceil_div(m, kBM) >= kSms ? 128 : 64;

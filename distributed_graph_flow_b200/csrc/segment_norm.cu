@@ -27,6 +27,13 @@
 // mean^2. All sums are fp32 in an order fixed by the sizes: results do not change from run to
 // run. Rows outside [off[0], off[nseg]) are written as zeros and their inputs
 // are never used.
+//
+// Measured (L2 flushed, forward + backward unless said): one segment of a
+// million rows x 256 bf16 channels, 16 groups, silu 807 us: x is read twice on the
+// way forward and x and dy twice on the way back, 4.1 GB, 5.1 TB/s; 300 ragged
+// segments in 250,001 rows x 200 fp32, gelu 375 us (1.6 GB); a merged batch of
+// 1024 graphs, 41,003 rows x 256 bf16, relu, forward 42 us: one segment per team,
+// so the longest one's chain of loads and sums and the five launches are what it takes.
 #include <algorithm>
 #include <string>
 
@@ -561,7 +568,8 @@ __global__ void __launch_bounds__(256) norm_merge_kernel(Params p) {
   const int lane = threadIdx.x / width, col = threadIdx.x - lane * width;
   const int64_t cg = p.channels / p.groups;
   for (int64_t item = blockIdx.x; item < static_cast<int64_t>(all.count) * blocks; item += gridDim.x) {
-    const int entry = static_cast<int>(item / blocks), g = static_cast<int>(item - static_cast<int64_t>(entry) * blocks) * width + col;
+    const int entry = static_cast<int>(item / blocks);
+    const int g = static_cast<int>(item - static_cast<int64_t>(entry) * blocks) * width + col;
     const int first = p.long_base[entry], tiles = (entry + 1 < all.count ? p.long_base[entry + 1] : all.tiles) - first;
     const int64_t rows = p.long_span[entry].y, seg = p.long_seg[entry];
     if (tiles <= 0) continue;  // only where offsets do not ascend
@@ -875,12 +883,13 @@ int make_plan(const char* who, int64_t rows, int64_t channels, int64_t groups, i
   // A team grows while the average segment takes it more than four steps of
   // kAhead rows per thread, or more than two as long as the teams do not fill
   // the GPU: more threads for the same segment repeat the fixed work of its
-  // sums. It takes segments of up to eight steps; longer ones would hold up
+  // sums (two or eight steps instead of four: within 1% over fifty drawn
+  // sizes). It takes segments of up to eight steps; longer ones would hold up
   // their block. Where the teams do not fill the GPU, only of up to three:
   // row tiles spread over the SMs that are idle (36 segments of 331,464 rows in
   // all, 16 fp32 channels: 35 us instead of 50; at 300 segments of 250,001 rows,
   // which fill it, 404 us at six steps, 394 at eight). Only where 24 steps cover all
-  // rows it takes any: two more launches would cost as much.
+  // rows it takes any: three more launches would cost as much.
   const int ahead = (dtype == DGFX_F32 ? kAhead<float> : kAhead<__nv_bfloat16>) / 2;
   const int64_t average = nseg > 0 ? ceil_div(rows, nseg) : 1;
   auto step_rows = [&](int team) { return static_cast<int64_t>(team / pl->quads) * ahead; };
