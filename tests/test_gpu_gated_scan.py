@@ -118,6 +118,17 @@ def test_one_window_over_many_tiles(cuda):
     _check(x, gate, off, h0, dh, df)
 
 
+@pytest.mark.parametrize("initial", [True, False])
+def test_windows_end_at_chunk_edges(cuda, initial):
+    """Windows that begin and end at the edges of chunks (16 rows), groups (512)
+    and supergroups (16384), and one row to either side of them."""
+    lengths = [16384, 512, 16, 16368 - 512, 512 * 31, 512, 1, 16383, 15, 0, 17, 511, 513, 16 * 900, 0, 5000]
+    off = _offsets(lengths, first=16)
+    rows = int(off[-1]) + 40
+    x, gate, dh, h0, df = _inputs(rows, 64, len(lengths), torch.float32, 13)
+    _check(x, gate, off, h0 if initial else None, dh, df)
+
+
 @pytest.mark.parametrize("have", [(True, False), (False, True), (False, False)])
 def test_missing_gradients(cuda, have):
     off = _offsets([40, 0, 200])

@@ -113,6 +113,27 @@ def test_channels(cuda, c, groups, dtype):
     _check(x, off, groups, w, b, dy, "gelu", what=f"{c}/{groups}")
 
 
+@pytest.mark.parametrize("c,groups", [(80, 40), (80, 80), (8, 1), (264, 33)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_long_segments_with_many_groups(cuda, c, groups, dtype):
+    """Row tiles joined per 32 groups and up to 32 lanes, short and empty segments
+    between the long ones, spare rows on both ends (zeros)."""
+    lengths = [2600, 3, 0, 9000, 1, 0, 3100]
+    off = _offsets(lengths, first=7)
+    used = int(off[-1])
+    x, w, b, dy = _inputs(used + 500, c, dtype, 6)
+    y, dx = _check(x[:used], off, groups, w, b, dy[:used], "silu", what=f"{c}/{groups}")
+    for t in (y, dx):
+        assert torch.count_nonzero(t[:7]) == 0
+    from distributed_graph_flow_b200 import aggregation
+
+    wide = [t.cuda() for t in (x, off, w, b, dy)]
+    y2, mean, rstd = aggregation.segment_group_norm(wide[0], wide[1], groups, wide[2], wide[3], activation="silu")
+    dx2 = aggregation.segment_group_norm_backward(wide[4], wide[0], wide[1], mean, rstd, wide[2], wide[3],
+                                                  activation="silu")[0]
+    assert torch.count_nonzero(y2[used:]) == 0 and torch.count_nonzero(dx2[used:]) == 0
+
+
 def test_widest_rows(cuda):
     off = _offsets([3, 20])
     x, w, b, dy = _inputs(23, 2048, torch.bfloat16, 3)
