@@ -162,7 +162,7 @@ def dense_concat(x1, x2, weight, bias=None, relu: bool = True, out=None, stream=
     if bias is not None and (bias.dtype != torch.float32 or int(bias.numel()) != n):
         raise ValueError("dense_concat: bias must be float32 [N]")
     if out is None:
-        out = torch.empty((m, n), dtype=torch.bfloat16, device=x1.device)
+        out = x1.new_empty((m, n))
     _native.check(_native.lib().dgfx_dense_concat_bf16(
         _native.ptr(x1), k1, _native.ptr(x2), k2, m, _native.ptr(weight), _native.ptr(bias), n, int(bool(relu)),
         _native.ptr(out), _native.stream_handle(stream)))
@@ -507,7 +507,7 @@ def gated_dense_concat(x1, x2, w_gate, w_up, b_gate=None, b_up=None, activation:
         with guard:
             return gated_dense_concat(x1, x2, w_gate, w_up, b_gate, b_up, activation, out)
     if out is None:
-        out = torch.empty((m, n), dtype=torch.bfloat16, device=x1.device)
+        out = x1.new_empty((m, n))
     ptr = _native.ptr
     _native.check(_native.lib().dgfx_gated_dense_concat_bf16(
         ptr(x1), k1, ptr(x2), k2, m, ptr(w_gate), ptr(w_up), ptr(b_gate), ptr(b_up), n, act, ptr(out),
