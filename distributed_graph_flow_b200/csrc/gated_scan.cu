@@ -46,10 +46,10 @@
 // zeros and their inputs are never used.
 //
 // Measured (L2 flushed): 20,000 windows of Zipf lengths in 600,011 rows x 64
-// bf16 channels, forward 98 us, of which the apply kernel 55 (4.2 TB/s); 30,000
-// windows in 1,200,007 rows x 128 bf16, forward + backward 647 us (apply 200 and
+// bf16 channels, forward 100 us, of which the apply kernel 55 (4.2 TB/s); 30,000
+// windows in 1,200,007 rows x 128 bf16, forward + backward 650 us (apply 200 and
 // 350: 1.0 GB at 5 TB/s, 1.6 GB at 4.6); 3 series of 393,209 rows x 96 fp32, forward +
-// backward 363 us (apply 80 and 140 at 6.1 and 5.7 TB/s, chunk kernels 64 and 58: inside of long
+// backward 361 us (apply 80 and 140 at 6.1 and 5.7 TB/s, chunk kernels 64 and 58: inside of long
 // windows the inputs are read twice). What is left above HBM: the two special
 // functions and some sixty instructions per channel pair and row.
 #include <algorithm>
