@@ -154,6 +154,35 @@ def test_partial_gradients(cuda):
     assert all(torch.equal(p, q) for p, q in zip(full[:2] + full[4:], no_w[:2] + no_w[4:]))
 
 
+def test_rows_past_32_bits(cuda):
+    """More than 2^31 values of h and 2^32 of the projections' gradients: the
+    last rows (all others are zero). Operands and results are rounded to bf16
+    once each, 2^-8 of the sum of magnitudes per rounding: four of them."""
+    from distributed_graph_flow_b200 import aggregation
+
+    rows, tail, n = (1 << 22) + 77, 300, 512
+    x, dh = (torch.zeros((rows, w), dtype=torch.bfloat16, device="cuda") for w in (8, n))
+    x1, _, wg, wu, _, _, d = _inputs(tail, 8, 0, n, 17, bias=False)
+    x[-tail:], dh[-tail:] = x1.cuda(), d.cuda()
+    wg, wu = wg.cuda(), wu.cuda()
+    h = aggregation.gated_dense_concat(x, None, wg, wu)
+    dx, _, dwg, dwu, _, _ = aggregation.gated_dense_concat_backward(dh, x, None, wg, wu)
+    aggregation.dense_check()
+    assert torch.count_nonzero(h[:-tail]) == 0 and torch.count_nonzero(dx[:-tail]) == 0
+    xd, wgd, wud, dd = x1.double().cuda(), wg.double(), wu.double(), d.double().cuda()
+    g, u = xd @ wgd.t(), xd @ wud.t()
+    a, s = act64(g, "silu"), _slope64(g, "silu")
+    dg, du = dd * u * s, dd * a
+
+    def near(got, exp, magnitude, what):
+        assert_within(got, exp.cpu(), (4 * H * magnitude + 1e-6).cpu(), what)
+
+    near(h[-tail:], a * u, (a * u).abs(), "h")
+    near(dx[-tail:], dg @ wgd + du @ wud, dg.abs() @ wgd.abs() + du.abs() @ wud.abs(), "dx")
+    near(dwg, dg.t() @ xd, dg.abs().t() @ xd.abs(), "dw_gate")
+    near(dwu, du.t() @ xd, du.abs().t() @ xd.abs(), "dw_up")
+
+
 def test_no_rows(cuda):
     from distributed_graph_flow_b200 import aggregation
 
