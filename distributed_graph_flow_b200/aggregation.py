@@ -583,7 +583,7 @@ def segment_group_norm(x, offsets, groups: int, weight=None, bias=None, eps: flo
         with guard:
             return segment_group_norm(x, offsets, groups, weight, bias, eps, activation)
     y = torch.empty_like(x)
-    mean = torch.empty((nseg, groups), dtype=torch.float32, device=x.device)
+    mean = x.new_empty((nseg, groups), dtype=torch.float32)
     rstd = torch.empty_like(mean)
     ws = _layer_workspace(x.device, need) if need else None
     ptr = _native.ptr
@@ -655,7 +655,7 @@ def gated_scan(x, gate, offsets, initial=None, return_sequence: bool = True, ret
         with guard:
             return gated_scan(x, gate, offsets, initial, return_sequence, return_saved)
     h = torch.empty_like(x) if return_sequence else None
-    final = torch.empty((nseg, channels), dtype=torch.float32, device=x.device)
+    final = x.new_empty((nseg, channels), dtype=torch.float32)
     saved = torch.empty(saved_n, dtype=torch.float32, device=x.device) if return_saved else None
     ws = _layer_workspace(x.device, need)
     ptr = _native.ptr

@@ -805,15 +805,17 @@ int launch_nacc(int nacc, const Maps& maps, const Args& p, int units, cudaStream
 constexpr int kSms = 148;
 
 // Accumulator columns: no wider than the product needs, and the widest tile
-// that still gives every SM one: a narrow tile reads A more often but spreads
-// a small product over the SMs (K = N = 256, 1000 rows: 4.9 us at 64 columns, 5.7
-// at 128, 8.2 on pairs; 20,000 rows: 17.9, 12.5 and 12.5; 32 outputs of 200,000
-// rows, K = 128: 13.4, 16.9 and 23.9).
+// that still gives every pair of CTAs, or half of the single ones, a tile: a narrow
+// tile reads A more often but spreads a small product over the SMs (K = N = 256,
+// 1000 rows: 4.9 us at 64 columns, 5.7 at 128, 8.2 on pairs; 20,000 rows: 17.9,
+// 12.5 and 12.5; 32 outputs of 200,000 rows, K = 128: 13.4, 16.9 and 23.9). With
+// fewer than half of the SMs at 128 columns, 64 columns take one wave too; above
+// it they take two (4096 rows: 6.8 against 6.0 us).
 int pick_nacc(int64_t m, int64_t cols) {
   if (cols <= 64) return 64;
   if (cols <= 128) return ceil_div(m, kBM) >= kSms ? 128 : 64;
   if (ceil_div(m, 2 * kBM) * ceil_div(cols, 256) >= kSms / 2) return 256;
-  if (ceil_div(m, kBM) * ceil_div(cols, 128) >= kSms) return 128;
+  if (ceil_div(m, kBM) * ceil_div(cols, 128) >= kSms / 2) return 128;
   return 64;
 }
 
