@@ -477,7 +477,7 @@ __global__ void __maxnreg__(64) norm_forward_kernel(Params p) {
       }
       continue;
     }
-    const float inv = 1.0f / (static_cast<float>(n) * static_cast<float>(cg));
+    const float count = static_cast<float>(n) * static_cast<float>(cg), inv = 1.0f / count;
     float mu[kCh], rs[kCh], acc[1][kCh] = {};
     const Share sh(p, at, begin, end);
     const RowStats rst = row_stats<T, false>(p, sh);
@@ -485,11 +485,12 @@ __global__ void __maxnreg__(64) norm_forward_kernel(Params p) {
     for (int c = 0; c < kCh; ++c) acc[0][c] = rst.have * rst.mean[c];
     group_sums<1>(p, acc, at, t, p.team, bar, red, gsum);
     each_group(p, at, g0, [&](int c, int g) {
-      mu[c] = at.on ? gsum[g] * inv : 0.0f;
+      // A division: small segments of near values multiply the mean's rounding.
+      mu[c] = at.on ? gsum[g] / count : 0.0f;
       const float d = rst.have > 0.0f ? rst.mean[c] - mu[c] : 0.0f;
       acc[0][c] = rst.m2[c] + rst.have * d * d;
     });
-    for (int g = t; g < p.groups; g += p.team) p.mean[s * p.groups + g] = gsum[g] * inv;
+    for (int g = t; g < p.groups; g += p.team) p.mean[s * p.groups + g] = gsum[g] / count;
     // Its first barrier also ends the reads of gsum above.
     group_sums<1>(p, acc, at, t, p.team, bar, red, gsum);
     each_group(p, at, g0, [&](int c, int g) { rs[c] = at.on ? rsqrtf(gsum[g] * inv + p.eps) : 0.0f; });
@@ -721,7 +722,9 @@ __device__ __forceinline__ void grad_rows(const Params& p, const Share& sh, cons
     for (int c = 0; c < 2; ++c) {
       float2 xh, dz;
       grad_terms<ACT>(f.v[c], g.v[c], minus.v[c], r.v[c], w.v[c], b.v[c], &xh, &dz);
-      f.v[c] = mul2(r.v[c], fma2(xh, m2.v[c], add2(mul2(dz, w.v[c]), m1.v[c])));
+      // Scalar products: a packed one would be fused with the addition behind it.
+      const float2 wdz = make_float2(__fmul_rn(dz.x, w.v[c].x), __fmul_rn(dz.y, w.v[c].y));
+      f.v[c] = mul2(r.v[c], fma2(xh, m2.v[c], add2(wdz, m1.v[c])));
     }
     float o[kCh];
     f.to(o);

@@ -134,6 +134,19 @@ def test_long_segments_with_many_groups(cuda, c, groups, dtype):
     assert torch.count_nonzero(y2[used:]) == 0 and torch.count_nonzero(dx2[used:]) == 0
 
 
+def test_single_values_have_no_gradient(cuda):
+    """A segment and group of one value: its normalised value is zero and its
+    gradient exactly zero, however large rstd = 1 / sqrt(eps) is."""
+    from distributed_graph_flow_b200 import aggregation
+
+    x, w, b, dy = (t.cuda() for t in _inputs(200, 40, torch.float32, 5))
+    off = _offsets([1] * 200).cuda()
+    y, mean, rstd = aggregation.segment_group_norm(x, off, 40, w, b)
+    assert torch.equal(mean, x) and torch.equal(y, b.expand(200, 40))
+    dx, dw, _ = aggregation.segment_group_norm_backward(dy, x, off, mean, rstd, w, b)
+    assert torch.count_nonzero(dx) == 0 and torch.count_nonzero(dw) == 0
+
+
 def test_widest_rows(cuda):
     off = _offsets([3, 20])
     x, w, b, dy = _inputs(23, 2048, torch.bfloat16, 3)
