@@ -29,9 +29,9 @@
 // are never used.
 //
 // Measured (L2 flushed, forward + backward unless said): one segment of a
-// million rows x 256 bf16 channels, 16 groups, silu 778 us: x is read twice on the
-// way forward, x and dy twice on the way back, 4.1 GB in all, 5.3 TB/s; 300 ragged
-// segments in 250,001 rows x 200 fp32, gelu 366 us (1.6 GB); a merged batch of
+// million rows x 256 bf16 channels, 16 groups, silu 792 us: x is read twice on the
+// way forward, x and dy twice on the way back, 4.1 GB in all, 5.2 TB/s; 300 ragged
+// segments in 250,001 rows x 200 fp32, gelu 363 us (1.6 GB); a merged batch of
 // 1024 graphs, 41,003 rows x 256 bf16, relu, forward 37 us: one segment per team,
 // so the longest one's chain of loads and sums and the five launches are what it
 // takes.
