@@ -193,13 +193,30 @@ def sage_mean_gated(rowptr, col, x, w_gate, w_up, b_gate=None, b_up=None, activa
     """GraphSAGE-mean layer with a gated update: agg = mean over in-neighbours
     of x (as ``sage_mean_linear_relu``), then act(concat[x, agg] @ w_gate.T +
     b_gate) * (concat[x, agg] @ w_up.T + b_up) (``gated_dense_concat``). x bf16
-    [N, F], w_gate and w_up bf16 [N_out, 2F]."""
-    torch = _native.require_cuda()
-    n_rows = int(rowptr.numel()) - 1
+    [N, F], w_gate and w_up bf16 [N_out, 2F]; agg, if given, must not overlap x."""
+    who = "sage_mean_gated"
+    n_rows = rowptr.numel() - 1
+    nodes, feat = _layer_matrix(who, "x", x, torch.bfloat16)
+    if not 0 <= n_rows <= nodes:
+        raise ValueError(f"{who}: rowptr has {n_rows} rows, x {nodes}")
+    if agg is not None:
+        _layer_operand(who, "agg", agg, (n_rows, feat), torch.bfloat16)
+        _layer_apart(who, "agg", agg, x=x)
+    _gated_operands(who, x[:n_rows], x[:n_rows], w_gate, w_up, b_gate, b_up)  # agg is as large as x[:n_rows]
+    _activation_code(who, activation)
+    if out is not None:
+        _layer_operand(who, "out", out, (n_rows, w_gate.shape[0]), torch.bfloat16)
+    # Both steps under one guard: agg, the SpMM's workspace and the launches
+    # share one device and stream, so that memory freed here is not handed out
+    # while another stream's kernels still use it.
+    guard = _layer_guard(who, stream, x, rowptr, col, w_gate, w_up, b_gate, b_up, agg, workspace, out)
+    if guard is not None:
+        with guard:
+            return sage_mean_gated(rowptr, col, x, w_gate, w_up, b_gate, b_up, activation, agg, workspace, out)
     if agg is None:
-        agg = torch.empty((n_rows, int(x.shape[1])), dtype=torch.bfloat16, device=x.device)
-    csr_spmm(rowptr, col, x, normalize=True, out=agg, workspace=workspace, stream=stream)
-    return gated_dense_concat(x[:n_rows], agg, w_gate, w_up, b_gate, b_up, activation, out=out, stream=stream)
+        agg = x.new_empty((n_rows, feat))
+    csr_spmm(rowptr, col, x, normalize=True, out=agg, workspace=workspace)
+    return gated_dense_concat(x[:n_rows], agg, w_gate, w_up, b_gate, b_up, activation, out=out)
 
 
 # ---------------------------------------------------------------------------
