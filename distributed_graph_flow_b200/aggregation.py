@@ -38,6 +38,16 @@ def _dtype_code(t) -> int:
     raise ValueError(f"unsupported dtype {t}; expected float32 or bfloat16")
 
 
+def _temporary(shape, dtype, device, stream):
+    """Memory that only the kernels of a call on ``stream`` (None: the current
+    one) use: from that stream's pool, so that it is not handed out again
+    before they are done, however soon the call drops it."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
 def csr_spmm(rowptr, col, x, val=None, normalize: bool = False, out=None, out_dtype=None, num_rows: Optional[int] = None,
              workspace=None, stream=None):
     """Y[r] = scale_r * sum_j val_j * X[col_j] over CSR row r.
@@ -59,7 +69,7 @@ def csr_spmm(rowptr, col, x, val=None, normalize: bool = False, out=None, out_dt
     need = ctypes.c_size_t()
     _native.check(_native.lib().dgfx_spmm_workspace_size(R, nnz, F, ctypes.byref(need)))
     if workspace is None or workspace.numel() < need.value:
-        workspace = torch.empty(need.value, dtype=torch.uint8, device=x.device)
+        workspace = _temporary((need.value,), torch.uint8, x.device, stream)
     _native.check(
         _native.lib().dgfx_spmm_csr(
             _native.ptr(rowptr), _native.ptr(col), _native.ptr(val), R, int(x.shape[0]), nnz, _native.ptr(x),
@@ -180,10 +190,10 @@ def sage_mean_linear_relu(rowptr, col, x, weight, bias=None, agg=None, workspace
     nodes, col = source nodes) of x, then relu(concat[x, agg] @ weight.T +
     bias). x bf16 [N, F]; weight bf16 [N_out, 2F]. Two launches: the SpMM
     (HBM-bound gather, bf16 out) and the tensor-core dense layer."""
-    torch = _native.require_cuda()
+    _native.require_cuda()
     n_rows = int(rowptr.numel()) - 1
     if agg is None:
-        agg = torch.empty((n_rows, int(x.shape[1])), dtype=torch.bfloat16, device=x.device)
+        agg = _temporary((n_rows, int(x.shape[1])), torch.bfloat16, x.device, stream)
     csr_spmm(rowptr, col, x, normalize=True, out=agg, workspace=workspace, stream=stream)
     return dense_concat(x[:n_rows], agg, weight, bias, relu=True, out=out, stream=stream)
 

@@ -37,3 +37,27 @@ def test_gated_sage_layer_keeps_its_memory_on_its_stream(cuda):
         assert torch.equal(got, ref)
         del junk, got
     aggregation.dense_check()
+
+
+def test_mean_and_dense_layer_keep_their_memory_on_their_stream(cuda):
+    from distributed_graph_flow_b200 import aggregation
+
+    rows, feat = 60000, 128
+    g, rowptr, col = _graph(rows, 32, 2)
+    x = torch.randn((rows, feat), generator=g, device="cuda").bfloat16()
+    weight = (0.1 * torch.randn((64, 2 * feat), generator=g, device="cuda")).bfloat16()
+    ref = aggregation.csr_spmm(rowptr, col, x, normalize=True)
+    ref_layer = aggregation.sage_mean_linear_relu(rowptr, col, x, weight)
+    need = aggregation.spmm_workspace(rows, col.numel(), feat, "cuda").numel()
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        got = aggregation.csr_spmm(rowptr, col, x, normalize=True, stream=side)
+        layer = aggregation.sage_mean_linear_relu(rowptr, col, x, weight, stream=side)
+        junk = [torch.full((need,), 255, dtype=torch.uint8, device="cuda") for _ in range(2)]
+        junk.append(torch.full((rows, feat), float("nan"), dtype=torch.bfloat16, device="cuda"))
+        torch.cuda.synchronize()
+        assert torch.equal(got, ref) and torch.equal(layer, ref_layer)
+        del junk, got, layer
+    aggregation.dense_check()

@@ -85,3 +85,42 @@ def test_the_gated_sage_layer_refuses_a_mean_over_its_input(log):
     rowptr, col, x, wg, wu = _operands()
     with pytest.raises(ValueError, match="agg must not overlap x"):
         aggregation.sage_mean_gated(rowptr, col, x, wg, wu, agg=x[1:3])
+
+
+def test_temporaries_of_the_mean_come_from_the_streams_pool(monkeypatch):
+    """csr_spmm drops its workspace, and sage_mean_linear_relu its mean, while
+    the kernels may still run: both belong to the stream that runs them."""
+    current, made = [None], []
+
+    @contextlib.contextmanager
+    def stream_context(stream):
+        current.append(stream)
+        yield
+        current.pop()
+
+    class _Lib:
+        def dgfx_spmm_workspace_size(self, rows, nnz, feat, need):
+            need._obj.value = 4096
+            return 0
+
+        def dgfx_spmm_csr(self, *args):
+            return 0
+
+    empty = torch.empty
+
+    def recorded(shape, *args, **kw):
+        made.append((tuple(shape) if not isinstance(shape, int) else (shape,), current[-1]))
+        return empty(shape, *args, **kw)
+
+    monkeypatch.setattr(_native, "require_cuda", lambda: torch)
+    monkeypatch.setattr(_native, "lib", _Lib)
+    monkeypatch.setattr(torch.cuda, "stream", stream_context)
+    monkeypatch.setattr(torch, "empty", recorded)
+    monkeypatch.setattr(aggregation, "dense_concat", lambda x1, x2, *args, **kw: x2)
+    rowptr, col, x, weight, _ = _operands()
+    stream = _Stream()
+    aggregation.csr_spmm(rowptr, col, x, stream=stream)
+    assert made == [((2, 16), None), ((4096,), stream)]  # the result is the caller's
+    made.clear()
+    aggregation.sage_mean_linear_relu(rowptr, col, x, weight, stream=stream)
+    assert made == [((2, 16), stream), ((4096,), stream)]
