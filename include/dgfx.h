@@ -45,7 +45,10 @@ enum {
 
 enum { DGFX_F32 = 0, DGFX_BF16 = 1 };
 
-/* Activations of the layer operators. GELU is the exact (erf) form. */
+/* Activations of the layer operators. GELU is the exact (erf) form. They are
+ * computed in fp32 with the exponential and reciprocal intrinsics: relative
+ * errors below (1.3 |z| + 7) 2^-24 for the sigmoid (as for the gates of the
+ * recurrence), one unit more for silu, and (24 + 1.4 z^2) 2^-24 for gelu. */
 enum {
   DGFX_ACT_NONE = 0,
   DGFX_ACT_RELU = 1,
