@@ -190,12 +190,17 @@ def _like_or_none(t: Optional[torch.Tensor], like: torch.Tensor) -> torch.Tensor
     return like.new_empty(0) if t is None else t
 
 
+def _packed(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """A strided or expanded operand as the kernels read it."""
+    return None if t is None else t.contiguous()
+
+
 @torch.library.custom_op(f"{_LIB}::gated_dense_concat", mutates_args=())
 def gated_dense_concat(x1: torch.Tensor, x2: Optional[torch.Tensor], w_gate: torch.Tensor, w_up: torch.Tensor,
                        b_gate: Optional[torch.Tensor], b_up: Optional[torch.Tensor],
                        activation: str = "silu") -> torch.Tensor:
-    return aggregation.gated_dense_concat(x1.contiguous(), None if x2 is None else x2.contiguous(), w_gate.contiguous(),
-                                          w_up.contiguous(), b_gate, b_up, activation)
+    return aggregation.gated_dense_concat(x1.contiguous(), _packed(x2), w_gate.contiguous(), w_up.contiguous(),
+                                          _packed(b_gate), _packed(b_up), activation)
 
 
 @gated_dense_concat.register_fake
@@ -209,8 +214,8 @@ def gated_dense_concat_grad(grad: torch.Tensor, x1: torch.Tensor, x2: Optional[t
                             activation: str, need_input: bool, need_weight: bool) -> List[torch.Tensor]:
     """[dx1, dx2, dw_gate, dw_up, db_gate, db_up], empty where there is none."""
     grads = aggregation.gated_dense_concat_backward(
-        grad.contiguous(), x1.contiguous(), None if x2 is None else x2.contiguous(), w_gate.contiguous(),
-        w_up.contiguous(), b_gate, b_up, activation, need_input, need_weight)
+        grad.contiguous(), x1.contiguous(), _packed(x2), w_gate.contiguous(), w_up.contiguous(), _packed(b_gate),
+        _packed(b_up), activation, need_input, need_weight)
     return [_like_or_none(g, grad) for g in grads]
 
 
@@ -253,7 +258,8 @@ def sage_mean_gated(rowptr, col, x, w_gate, w_up, b_gate=None, b_up=None, activa
 def _segment_group_norm(x: torch.Tensor, offsets: torch.Tensor, groups: int, weight: Optional[torch.Tensor],
                         bias: Optional[torch.Tensor], eps: float,
                         activation: str) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    return aggregation.segment_group_norm(x.contiguous(), offsets.contiguous(), groups, weight, bias, eps, activation)
+    return aggregation.segment_group_norm(x.contiguous(), offsets.contiguous(), groups, _packed(weight), _packed(bias), eps,
+                                          activation)
 
 
 @_segment_group_norm.register_fake
@@ -268,7 +274,7 @@ def _segment_group_norm_grad(grad: torch.Tensor, x: torch.Tensor, offsets: torch
                              activation: str) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(dx, dweight, dbias), empty where there is no weight or bias."""
     dx, dw, db = aggregation.segment_group_norm_backward(grad.contiguous(), x.contiguous(), offsets.contiguous(), mean,
-                                                         rstd, weight, bias, activation)
+                                                         rstd, _packed(weight), _packed(bias), activation)
     return dx, _like_or_none(dw, mean), _like_or_none(db, mean)
 
 
@@ -319,7 +325,7 @@ def _gated_scan(x: torch.Tensor, gate: torch.Tensor, offsets: torch.Tensor, init
                 keep_states: bool) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(h, final, states for the backward pass: empty unless keep_states)."""
     out = aggregation.gated_scan(x.contiguous(), gate.contiguous(), offsets.contiguous(),
-                                 None if initial is None else initial.contiguous(), return_saved=keep_states)
+                                 _packed(initial), return_saved=keep_states)
     return out if keep_states else (*out, out[1].new_empty(0))
 
 
@@ -335,8 +341,8 @@ def _gated_scan_grad(grad: Optional[torch.Tensor], grad_final: Optional[torch.Te
                      initial: Optional[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(dx, dgate, dinitial), the last empty without initial."""
     dx, dgate, dinitial = aggregation.gated_scan_backward(
-        None if grad is None else grad.contiguous(), x.contiguous(), gate.contiguous(), offsets.contiguous(), saved,
-        None if initial is None else initial.contiguous(), None if grad_final is None else grad_final.contiguous())
+        _packed(grad), x.contiguous(), gate.contiguous(), offsets.contiguous(), saved, _packed(initial),
+        _packed(grad_final))
     return dx, dgate, _like_or_none(dinitial, saved)
 
 

@@ -83,3 +83,29 @@ def test_exact_ones(cuda, act):
     one = torch.ones_like(z)
     assert torch.equal(y, z if act == "none" else z.clamp_min(0))
     assert torch.equal(slope, one if act == "none" else (z > 0).double())
+
+
+def test_strided_parameters_through_the_torch_operators(cuda):
+    """Biases, weights and affine parameters strided or expanded: the values
+    and gradients of their packed copies."""
+    from distributed_graph_flow_b200 import torch_ops
+
+    g = torch.Generator(device="cuda").manual_seed(3)
+    off = torch.tensor([0, 30, 64], device="cuda")
+    x = torch.randn((64, 32), generator=g, device="cuda")
+    xb, w = x.bfloat16(), torch.randn((40, 32), generator=g, device="cuda").bfloat16()
+    long = torch.randn(80, generator=g, device="cuda")
+
+    def run(pack):
+        base = long.clone().requires_grad_(True)
+        one = torch.full((1,), 0.5, device="cuda", requires_grad=True)
+        strided, expanded, affine = base[::2], one.expand(40), base[1:64:2]
+        if pack:
+            strided, expanded, affine = strided.contiguous(), expanded.contiguous(), affine.contiguous()
+        h = torch.ops.dgfx.gated_dense_concat(xb, None, w, w, strided, expanded, "silu")
+        y = torch_ops.segment_group_norm(x, off, 4, affine, one.expand(32) if not pack else one.expand(32).contiguous(),
+                                         activation="silu")
+        (h.float().square().sum() + y.square().sum()).backward()
+        return h, y, base.grad, one.grad
+
+    assert all(torch.equal(p, q) for p, q in zip(run(False), run(True)))
