@@ -855,7 +855,6 @@ Plan make_plan(int64_t m, int64_t k1, int64_t k2, int64_t n) {
   pl.kb_split = static_cast<int>(ceil_div(kb, want));
   pl.splits = static_cast<int>(ceil_div(kb, pl.kb_split));
   pl.weight.units = pl.weight.n_tiles * pl.splits;
-  pl.weight.units_per_n = pl.splits;
   return pl;
 }
 

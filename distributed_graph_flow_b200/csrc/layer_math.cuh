@@ -134,7 +134,6 @@ template <class T>
 struct Vec16;
 template <>
 struct Vec16<float> {
-  static constexpr int N = 4;
   __device__ static __forceinline__ void unpack(const uint4& r, float (&f)[4]) {
     f[0] = __uint_as_float(r.x);
     f[1] = __uint_as_float(r.y);
@@ -147,7 +146,6 @@ struct Vec16<float> {
 };
 template <>
 struct Vec16<__nv_bfloat16> {
-  static constexpr int N = 8;
   __device__ static __forceinline__ void unpack(const uint4& r, float (&f)[8]) {
     const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
@@ -155,15 +153,6 @@ struct Vec16<__nv_bfloat16> {
       f[2 * q] = __uint_as_float(w[q] << 16);
       f[2 * q + 1] = __uint_as_float(w[q] & 0xFFFF0000u);
     }
-  }
-  __device__ static __forceinline__ uint4 pack(const float (&f)[8]) {
-    uint32_t w[4];
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * q], f[2 * q + 1]);
-      w[q] = *reinterpret_cast<const uint32_t*>(&h);
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
   }
 };
 

@@ -505,17 +505,14 @@ __global__ void __maxnreg__(64) norm_forward_kernel(Params p) {
 
 // One row tile of a listed segment.
 struct Tile {
-  int entry, count_tiles, first;
-  int64_t seg, begin, end, rows_of_seg;  // rows [begin, end)
+  int entry;
+  int64_t seg, begin, end;  // rows [begin, end)
   __device__ Tile(const Params& p, const LongList& all, int tile) {
     entry = find_long(p.long_base, all.count, tile);
-    first = p.long_base[entry];
-    count_tiles = (entry + 1 < all.count ? p.long_base[entry + 1] : all.tiles) - first;
     seg = p.long_seg[entry];
     const longlong2 span = p.long_span[entry];
-    const int64_t b = span.x, e = b + span.y;
-    rows_of_seg = span.y;
-    begin = b + static_cast<int64_t>(tile - first) * p.tile_rows;
+    const int64_t e = span.x + span.y;
+    begin = span.x + static_cast<int64_t>(tile - p.long_base[entry]) * p.tile_rows;
     end = begin + p.tile_rows < e ? begin + p.tile_rows : e;
   }
 };
