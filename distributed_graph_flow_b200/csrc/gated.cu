@@ -986,6 +986,9 @@ extern "C" int dgfx_gated_dense_concat_backward_bf16(const void* d_dh, const voi
   const Plan pl = make_plan(m, k1, k2, n);
   const Work ws = carve(d_workspace, workspace_bytes, pl, m, kk, n);
   if (d_workspace == nullptr || !ws.ok) return fail(DGFX_ERR_WORKSPACE, std::string(who) + ": workspace too small");
+  if (!ptr_aligned16(d_workspace)) {
+    return fail(DGFX_ERR_INVALID_ARGUMENT, std::string(who) + ": the workspace must be 16-byte aligned");
+  }
   unsigned int* err = dense_err_word();
   if (err == nullptr) return fail(DGFX_ERR_CUDA, std::string(who) + ": status word unavailable");
 

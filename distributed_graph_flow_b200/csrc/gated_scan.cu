@@ -828,6 +828,9 @@ extern "C" int dgfx_gated_scan(const void* d_x, const void* d_gate, int dtype, i
   if (rows > 0 && (d_workspace == nullptr || !ok)) {
     return fail(DGFX_ERR_WORKSPACE, "dgfx_gated_scan: workspace too small");
   }
+  if (rows > 0 && !ptr_aligned16(d_workspace)) {
+    return fail(DGFX_ERR_INVALID_ARGUMENT, "dgfx_gated_scan: the workspace must be 16-byte aligned");
+  }
   p.x = d_x;
   p.gate = d_gate;
   p.off = d_offsets;
@@ -861,6 +864,9 @@ extern "C" int dgfx_gated_scan_backward(const void* d_x, const void* d_gate, int
   carve(d_workspace, workspace_bytes, rows, channels, &p, &ok);
   if (rows > 0 && (d_workspace == nullptr || !ok)) {
     return fail(DGFX_ERR_WORKSPACE, "dgfx_gated_scan_backward: workspace too small");
+  }
+  if (rows > 0 && !ptr_aligned16(d_workspace)) {
+    return fail(DGFX_ERR_INVALID_ARGUMENT, "dgfx_gated_scan_backward: the workspace must be 16-byte aligned");
   }
   p.x = d_x;
   p.gate = d_gate;

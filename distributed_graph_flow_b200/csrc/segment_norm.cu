@@ -1051,6 +1051,9 @@ extern "C" int dgfx_segment_group_norm(const void* d_x, int dtype, int64_t rows,
   if (pl.longs) {
     w = carve(d_workspace, workspace_bytes, pl, channels, groups, false);
     if (d_workspace == nullptr || !w.ok) return fail(DGFX_ERR_WORKSPACE, "dgfx_segment_group_norm: workspace too small");
+    if (!ptr_aligned16(d_workspace)) {
+      return fail(DGFX_ERR_INVALID_ARGUMENT, "dgfx_segment_group_norm: the workspace must be 16-byte aligned");
+    }
   }
   Params p = make_params(pl, w, rows, channels, groups, nseg);
   p.x = d_x;
@@ -1086,6 +1089,9 @@ extern "C" int dgfx_segment_group_norm_backward(const void* d_dy, const void* d_
   const Work w = carve(d_workspace, workspace_bytes, pl, channels, groups, true);
   if (d_workspace == nullptr || !w.ok) {
     return fail(DGFX_ERR_WORKSPACE, "dgfx_segment_group_norm_backward: workspace too small");
+  }
+  if (!ptr_aligned16(d_workspace)) {
+    return fail(DGFX_ERR_INVALID_ARGUMENT, "dgfx_segment_group_norm_backward: the workspace must be 16-byte aligned");
   }
   Params p = make_params(pl, w, rows, channels, groups, nseg);
   p.x = d_x;

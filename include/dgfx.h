@@ -13,7 +13,8 @@
  *     status caster (dgf/src/util/status_caster.h:17-21, 83-88).
  *   - Work is enqueued on the caller's stream. Temporaries live in a
  *     caller-provided workspace whose size the matching *_workspace_size
- *     query returns; the library allocates no per-call device memory.
+ *     query returns; the library allocates no per-call device memory. The
+ *     layer operators refuse a workspace that is not 16-byte aligned.
  *   - No entry point falls back to a CPU implementation.
  */
 #ifndef DGFX_H_
