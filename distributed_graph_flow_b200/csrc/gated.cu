@@ -9,7 +9,10 @@
 //   dX = dg Wg + du Wu,  [dWg; dWu] = D^T X,  dbg, dbu = column sums.
 // D is rounded once, to be a matrix operand of the two products that follow;
 // the bias gradients are summed from its fp32 values before that. Products
-// accumulate in fp32.
+// accumulate in fp32. That rounding is as large as the results' own: dX and dW
+// are off by 2.3e-3 (2-norm, relative) instead of the 1.7e-3 of a single
+// rounding to bf16. Keeping D in two bf16 terms would double both products
+// (880 of 2090 us at the sizes below).
 //
 // One kernel body, four kinds of tile (128 rows by up to 256 accumulator
 // columns per CTA, K-blocks of 64):
@@ -38,10 +41,11 @@
 //
 // Bound by the tensor cores where there are many rows (K = 512: 4 M N K flop
 // against 2 M (K + N) bytes), at small ones by the chain of one tile. Measured at
-// 500,000 rows, K = 256 + 256, N = 512, silu: forward 385 us by itself (1.36
-// PFLOP/s), 485 us in a loop (1.08), where power holds the clock down; training
-// 2.2 ms in a loop: forward 385, kGates 550 (2 GB of X,
-// dh and D, for which HBM alone takes 310), kInput 412, kWeights 470, finish 5. Tiles of 128 x
+// 500,000 rows, K = 256 + 256, N = 512, silu: forward 380 us by itself (1.38
+// PFLOP/s), 465 to 505 us in a loop (1.04 to 1.13), where power holds the clock down; training
+// 2.1 to 2.25 ms in a loop, by the box. Its kernels by themselves, at the full clock, take
+// 1.8 ms: forward 380, kGates 550 (2 GB of X,
+// dh and D, for which HBM alone takes 310), kInput 412, kWeights 464, finish 5. Tiles of 128 x
 // 256 on single CTAs took 423, 779, 438 and 519. One row: 7 us.
 #include <algorithm>
 

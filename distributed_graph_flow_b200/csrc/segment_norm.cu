@@ -11,7 +11,8 @@
 //
 // Bound by HBM. A short segment (a sampled graph) is the work of a team of
 // threads: it reads the segment for the sums and again for the result, the second
-// time from L1. A team is the smallest power of two of threads (32 .. 512,
+// time from L1 as long as the segments of an SM's teams fit there (the average one does; the
+// largest that a team takes comes from L2). A team is the smallest power of two of threads (32 .. 512,
 // at least a row) that reads the average segment in a few steps, so many
 // small segments share a block. Segments of more than three to eight steps are
 // listed and go through three more kernels: the first reads row
@@ -29,12 +30,16 @@
 // are never used.
 //
 // Measured (L2 flushed, forward + backward unless said): one segment of a
-// million rows x 256 bf16 channels, 16 groups, silu 792 us: x is read twice on the
+// million rows x 256 bf16 channels, 16 groups, silu 784 us: x is read twice on the
 // way forward, x and dy twice on the way back, 4.1 GB in all, 5.2 TB/s; 300 ragged
-// segments in 250,001 rows x 200 fp32, gelu 363 us (1.6 GB); a merged batch of
+// segments in 250,001 rows x 200 fp32, gelu 375 us (1.6 GB); a merged batch of
 // 1024 graphs, 41,003 rows x 256 bf16, relu, forward 37 us: one segment per team,
 // so the longest one's chain of loads and sums and the five launches are what it
-// takes.
+// takes. Segments of a single row run far below HBM: a team's fixed work per segment
+// decides (a million rows x 64 bf16, one group: forward 1.26 ms, 0.2 TB/s; x 256
+// 2.26 ms, 0.45 TB/s). At its 80 registers norm_backward_kernel spills 56 to 100
+// bytes per thread with an activation in bf16 (8 without), 40 to 64 in fp32 (but for none
+// and relu); norm_forward_kernel spills 20 with gelu in bf16, the tile kernels up to 16.
 #include <algorithm>
 #include <string>
 
