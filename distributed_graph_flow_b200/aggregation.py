@@ -57,6 +57,9 @@ def csr_spmm(rowptr, col, x, val=None, normalize: bool = False, out=None, out_dt
     scale_r = 1 / max(deg_r, 1).
     """
     torch = _native.require_cuda()
+    if x.get_device() not in (-1, _native.current_device()):  # launches go to x's device
+        with torch.cuda.device(x.get_device()):
+            return csr_spmm(rowptr, col, x, val, normalize, out, out_dtype, num_rows, workspace, stream)
     R = int(rowptr.numel()) - 1 if num_rows is None else int(num_rows)
     nnz = int(col.numel())
     F = int(x.shape[1])

@@ -124,3 +124,39 @@ def test_temporaries_of_the_mean_come_from_the_streams_pool(monkeypatch):
     made.clear()
     aggregation.sage_mean_linear_relu(rowptr, col, x, weight, stream=stream)
     assert made == [((2, 16), stream), ((4096,), stream)]
+
+
+def test_the_mean_runs_on_the_device_of_its_operands(monkeypatch):
+    """Whatever device is the current one: its streams do not take the launches."""
+    device, launched = [0], []
+
+    class _Elsewhere(torch.Tensor):
+        def get_device(self):
+            return 1
+
+    @contextlib.contextmanager
+    def device_context(index):
+        device.append(index)
+        yield
+        device.pop()
+
+    class _Lib:
+        def dgfx_spmm_workspace_size(self, rows, nnz, feat, need):
+            need._obj.value = 64
+            return 0
+
+        def dgfx_spmm_csr(self, *args):
+            launched.append((device[-1], args[-1]))
+            return 0
+
+    monkeypatch.setattr(_native, "require_cuda", lambda: torch)
+    monkeypatch.setattr(_native, "lib", _Lib)
+    monkeypatch.setattr(_native, "current_device", lambda: device[-1])
+    monkeypatch.setattr(_native, "stream_handle", lambda stream=None: 100 + device[-1] if stream is None else stream.cuda_stream)
+    monkeypatch.setattr(torch.cuda, "device", device_context)
+    rowptr, col, x, _, _ = _operands()
+    aggregation.csr_spmm(rowptr, col, x)
+    there = torch.Tensor._make_subclass(_Elsewhere, x)
+    out = aggregation.csr_spmm(rowptr, col, there, None, True, None, torch.float32)
+    assert launched == [(0, 100), (1, 101)] and device == [0]
+    assert out.shape == (2, 16) and out.dtype == torch.float32
